@@ -119,7 +119,7 @@ def prepare(case, seed):
 
 # ---------------------------------------------------------------------------------------------------------------------------------------- the plain forms
 def _pack(x, signed):
-    """Codes (uint8, two's complement where signed) and scale bytes (e + 127; 255 marks a block with a non-finite entry) of an activation; padding columns are zero."""
+    """Codes (uint8, two's complement where signed) and scale bytes (e + 127; 255 marks a block with a non-finite entry, whose codes are 1) of an activation; padding columns are zero."""
     n, k = x.shape
     kb = (k + 31) // 32
     v = torch.zeros((n, 32 * kb), dtype=torch.float32, device=x.device)
@@ -132,7 +132,7 @@ def _pack(x, signed):
     e = torch.where(a > 0, (e - shift + (m > top).int()).clamp_min(-126), torch.full_like(e, -126))
     c = torch.round(torch.ldexp(v, -e[..., None]))
     c = c.clamp(-127, 127) if signed else torch.where(v > 0, c.clamp(1, 255), torch.zeros_like(c))
-    c = torch.where(bad[..., None], torch.zeros_like(c), c)
+    c = torch.where(bad[..., None], torch.ones_like(c), c)
     codes = c.to(torch.int8).view(torch.uint8) if signed else c.to(torch.uint8)
     return codes.view(n, 32 * kb), torch.where(bad, torch.full_like(e, 255), e + 127).to(torch.uint8)
 
@@ -161,8 +161,7 @@ def _plain(s):
     if op == "dense_backward":
         dz = s["dy"].float()
         if c["relu"]:
-            open_ = (s["y_codes"] > 0) | (s["y_scales"] == 255).repeat_interleave(32, 1)
-            dz = torch.where(open_[:, :c["o"]], dz, torch.zeros_like(dz))
+            dz = torch.where(s["y_codes"][:, :c["o"]] > 0, dz, torch.zeros_like(dz))
         x = _restore(s["x_codes"], s["x_scales"], c["k"], False)
         return {"dx": (dz @ s["w"].float()).to(t), "dw": (dz.t() @ x).to(t), "db": dz.sum(0).to(t)}
     rows = s["index"].repeat_interleave(c["per"]) if c["per"] > 1 else s["index"]
