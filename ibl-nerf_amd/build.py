@@ -18,7 +18,9 @@ OBJ = os.path.join(HERE, "build")
 LIB = os.path.join(HERE, "libiblnerf_hip.so")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 ARCH = "gfx950"
-COMMON = ["--offload-arch=" + ARCH, "-O3", "-std=c++17", "-fPIC", "-Wall", "-Wno-unused-function",
+# no packed fp32 instructions (v_pk_add / mul / fma_f32): some of their forms have given wrong results now and then; clang's host pass says that it does not know the
+# feature, which is harmless
+COMMON = ["--offload-arch=" + ARCH, "-O3", "-std=c++17", "-fPIC", "-Wall", "-Wno-unused-function", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
           "-I" + os.path.join(os.path.dirname(HERE), "include")]
 # (source, extra flags placed before -c[, object name]); every instantiation of the two MLP kernels is its own object
 # so that they compile side by side (each takes a minute or more)
