@@ -17,5 +17,13 @@ from .model import IBLNeRF, create_IBLNeRF, network_query_fn  # noqa: F401,E402
 from .export import render_decomp_path  # noqa: F401,E402
 from .renderer import Renderer, get_rays, render_decomp  # noqa: F401,E402
 
-__all__ = ["binding", "checkpoint", "config", "dataset", "dist", "export", "model", "renderer", "render_views", "render_decomp_path", "IBLNeRF", "create_IBLNeRF", "network_query_fn",
+__all__ = ["binding", "checkpoint", "config", "dataset", "dist", "export", "layers", "model", "renderer", "render_views", "render_decomp_path", "IBLNeRF", "create_IBLNeRF", "network_query_fn",
            "Renderer", "get_rays", "render_decomp"]
+
+
+def __getattr__(name):
+    """`layers` defines torch.autograd Functions and imports torch with them: loaded when it is first asked for (reading a config or a dataset needs no torch)."""
+    if name == "layers":
+        import importlib
+        return importlib.import_module(__name__ + ".layers")
+    raise AttributeError("module %r has no attribute %r" % (__name__, name))

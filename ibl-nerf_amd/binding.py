@@ -1,4 +1,4 @@
-"""ctypes binding of the C-ABI in include/iblnerf.h (libiblnerf_hip.so, built by build.py).
+"""ctypes binding of the C-ABI in include/iblnerf.h and include/iblnerf_layers.h (libiblnerf_hip.so, built by build.py).
 
 There is no CPU fallback: if the library is missing, or no HIP device is present, the compute
 entry points raise.  Nothing in this package imports oracle/.
@@ -27,6 +27,8 @@ EXPORTS = [
     "iblnerf_last_executed_flops", "iblnerf_estimate_policy", "iblnerf_ray_outputs_backward_gt", "iblnerf_ray_outputs_backward_rays", "iblnerf_coarse_z_rays", "iblnerf_aux_query", "iblnerf_aux_backward", "iblnerf_ray_outputs_backward_env", "iblnerf_set_select_tmin", "iblnerf_set_chunk_cuts",
     "iblnerf_decide_route", "iblnerf_set_route", "iblnerf_get_route", "iblnerf_copy_route", "iblnerf_describe_route", "iblnerf_last_slot_units", "iblnerf_trunk_density_fp32", "iblnerf_set_offset_tier_threshold",
     "iblnerf_escalate_route", "iblnerf_set_lists", "iblnerf_set_tapped_lists", "iblnerf_get_rays_strided", "iblnerf_get_rays_pixels", "iblnerf_set_tier_thresholds", "iblnerf_decide_route_outputs", "iblnerf_upload_weights_arch",
+    "iblnerf_layers_last_error", "iblnerf_checkpoint", "iblnerf_checkpoint_values", "iblnerf_dense_forward", "iblnerf_dense_backward_workspace", "iblnerf_dense_backward",
+    "iblnerf_lookup", "iblnerf_lookup_backward_workspace", "iblnerf_lookup_backward",
 ]
 
 
@@ -272,6 +274,22 @@ def load_library(path: str = LIB_PATH):
     lib.iblnerf_sample_pdf_u.restype = C.c_int
     lib.iblnerf_set_profiling.argtypes = [C.c_void_p, C.c_int]
     lib.iblnerf_last_mlp_time.argtypes = [C.c_void_p, C.POINTER(C.c_float), C.POINTER(C.c_int), C.POINTER(C.c_double)]
+    # include/iblnerf_layers.h
+    I, L = C.c_int, C.c_int64
+    lib.iblnerf_layers_last_error.argtypes = []
+    lib.iblnerf_layers_last_error.restype = C.c_char_p
+    lib.iblnerf_checkpoint.argtypes = [FP, I, FP, L, L, I, I, FP, FP]
+    lib.iblnerf_checkpoint_values.argtypes = [FP, FP, FP, L, I, I, I, FP, L]
+    lib.iblnerf_dense_forward.argtypes = [FP, I, FP, L, L, I, FP, L, I, FP, I, FP, L, FP, FP]
+    lib.iblnerf_dense_backward_workspace.argtypes = [I, L, I, I]
+    lib.iblnerf_dense_backward_workspace.restype = C.c_size_t
+    lib.iblnerf_dense_backward.argtypes = [FP, I, FP, L, L, I, I, FP, FP, I, FP, FP, L, FP, L, I, FP, FP, FP, C.c_size_t]
+    lib.iblnerf_lookup.argtypes = [FP, I, FP, L, L, I, FP, I, L, L, C.c_float, FP, L]
+    lib.iblnerf_lookup_backward_workspace.argtypes = [L, L, L, I]
+    lib.iblnerf_lookup_backward_workspace.restype = C.c_size_t
+    lib.iblnerf_lookup_backward.argtypes = [FP, I, FP, L, FP, I, L, L, L, I, C.c_float, FP, FP, C.c_size_t]
+    for n in ("iblnerf_checkpoint", "iblnerf_checkpoint_values", "iblnerf_dense_forward", "iblnerf_dense_backward", "iblnerf_lookup", "iblnerf_lookup_backward"):
+        getattr(lib, n).restype = C.c_int
     for n in ("iblnerf_create", "iblnerf_upload_weights", "iblnerf_upload_lut", "iblnerf_pack_weights_host",
               "iblnerf_get_rays", "iblnerf_network_query", "iblnerf_sample_pdf", "iblnerf_render_rays",
               "iblnerf_set_profiling", "iblnerf_last_mlp_time", "iblnerf_range_status", "iblnerf_pack_weights_host_mx"):
@@ -284,6 +302,12 @@ def default_options() -> Options:
     o = Options()
     load_library().iblnerf_default_options(C.byref(o))
     return o
+
+
+def check_layers(rc: int):
+    """A call of include/iblnerf_layers.h (no context: the message is the calling thread's)."""
+    if rc != 0:
+        raise IblNerfError("iblnerf status %d: %s" % (rc, (load_library().iblnerf_layers_last_error() or b"").decode()))
 
 
 def check(ctx, rc: int):

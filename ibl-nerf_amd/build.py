@@ -69,6 +69,9 @@ SOURCES = [
     ("trunk_fp32_kernel.hip", []),
     ("generic_mlp.hip", []),
     ("wgrad_kernel.hip", []),
+    ("dense_kernel.hip", []),
+    ("lookup_kernel.hip", []),
+    ("layers_api.cpp", ["-x", "hip"]),
     ("api.cpp", ["-x", "hip"]),
     ("pack.cpp", ["-x", "hip"]),
 ]

@@ -1,0 +1,408 @@
+// Table rows by index with a scale (a code for the view of each ray), and the table's gradient by sorted tokens.
+//
+//   out[p][c] = scale * table[index[p / per]][c]            d table[t][c] = scale * sum over the rows p with index[p / per] = t of dOut[p][c]
+//
+// A negative index is a row without a code: zeros, no gradient.  An index beyond the table reads NaN (a wrong index shows) and has no gradient.
+//
+// The gradient is bound by reading dOut once, in an order that the tokens set.  The positions are sorted by token (stable, so a token's rows keep their order), the sorted
+// rows are cut into pieces of equal length — a token that most rows share (a batch drawn from few views) costs no more than any other — and each piece adds up its
+// runs of equal tokens in 32 bits.  A run inside one piece is finished there; the pieces of a longer run are joined in order by k_lookup_join.  No atomics on
+// values: the same inputs give the same bits.
+#include "layer_elems.h"
+#include "layers.h"
+
+namespace ibl {
+
+namespace {
+
+constexpr int SMALL = 4096;          // positions that one workgroup sorts in LDS
+constexpr int TILE = 4096;           // positions a workgroup of the large sort takes
+constexpr int BINS = 512;            // at most 9 bits a pass
+
+__device__ __forceinline__ long index_at(const void* index, int index64, long i) {
+    return index64 ? static_cast<const long long*>(index)[i] : (long)static_cast<const int*>(index)[i];
+}
+// a position's sort key: its token, or v (behind all tokens) where it has none
+__device__ __forceinline__ unsigned key_at(const LookupGrad& a, long i) {
+    const long t = index_at(a.index, a.index64, i);
+    return t >= 0 && t < a.v ? (unsigned)t : (unsigned)a.v;
+}
+
+// thread `t` of `threads` clears its share of a table of 2- or 4-byte elements
+__device__ __forceinline__ void clear(void* table, size_t bytes, size_t t, size_t threads) {
+    size_t whole = 0;
+    if ((reinterpret_cast<uintptr_t>(table) & 15) == 0) {
+        whole = bytes / 16;
+        for (size_t i = t; i < whole; i += threads) static_cast<u32x4*>(table)[i] = u32x4{0, 0, 0, 0};
+    }
+    for (size_t i = 8 * whole + t; i < bytes / 2; i += threads) static_cast<unsigned short*>(table)[i] = 0;
+}
+
+template <int T> __global__ __launch_bounds__(256) void k_lookup(Lookup a) {
+    const int cpr = (a.d + 7) >> 3;
+    const long total = a.n * a.per * cpr;
+    for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long)gridDim.x * 256) {
+        const long row = i / cpr;
+        const int c = 8 * (int)(i - row * cpr);
+        const long t = index_at(a.index, a.index64, a.per == 1 ? row : row / a.per);
+        float f[8];
+        if (t >= 0 && t < a.v) {
+            to_floats<T>(load8<T>(static_cast<const char*>(a.table) + t * a.ld_table * Bytes<T>::v, c, a.d), f);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) f[e] *= a.scale;
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) f[e] = t < 0 ? 0.0f : __builtin_nanf("");
+        }
+        store8<T>(static_cast<char*>(a.out) + row * a.ld_out * Bytes<T>::v, c, a.d, from_floats<T>(f));
+    }
+}
+
+// ------------------------------------------------------------------------------------------------------------------------------------------------ sorting
+// Lanes of the wave whose digit equals this lane's (only lanes with `in` count)
+__device__ __forceinline__ unsigned long long peers(unsigned digit, int bits, bool in) {
+    unsigned long long m = __ballot(in);
+    for (int b = 0; b < bits; ++b) {
+        const bool one = (digit >> b) & 1;
+        const unsigned long long v = __ballot(one);
+        m &= one ? v : ~v;
+    }
+    return m;
+}
+
+// One stable pass over `rounds` x 64 keys of each wave: the key's rank among the wave's keys of the same digit, the wave's digit counts in hist[wave][BINS]
+template <int WAVES> __device__ __forceinline__ unsigned rank_in_wave(unsigned digit, int bits, bool in, unsigned* hist, int wave, int lane) {
+    const unsigned long long m = peers(digit, bits, in);
+    unsigned before = 0;
+    if (in) before = hist[wave * BINS + digit];
+    const unsigned lower = __popcll(m & ((1ull << lane) - 1));
+    __builtin_amdgcn_wave_barrier();
+    if (in && lower == 0) hist[wave * BINS + digit] = before + (unsigned)__popcll(m);
+    __builtin_amdgcn_wave_barrier();
+    return before + lower;
+}
+
+// up to SMALL positions, all passes in one workgroup of 16 waves; wave w holds positions 256 w .. 256 w + 255
+__global__ __launch_bounds__(1024) void k_sort_small(LookupGrad a, int passes, int bits, unsigned* keys, unsigned* pos, size_t zero_bytes) {
+    __shared__ unsigned lk[SMALL], lp[SMALL];
+    __shared__ unsigned hist[16 * BINS];
+    __shared__ unsigned base[BINS];
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, n = (int)a.n;
+    clear(a.dtable, zero_bytes, t, 1024);
+    for (int i = t; i < n; i += 1024) { lk[i] = key_at(a, i); lp[i] = (unsigned)i; }
+    __syncthreads();
+    for (int pass = 0; pass < passes; ++pass) {
+        const int shift = pass * bits;
+        const unsigned mask = (1u << bits) - 1;
+        for (int i = t; i < 16 * BINS; i += 1024) hist[i] = 0;
+        __syncthreads();
+        unsigned k[4], p[4], r[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int i = 256 * wave + 64 * q + lane;
+            const bool in = i < n;
+            k[q] = in ? lk[i] : 0;
+            p[q] = in ? lp[i] : 0;
+            r[q] = rank_in_wave<16>((k[q] >> shift) & mask, bits, in, hist, wave, lane);
+        }
+        __syncthreads();
+        // the waves' counts of a digit become exclusive sums; base = the digit's total
+        if (t < BINS) {
+            unsigned s = 0;
+#pragma unroll
+            for (int w = 0; w < 16; ++w) { const unsigned h = hist[w * BINS + t]; hist[w * BINS + t] = s; s += h; }
+            base[t] = s;
+        }
+        __syncthreads();
+        if (t < 64) {      // exclusive sums over the digits, 8 a lane
+            unsigned v[BINS / 64], s = 0;
+#pragma unroll
+            for (int q = 0; q < BINS / 64; ++q) { v[q] = base[t * (BINS / 64) + q]; s += v[q]; }
+            unsigned x = s;
+#pragma unroll
+            for (int m = 1; m < 64; m <<= 1) { const unsigned y = __shfl_up(x, m); if (lane >= m) x += y; }
+            x -= s;
+#pragma unroll
+            for (int q = 0; q < BINS / 64; ++q) { base[t * (BINS / 64) + q] = x; x += v[q]; }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int i = 256 * wave + 64 * q + lane;
+            if (i < n) {
+                const unsigned dg = (k[q] >> shift) & mask, at = base[dg] + hist[wave * BINS + dg] + r[q];
+                lk[at] = k[q];
+                lp[at] = p[q];
+            }
+        }
+        __syncthreads();
+    }
+    for (int i = t; i < n; i += 1024) { keys[i] = lk[i]; pos[i] = lp[i]; }
+}
+
+// Large sort, one pass = three launches: digit counts of each tile, their exclusive sums along the tiles (one workgroup a digit), the scatter.
+// The first pass reads the caller's index; its counting launch also clears the gradient table (tokens that no row has keep zero).
+__global__ __launch_bounds__(256) void k_sort_count(LookupGrad a, const unsigned* keys, int shift, int bits, unsigned* counts, size_t zero_bytes) {
+    __shared__ unsigned hist[BINS];
+    clear(a.dtable, zero_bytes, (size_t)blockIdx.x * 256 + threadIdx.x, (size_t)gridDim.x * 256);
+    for (int i = threadIdx.x; i < BINS; i += 256) hist[i] = 0;
+    __syncthreads();
+    const long i0 = (long)blockIdx.x * TILE;
+    for (int q = threadIdx.x; q < TILE; q += 256)
+        if (i0 + q < a.n) atomicAdd(&hist[((keys ? keys[i0 + q] : key_at(a, i0 + q)) >> shift) & ((1u << bits) - 1)], 1u);
+    __syncthreads();
+    for (int i = threadIdx.x; i < (1 << bits); i += 256) counts[(size_t)i * gridDim.x + blockIdx.x] = hist[i];
+}
+
+__global__ __launch_bounds__(256) void k_sort_scan(unsigned* counts, int tiles, unsigned* totals) {
+    __shared__ unsigned part[4];
+    unsigned* row = counts + (size_t)blockIdx.x * tiles;
+    const int t = threadIdx.x, lane = t & 63;
+    unsigned carry = 0;
+    for (int i0 = 0; i0 < tiles; i0 += 256) {
+        const unsigned v = i0 + t < tiles ? row[i0 + t] : 0;
+        unsigned x = v;
+#pragma unroll
+        for (int m = 1; m < 64; m <<= 1) { const unsigned y = __shfl_up(x, m); if (lane >= m) x += y; }
+        if (lane == 63) part[t >> 6] = x;
+        __syncthreads();
+        unsigned before = carry, all = 0;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) { if (w < (t >> 6)) before += part[w]; all += part[w]; }
+        if (i0 + t < tiles) row[i0 + t] = before + x - v;
+        carry += all;
+        __syncthreads();
+    }
+    if (t == 0) totals[blockIdx.x] = carry;
+}
+
+__global__ __launch_bounds__(256) void k_sort_scatter(LookupGrad a, const unsigned* keys, const unsigned* pos, int shift, int bits, const unsigned* counts, const unsigned* totals,
+                                                      unsigned* keys_out, unsigned* pos_out) {
+    __shared__ unsigned hist[4 * BINS];
+    __shared__ unsigned base[BINS];
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, bins = 1 << bits;
+    for (int i = t; i < 4 * BINS; i += 256) hist[i] = 0;
+    for (int i = t; i < BINS; i += 256) base[i] = i < bins ? totals[i] : 0;
+    __syncthreads();
+    if (t < 64) {
+        unsigned v[BINS / 64], s = 0;
+#pragma unroll
+        for (int q = 0; q < BINS / 64; ++q) { v[q] = base[t * (BINS / 64) + q]; s += v[q]; }
+        unsigned x = s;
+#pragma unroll
+        for (int m = 1; m < 64; m <<= 1) { const unsigned y = __shfl_up(x, m); if (lane >= m) x += y; }
+        x -= s;
+#pragma unroll
+        for (int q = 0; q < BINS / 64; ++q) { base[t * (BINS / 64) + q] = x; x += v[q]; }
+    }
+    const long i0 = (long)blockIdx.x * TILE + (long)wave * (TILE / 4);
+    unsigned k[16], p[16], r[16];
+#pragma unroll
+    for (int q = 0; q < 16; ++q) {
+        const long i = i0 + 64 * q + lane;
+        const bool in = i < a.n;
+        k[q] = in ? (keys ? keys[i] : key_at(a, i)) : 0;
+        p[q] = in ? (pos ? pos[i] : (unsigned)i) : 0;
+    }
+#pragma unroll
+    for (int q = 0; q < 16; ++q) r[q] = rank_in_wave<4>((k[q] >> shift) & (bins - 1), bits, i0 + 64 * q + lane < a.n, hist, wave, lane);
+    __syncthreads();
+    for (int i = t; i < bins; i += 256) {
+        unsigned s = base[i] + counts[(size_t)i * gridDim.x + blockIdx.x];
+#pragma unroll
+        for (int w = 0; w < 4; ++w) { const unsigned h = hist[w * BINS + i]; hist[w * BINS + i] = s; s += h; }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < 16; ++q)
+        if (i0 + 64 * q + lane < a.n) {
+            const unsigned at = hist[wave * BINS + ((k[q] >> shift) & (bins - 1))] + r[q];
+            keys_out[at] = k[q];
+            pos_out[at] = p[q];
+        }
+}
+
+// ------------------------------------------------------------------------------------------------------------------------------------------------ summing
+template <int T> __device__ __forceinline__ void put_sum(const LookupGrad& a, unsigned token, int c, const float (&s)[8]) {
+    float f[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = s[e] * a.scale;
+    store8<T>(static_cast<char*>(a.dtable) + (size_t)token * a.d * Bytes<T>::v, c, a.d, from_floats<T>(f));
+}
+
+// A thread = 8 columns of one piece: sorted rows [piece * len, piece * len + len), sorted row i = row i % per of the entry i / per.  part [pieces][2][8 cpr]: the sum of the
+// run that comes in from the piece before (0) and of the run that goes on into the next (1).
+template <int T> __global__ __launch_bounds__(256) void k_lookup_sum(LookupGrad a, const unsigned* keys, const unsigned* pos, long pieces, int len, float* part) {
+    constexpr int U = 8;      // rows in flight
+    const int cpr = (a.d + 7) >> 3;
+    const long id = (long)blockIdx.x * 256 + threadIdx.x;
+    const long piece = id / cpr;
+    if (piece >= pieces) return;
+    const int c = 8 * (int)(id - piece * cpr);
+    const long rows = a.n * a.per, i0 = piece * len, i1 = i0 + len < rows ? i0 + len : rows;
+    const unsigned none = (unsigned)a.v;
+    float* out = part + (size_t)piece * 2 * 8 * cpr + c;
+    auto keep = [&](int which, const float (&s)[8]) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) out[which * 8 * cpr + e] = s[e];
+    };
+    unsigned cur = keys[i0 / a.per];
+    bool coming = i0 > 0 && keys[(i0 - 1) / a.per] == cur;
+    float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    for (long i = i0; i < i1; i += U) {
+        unsigned k[U];
+        Raw8<T> v[U];
+        long e = i / a.per, q = i - e * a.per;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const bool in = i + u < i1;
+            k[u] = in ? keys[e] : none;
+            v[u] = in && k[u] != none ? load8<T>(static_cast<const char*>(a.dout) + ((long)pos[e] * a.per + q) * a.ld_dout * Bytes<T>::v, c, a.d) : zero8<T>();
+            if (++q == a.per) { q = 0; ++e; }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (i + u < i1 && k[u] != cur) {
+                if (coming) keep(0, s);
+                else if (cur != none) put_sum<T>(a, cur, c, s);
+                coming = false;
+                cur = k[u];
+#pragma unroll
+                for (int x = 0; x < 8; ++x) s[x] = 0.0f;
+            }
+            float f[8];
+            to_floats<T>(v[u], f);
+#pragma unroll
+            for (int x = 0; x < 8; ++x) s[x] += f[x];
+        }
+    }
+    if (cur == none) return;
+    if (coming) keep(0, s);
+    else if (i1 < rows && keys[i1 / a.per] == cur) keep(1, s);
+    else put_sum<T>(a, cur, c, s);
+}
+
+// One workgroup a piece: if a run begins in it and goes on, the run's partial sums — its own and those of the pieces it comes into — are added up: each thread a column and
+// every G-th piece, then the G sums in order.
+template <int T> __global__ __launch_bounds__(256) void k_lookup_join(LookupGrad a, const unsigned* keys, long pieces, int len, const float* part) {
+    __shared__ float sums[256];
+    const long piece = blockIdx.x, rows = a.n * a.per, i0 = piece * len, i1 = i0 + len;
+    if (i1 >= rows) return;
+    const unsigned tok = keys[(i1 - 1) / a.per];
+    if (tok == (unsigned)a.v || keys[i1 / a.per] != tok) return;
+    if (i0 > 0 && keys[(i0 - 1) / a.per] == tok) return;      // the run began in an earlier piece
+    long lo = i1 / a.per, hi = a.n;                           // first entry behind the run
+    while (lo < hi) {
+        const long m = (lo + hi) >> 1;
+        if (keys[m] <= tok) lo = m + 1; else hi = m;
+    }
+    const long more = (lo * a.per - 1) / len - piece;         // pieces that the run comes into
+    const int w = 8 * ((a.d + 7) >> 3);
+    const float* first = part + (size_t)piece * 2 * w;
+    for (int c0 = 0; c0 < a.d; c0 += 256) {
+        const int cols = a.d - c0 < 256 ? a.d - c0 : 256, g = 256 / cols;
+        const int c = threadIdx.x % cols, y = threadIdx.x / cols;
+        float s = 0.0f;
+        if (y < g) {
+            if (y == 0) s = first[w + c0 + c];
+            const float* p = first + 2 * w + c0 + c;
+#pragma unroll 4
+            for (long q = y; q < more; q += g) s += p[(size_t)q * 2 * w];
+        }
+        sums[threadIdx.x] = s;
+        __syncthreads();
+        if (threadIdx.x < cols) {
+            float r = 0.0f;
+            for (int q = 0; q < g; ++q) r += sums[q * cols + threadIdx.x];
+            r *= a.scale;
+            const size_t at = (size_t)tok * a.d + c0 + threadIdx.x;
+            if constexpr (T == LT_F32) static_cast<float*>(a.dtable)[at] = r;
+            else static_cast<unsigned short*>(a.dtable)[at] = (unsigned short)pack2<T>(r, 0.0f);
+        }
+        __syncthreads();
+    }
+}
+
+__global__ __launch_bounds__(256) void k_clear(void* table, size_t bytes) { clear(table, bytes, (size_t)blockIdx.x * 256 + threadIdx.x, (size_t)gridDim.x * 256); }
+
+struct Plan {
+    long rows, pieces;
+    int len, passes, bits, tiles;
+    size_t keys, pos, keys2, pos2, counts, totals, part, bytes;      // offsets into the workspace
+};
+
+Plan plan(long n, long per, long v, int d) {
+    Plan p;
+    p.rows = n * per;
+    // pieces: enough threads (a thread = 8 columns of a piece) to fill the chip's 256 x 4 SIMDs a few waves deep; 16 rows at least, so that partial sums stay few
+    const long cpr = (d + 7) / 8;
+    long len = (p.rows * cpr + 131071) / 131072;
+    len = len < 16 ? 16 : len > 256 ? 256 : (len + 7) & ~7L;
+    p.len = (int)len;
+    p.pieces = (p.rows + len - 1) / len;
+    int all = 1;
+    while ((v >> all) != 0) ++all;               // keys are 0 .. v
+    p.passes = (all + 8) / 9;
+    p.bits = (all + p.passes - 1) / p.passes;
+    p.tiles = n > SMALL ? (int)((n + TILE - 1) / TILE) : 0;
+    size_t at = 0;
+    auto take = [&](size_t bytes) { const size_t was = at; at += (bytes + 255) & ~(size_t)255; return was; };
+    p.keys = take((size_t)n * 4);
+    p.pos = take((size_t)n * 4);
+    p.keys2 = take(p.tiles ? (size_t)n * 4 : 0);
+    p.pos2 = take(p.tiles ? (size_t)n * 4 : 0);
+    p.counts = take((size_t)p.tiles << (p.bits + 2));
+    p.totals = take(BINS * 4);
+    p.part = take((size_t)p.pieces * 2 * 8 * cpr * 4);
+    p.bytes = at;
+    return p;
+}
+
+template <int T> hipError_t lookup_backward(const LookupGrad& a, hipStream_t s) {
+    const Plan p = plan(a.n, a.per, a.v, a.d);
+    char* ws = static_cast<char*>(a.ws);
+    auto u = [&](size_t at) { return reinterpret_cast<unsigned*>(ws + at); };
+    const size_t zero = (size_t)a.v * a.d * Bytes<T>::v;
+    if (a.n == 0 || p.tiles == 0) {
+        // a table of up to 64 KB is cleared by the sorting workgroup, a larger one by a launch of its own
+        const bool own = a.n > 0 && zero <= 65536;
+        if (!own) hipLaunchKernelGGL(k_clear, dim3((unsigned)(zero / 4096 < 4095 ? zero / 4096 + 1 : 4096)), dim3(256), 0, s, a.dtable, zero);
+        if (a.n == 0) return hipGetLastError();
+        hipLaunchKernelGGL(k_sort_small, dim3(1), dim3(1024), 0, s, a, p.passes, p.bits, u(p.keys), u(p.pos), own ? zero : 0);
+    } else {
+        const unsigned *kin = nullptr, *pin = nullptr;
+        for (int pass = 0; pass < p.passes; ++pass) {
+            const bool to2 = ((p.passes - 1 - pass) & 1) != 0;      // the last pass ends in keys / pos
+            unsigned *ko = u(to2 ? p.keys2 : p.keys), *po = u(to2 ? p.pos2 : p.pos);
+            hipLaunchKernelGGL(k_sort_count, dim3(p.tiles), dim3(256), 0, s, a, kin, pass * p.bits, p.bits, u(p.counts), pass == 0 ? zero : 0);
+            hipLaunchKernelGGL(k_sort_scan, dim3(1u << p.bits), dim3(256), 0, s, u(p.counts), p.tiles, u(p.totals));
+            hipLaunchKernelGGL(k_sort_scatter, dim3(p.tiles), dim3(256), 0, s, a, kin, pin, pass * p.bits, p.bits, u(p.counts), u(p.totals), ko, po);
+            kin = ko;
+            pin = po;
+        }
+    }
+    const long threads = p.pieces * ((a.d + 7) / 8);
+    float* part = reinterpret_cast<float*>(ws + p.part);
+    hipLaunchKernelGGL((k_lookup_sum<T>), dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, s, a, u(p.keys), u(p.pos), p.pieces, p.len, part);
+    if (p.pieces > 1) hipLaunchKernelGGL((k_lookup_join<T>), dim3((unsigned)p.pieces), dim3(256), 0, s, a, u(p.keys), p.pieces, p.len, part);
+    return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t launch_lookup(int type, const Lookup& a, hipStream_t s) {
+    const long blocks = (a.n * a.per * ((a.d + 7) / 8) + 255) / 256;
+    const dim3 g((unsigned)(blocks < 16384 ? blocks : 16384)), b(256);
+    if (type == LT_F32) hipLaunchKernelGGL((k_lookup<LT_F32>), g, b, 0, s, a);
+    else if (type == LT_BF16) hipLaunchKernelGGL((k_lookup<LT_BF16>), g, b, 0, s, a);
+    else hipLaunchKernelGGL((k_lookup<LT_F16>), g, b, 0, s, a);
+    return hipGetLastError();
+}
+
+size_t lookup_backward_bytes(long n, long per, long v, int d) { return plan(n, per, v, d).bytes; }
+
+hipError_t launch_lookup_backward(int type, const LookupGrad& a, hipStream_t s) {
+    return type == LT_F32 ? lookup_backward<LT_F32>(a, s) : type == LT_BF16 ? lookup_backward<LT_BF16>(a, s) : lookup_backward<LT_F16>(a, s);
+}
+
+}  // namespace ibl

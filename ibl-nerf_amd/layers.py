@@ -1,0 +1,275 @@
+"""Trainable layers on hand-written kernels: dense layers whose backward pass reads 8-bit checkpoints of their activations, and rows of a table by index (a code for the view
+of each ray) with the table's gradient by sorted tokens.  include/iblnerf_layers.h is the C boundary; csrc/dense_kernel.hip and csrc/lookup_kernel.hip say what bounds
+them.
+
+They train what the fused backward (training.py) is not built for: networks outside the 8 x 256 shape, layer by layer (`network_forward` below,
+model.fused_network_query, training.render_rays_train).
+
+    y, kept = dense(x, weight, bias, relu=True)        autograd; keeps 1.03 bytes an activation instead of x and y
+    y, kept = dense(y, weight2, bias2, kept=kept)      the next layer reads the checkpoint that the first has written
+    rows = lookup(codes, view, scale)                  autograd
+
+Tensors are float32, bfloat16 or float16 on one GPU; rows may be strided, what lies along a row is contiguous (anything else is copied).  Calls run on the current stream of the
+tensors' device and never synchronise."""
+from __future__ import annotations
+
+import contextlib
+
+import torch
+
+from . import binding as B
+
+_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+MAX_COLUMNS = 65536
+
+
+def _type(t, what):
+    code = _TYPES.get(t.dtype)
+    if code is None:
+        raise TypeError("%s must be float32, bfloat16 or float16, got %s" % (what, t.dtype))
+    return code
+
+
+def _on(t):
+    """(library, stream, guard): the tensor's device made current for the call where it is not."""
+    if not t.is_cuda:
+        raise B.IblNerfError("the layer operators have no CPU path: got a tensor on %s" % t.device)
+    lib, dev = B.load_library(), t.device.index
+    guard = contextlib.nullcontext() if dev == torch.cuda.current_device() else torch.cuda.device(dev)
+    return lib, torch.cuda.current_stream(dev).cuda_stream, guard
+
+
+def _same(t, like, what, dtype=None):
+    if t.device != like.device:
+        raise ValueError("%s is on %s, the call's other tensors on %s" % (what, t.device, like.device))
+    if dtype is not None and t.dtype != dtype:
+        raise TypeError("%s must be %s, got %s" % (what, dtype, t.dtype))
+
+
+def _rows(t, what):
+    """t [..., k] as [n, k] with unit stride along a row and its row stride in elements."""
+    if t.dim() < 1 or not 1 <= t.shape[-1] <= MAX_COLUMNS:
+        raise ValueError("%s must be [..., k] with 1 <= k <= %d, got %s" % (what, MAX_COLUMNS, tuple(t.shape)))
+    k = t.shape[-1]
+    if t.dim() != 2:
+        t = t.reshape(-1, k) if t.numel() else t.new_empty((0, k))
+    if (k > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < k):
+        t = t.contiguous()
+    return t, (t.stride(0) if t.shape[0] > 1 else k)
+
+
+class Checkpoint:
+    """An activation [n, columns] in 8 bits: `codes` [n, 32 ceil(columns / 32)] uint8 and `scales` [n, ceil(columns / 32)] uint8 (include/iblnerf_layers.h has the format).
+    `signed`: two's-complement codes; unsigned ones come from a ReLU."""
+
+    __slots__ = ("codes", "scales", "columns", "signed")
+
+    def __init__(self, codes, scales, columns, signed=False):
+        blocks = (int(columns) + 31) // 32
+        if codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
+            raise TypeError("a checkpoint's codes and scales are uint8, got %s and %s" % (codes.dtype, scales.dtype))
+        if columns < 1 or codes.dim() != 2 or tuple(codes.shape) != (scales.shape[0], 32 * blocks) or tuple(scales.shape) != (codes.shape[0], blocks):
+            raise ValueError("a checkpoint of %d columns has codes [n, %d] and scales [n, %d], got %s and %s" % (columns, 32 * blocks, blocks, tuple(codes.shape), tuple(scales.shape)))
+        _same(scales, codes, "scales")
+        self.codes, self.scales, self.columns, self.signed = codes.contiguous(), scales.contiguous(), int(columns), bool(signed)
+
+    @property
+    def rows(self):
+        return self.codes.shape[0]
+
+    def values(self, dtype=torch.float32):
+        """The values the checkpoint stands for, [n, columns]: exact in float32 and bfloat16 (at most 8 significant bits)."""
+        out = torch.empty((self.rows, self.columns), dtype=dtype, device=self.codes.device)
+        t = _type(out, "the values")
+        lib, stream, guard = _on(out)
+        with guard:
+            B.check_layers(lib.iblnerf_checkpoint_values(stream, self.codes.data_ptr(), self.scales.data_ptr(), self.rows, self.columns, int(self.signed), t, out.data_ptr(), self.columns))
+        return out
+
+
+def _codes_like(x, n, columns):
+    blocks = (columns + 31) // 32
+    return torch.empty((n, 32 * blocks), dtype=torch.uint8, device=x.device), torch.empty((n, blocks), dtype=torch.uint8, device=x.device)
+
+
+def checkpoint(x, signed=True):
+    """The 8-bit checkpoint of x [..., k] (rows flattened).  signed=False: negative entries become zero."""
+    t = _type(x, "x")
+    lib, stream, guard = _on(x)
+    x, ld = _rows(x.detach(), "x")
+    n, k = x.shape
+    codes, scales = _codes_like(x, n, k)
+    with guard:
+        B.check_layers(lib.iblnerf_checkpoint(stream, t, x.data_ptr(), ld, n, k, int(bool(signed)), codes.data_ptr(), scales.data_ptr()))
+    return Checkpoint(codes, scales, k, signed)
+
+
+def _weight(weight, k, like, dtype):
+    if weight.dim() != 2 or weight.shape[1] != k:
+        raise ValueError("a layer of %d inputs takes a weight [o, %d], got %s" % (k, k, tuple(weight.shape)))
+    _same(weight, like, "weight", dtype)
+    return _rows(weight.detach(), "weight")
+
+
+def dense_forward(x, weight, bias=None, relu=False, keep=True):
+    """y = x weight^T + bias (negative values to zero if relu), x [..., k], weight [o, k], bias [o] or None, all of one type -> (y [..., o], y's checkpoint or None).
+    keep=False: no checkpoint (nothing will be trained)."""
+    t = _type(x, "x")
+    lib, stream, guard = _on(x)
+    lead = x.shape[:-1]
+    x, ld = _rows(x.detach(), "x")
+    n, k = x.shape
+    w, ldw = _weight(weight, k, x, x.dtype)
+    o = w.shape[0]
+    if not 1 <= o <= MAX_COLUMNS:
+        raise ValueError("a layer has 1 to %d outputs, got %d" % (MAX_COLUMNS, o))
+    if bias is not None:
+        if tuple(bias.shape) != (o,):
+            raise ValueError("the bias of a layer of %d outputs is [%d], got %s" % (o, o, tuple(bias.shape)))
+        _same(bias, x, "bias", x.dtype)
+        bias = bias.detach().contiguous()
+    y = torch.empty((n, o), dtype=x.dtype, device=x.device)
+    codes, scales = _codes_like(x, n, o) if keep else (None, None)
+    with guard:
+        B.check_layers(lib.iblnerf_dense_forward(stream, t, x.data_ptr(), ld, n, k, w.data_ptr(), ldw, o, None if bias is None else bias.data_ptr(), int(bool(relu)), y.data_ptr(), o,
+                                                 codes.data_ptr() if keep else None, scales.data_ptr() if keep else None))
+    return y.reshape(lead + (o,)), (Checkpoint(codes, scales, o, not relu) if keep else None)
+
+
+def dense_backward(dy, x, weight, relu=None, need_dx=True, need_dw=True, need_db=True, grad_dtype=None):
+    """The gradients of dense_forward from checkpoints: dy [..., o], x the Checkpoint of the layer's input, relu the Checkpoint of its output (None: the layer has no ReLU)
+    -> (dX [..., k], dW [o, k], db [o]), None where not asked for.  grad_dtype: dW's and db's type (dy's own by default, or float32)."""
+    t = _type(dy, "dy")
+    lib, stream, guard = _on(dy)
+    lead = dy.shape[:-1]
+    dy, ld = _rows(dy.detach(), "dy")
+    n, o = dy.shape
+    if not isinstance(x, Checkpoint) or x.rows != n:
+        raise ValueError("x must be the Checkpoint of the layer's %d input rows" % n)
+    k = x.columns
+    w, ldw = _weight(weight, k, dy, dy.dtype)
+    if w.shape[0] != o:
+        raise ValueError("dy has %d columns, the weight %d rows" % (o, w.shape[0]))
+    _same(x.codes, dy, "the input's checkpoint")
+    if relu is not None:
+        if not isinstance(relu, Checkpoint) or relu.rows != n or relu.columns != o or relu.signed:
+            raise ValueError("relu must be the unsigned Checkpoint of the layer's output [%d, %d]" % (n, o))
+        _same(relu.codes, dy, "the output's checkpoint")
+    grad_dtype = grad_dtype or dy.dtype
+    if grad_dtype not in (dy.dtype, torch.float32):
+        raise TypeError("the parameters' gradients are %s or float32, not %s" % (dy.dtype, grad_dtype))
+    dev = dy.device
+    dx = torch.empty((n, k), dtype=dy.dtype, device=dev) if need_dx else None
+    dw = torch.empty((o, k), dtype=grad_dtype, device=dev) if need_dw or need_db else None
+    db = torch.empty((o,), dtype=grad_dtype, device=dev) if need_db else None
+    ws = torch.empty((lib.iblnerf_dense_backward_workspace(t, n, k, o),), dtype=torch.uint8, device=dev) if dw is not None else None
+    with guard:
+        B.check_layers(lib.iblnerf_dense_backward(stream, t, dy.data_ptr(), ld, n, k, o, x.codes.data_ptr(), x.scales.data_ptr(), int(x.signed), None if relu is None else relu.codes.data_ptr(),
+                                                  w.data_ptr(), ldw, None if dx is None else dx.data_ptr(), k, _TYPES[grad_dtype], None if dw is None else dw.data_ptr(),
+                                                  None if db is None else db.data_ptr(), None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel()))
+    return (None if dx is None else dx.reshape(lead + (k,))), (dw if need_dw else None), db
+
+
+class _Dense(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, relu, x_codes, x_scales, x_signed):
+        w = weight.to(x.dtype)
+        y, kept = dense_forward(x, w, None if bias is None else bias.to(x.dtype), relu)
+        if x_codes is None:
+            own = checkpoint(x)
+            x_codes, x_scales, x_signed = own.codes, own.scales, True
+        ctx.relu, ctx.x_signed, ctx.has_bias, ctx.type, ctx.bias_dtype = relu, x_signed, bias is not None, x.dtype, None if bias is None else bias.dtype
+        ctx.save_for_backward(weight, x_codes, x_scales, *((kept.codes, kept.scales) if relu else ()))
+        ctx.mark_non_differentiable(kept.codes, kept.scales)
+        return y, kept.codes, kept.scales
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy, _codes, _scales):
+        weight, xc, xs, *out = ctx.saved_tensors
+        k, o = weight.shape[1], weight.shape[0]
+        need_x, need_w, need_b = ctx.needs_input_grad[:3]
+        dx, dw, db = dense_backward(dy.to(ctx.type), Checkpoint(xc, xs, k, ctx.x_signed), weight.to(ctx.type), Checkpoint(*out, o) if ctx.relu else None, need_x, need_w, need_b and ctx.has_bias,
+                                    torch.float32 if weight.dtype == torch.float32 else None)
+        return dx, dw, db, None, None, None, None
+
+
+def dense(x, weight, bias=None, relu=False, kept=None):
+    """dense_forward with autograd -> (y, Checkpoint of y).  kept: the Checkpoint of x that an earlier layer has written (None: one is made here, signed) — the backward pass
+    reads the checkpoints of x and, under a ReLU, of y, so neither tensor is held for it.  Parameters may be float32 beside 16-bit activations: they are cast for the
+    products, and their gradients are float32 sums.  First derivatives only."""
+    if kept is not None and (kept.columns != x.shape[-1] or kept.rows * kept.columns != x.numel()):
+        raise ValueError("kept is a checkpoint of [%d, %d], x is %s" % (kept.rows, kept.columns, tuple(x.shape)))
+    y, codes, scales = _Dense.apply(x, weight, bias, bool(relu), *((None, None, True) if kept is None else (kept.codes, kept.scales, kept.signed)))
+    return y, Checkpoint(codes, scales, weight.shape[0], not relu)
+
+
+def _index(index, like):
+    if index.dtype not in (torch.int32, torch.int64):
+        raise TypeError("index must be int32 or int64, got %s" % index.dtype)
+    _same(index, like, "index")
+    return index.contiguous(), 64 if index.dtype == torch.int64 else 32
+
+
+def _lookup(table, index, scale, rows_per_index, out):
+    t = _type(table, "table")
+    lib, stream, guard = _on(table)
+    if table.dim() != 2 or table.shape[0] < 1:
+        raise ValueError("table must be [v, d] with at least one row, got %s" % (tuple(table.shape),))
+    tab, ld = _rows(table.detach(), "table")
+    v, d = tab.shape
+    idx, bits = _index(index, table)
+    n, per = idx.numel(), int(rows_per_index)
+    if per < 1:
+        raise ValueError("rows_per_index must be at least 1, got %d" % per)
+    shape = tuple(index.shape[:-1]) + (index.shape[-1] * per, d) if index.dim() else (per, d)
+    if out is None:
+        out = torch.empty(shape, dtype=table.dtype, device=table.device)
+    else:
+        _same(out, table, "out", table.dtype)
+        if out.dim() != 2 or tuple(out.shape) != (n * per, d) or (d > 1 and out.stride(1) != 1) or (out.shape[0] > 1 and out.stride(0) < d):
+            raise ValueError("out must be [%d, %d] with unit stride along a row, got %s strides %s" % (n * per, d, tuple(out.shape), tuple(out.stride())))
+    ld_out = out.stride(0) if out.dim() == 2 and out.shape[0] > 1 else d
+    with guard:
+        B.check_layers(lib.iblnerf_lookup(stream, t, tab.data_ptr(), ld, v, d, idx.data_ptr(), bits, n, per, float(scale), out.data_ptr(), ld_out))
+    return out
+
+
+def lookup_backward(dout, index, v, scale=1.0, rows_per_index=1):
+    """d table [v, d] = scale * the sums of dout [..., d] over each token's rows (rows in index's order, rows_per_index of them each).  Rows with an index outside [0, v)
+    count nowhere.  The same inputs give the same bits."""
+    t = _type(dout, "dout")
+    lib, stream, guard = _on(dout)
+    dout, ld = _rows(dout.detach(), "dout")
+    idx, bits = _index(index, dout)
+    n, per, d = idx.numel(), int(rows_per_index), dout.shape[1]
+    if per < 1 or int(v) < 1 or n * per != dout.shape[0]:
+        raise ValueError("%d indices with %d rows each over a table of %d rows do not fit %d gradient rows" % (n, per, int(v), dout.shape[0]))
+    grad = torch.empty((int(v), d), dtype=dout.dtype, device=dout.device)
+    ws = torch.empty((lib.iblnerf_lookup_backward_workspace(n, per, int(v), d),), dtype=torch.uint8, device=dout.device)
+    with guard:
+        B.check_layers(lib.iblnerf_lookup_backward(stream, t, dout.data_ptr(), ld, idx.data_ptr(), bits, n, per, int(v), d, float(scale), grad.data_ptr(), ws.data_ptr(), ws.numel()))
+    return grad
+
+
+class _Lookup(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, table, index, scale, per):
+        ctx.save_for_backward(index)
+        ctx.v, ctx.scale, ctx.per = table.shape[0], scale, per
+        return _lookup(table, index, scale, per, None)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout):
+        (index,) = ctx.saved_tensors
+        return lookup_backward(dout, index, ctx.v, ctx.scale, ctx.per), None, None, None
+
+
+def lookup(table, index, scale=1.0, rows_per_index=1, out=None):
+    """scale * table[index]: table [v, d], index [...] int32 or int64 -> [..., d]; rows_per_index > 1 repeats each row (a ray's code for each of its samples): the last axis of
+    index grows by that factor.  A negative index is a row without a code (zeros, no gradient); one beyond the table reads NaN.  Differentiable in the table; `out`
+    ([n, d], rows may be strided: a slice of a wider input) is written instead of a new tensor, without autograd."""
+    if out is None and torch.is_grad_enabled() and table.requires_grad:
+        return _Lookup.apply(table, index, float(scale), int(rows_per_index))
+    return _lookup(table, index, scale, rows_per_index, out)
