@@ -27,7 +27,8 @@ EXPORTS = [
     "iblnerf_last_executed_flops", "iblnerf_estimate_policy", "iblnerf_ray_outputs_backward_gt", "iblnerf_ray_outputs_backward_rays", "iblnerf_coarse_z_rays", "iblnerf_aux_query", "iblnerf_aux_backward", "iblnerf_ray_outputs_backward_env", "iblnerf_set_select_tmin", "iblnerf_set_chunk_cuts",
     "iblnerf_decide_route", "iblnerf_set_route", "iblnerf_get_route", "iblnerf_copy_route", "iblnerf_describe_route", "iblnerf_last_slot_units", "iblnerf_trunk_density_fp32", "iblnerf_set_offset_tier_threshold",
     "iblnerf_escalate_route", "iblnerf_set_lists", "iblnerf_set_tapped_lists", "iblnerf_get_rays_strided", "iblnerf_get_rays_pixels", "iblnerf_set_tier_thresholds", "iblnerf_decide_route_outputs", "iblnerf_upload_weights_arch",
-    "iblnerf_layers_last_error", "iblnerf_checkpoint", "iblnerf_checkpoint_values", "iblnerf_dense_forward", "iblnerf_dense_backward_workspace", "iblnerf_dense_backward",
+    "iblnerf_layers_last_error", "iblnerf_checkpoint", "iblnerf_checkpoint_values", "iblnerf_dense_forward_workspace", "iblnerf_dense_forward", "iblnerf_dense_backward_workspace",
+    "iblnerf_dense_backward",
     "iblnerf_lookup", "iblnerf_lookup_backward_workspace", "iblnerf_lookup_backward",
 ]
 
@@ -280,15 +281,16 @@ def load_library(path: str = LIB_PATH):
     lib.iblnerf_layers_last_error.restype = C.c_char_p
     lib.iblnerf_checkpoint.argtypes = [FP, I, FP, L, L, I, I, FP, FP]
     lib.iblnerf_checkpoint_values.argtypes = [FP, FP, FP, L, I, I, I, FP, L]
-    lib.iblnerf_dense_forward.argtypes = [FP, I, FP, L, L, I, FP, L, I, FP, I, FP, L, FP, FP]
-    lib.iblnerf_dense_backward_workspace.argtypes = [I, L, I, I]
-    lib.iblnerf_dense_backward_workspace.restype = C.c_size_t
+    lib.iblnerf_dense_forward.argtypes = [FP, I, FP, L, L, I, FP, L, I, FP, I, FP, L, FP, FP, FP, C.c_size_t]
+    for n in ("iblnerf_dense_forward_workspace", "iblnerf_dense_backward_workspace"):
+        getattr(lib, n).argtypes = [I, L, I, I]
+        getattr(lib, n).restype = C.c_size_t
     lib.iblnerf_dense_backward.argtypes = [FP, I, FP, L, L, I, I, FP, FP, I, FP, FP, L, FP, L, I, FP, FP, FP, C.c_size_t]
     lib.iblnerf_lookup.argtypes = [FP, I, FP, L, L, I, FP, I, L, L, C.c_float, FP, L]
     lib.iblnerf_lookup_backward_workspace.argtypes = [L, L, L, I]
     lib.iblnerf_lookup_backward_workspace.restype = C.c_size_t
     lib.iblnerf_lookup_backward.argtypes = [FP, I, FP, L, FP, I, L, L, L, I, C.c_float, FP, FP, C.c_size_t]
-    for n in ("iblnerf_checkpoint", "iblnerf_checkpoint_values", "iblnerf_dense_forward", "iblnerf_dense_backward", "iblnerf_lookup", "iblnerf_lookup_backward"):
+    for n in ("iblnerf_checkpoint", "iblnerf_checkpoint_values", "iblnerf_dense_forward_workspace", "iblnerf_dense_forward", "iblnerf_dense_backward", "iblnerf_lookup", "iblnerf_lookup_backward"):
         getattr(lib, n).restype = C.c_int
     for n in ("iblnerf_create", "iblnerf_upload_weights", "iblnerf_upload_lut", "iblnerf_pack_weights_host",
               "iblnerf_get_rays", "iblnerf_network_query", "iblnerf_sample_pdf", "iblnerf_render_rays",

@@ -12,6 +12,8 @@
 // same fp32 accumulator: what is left out (lr + rl + rr) is at most 2^-24 of |x||w|, the size of fp32's own rounding of a product; six 16-bit products take 24 matrix-core
 // slots where the fp32 instruction takes 64.  (An infinity in a float32 operand, or a magnitude above bfloat16's largest, 3.39e38, comes out as NaN: its lower parts are
 // inf - inf.)  A checkpoint's value is one part by itself: three products.
+#include <atomic>
+
 #include "layer_elems.h"
 #include "layers.h"
 
@@ -62,48 +64,96 @@ template <int BK> __device__ __forceinline__ int along(int i, int c) {
     constexpr int C = BK / 8;
     return i * BK + ((c ^ ((i / (16 / C)) % C)) * 8);
 }
-// "across": one row of 128 columns for each reduction index; the 64-byte chunk c of row p at place c ^ (p & 3): the transposing read below takes 4 rows x 64 bytes at once
-__device__ __forceinline__ int across(int p, int c32) { return p * 128 + ((c32 ^ (p & 3)) * 32); }
+// "across": one row of W columns for each reduction index; the 64-byte chunk c of row p at place c ^ (p & 3): the transposing read below takes 4 rows x 64 bytes at once
+template <int W> __device__ __forceinline__ int across(int p, int c32) { return p * W + ((c32 ^ (p & 3)) * 32); }
 
 // Operand fragments of step ks (16 reduction elements): lane (i = lane & 31, h = lane >> 5) holds elements 8 h .. 8 h + 7 of column / row i of the 32-wide tile
 template <int BK> __device__ __forceinline__ u32x4 frag_along(const unsigned short* t, int row0, int ks, int lane) {
     return *reinterpret_cast<const u32x4*>(t + along<BK>(row0 + (lane & 31), 2 * ks + (lane >> 5)));
 }
 // ds_read_tr16_b64: 16 lanes read 4 rows of 16 columns (8 bytes each) and get column (lane & 15), 4 rows each: two reads make the 8 reduction elements
-__device__ __forceinline__ u32x4 frag_across(const unsigned short* t, int c32, int ks, int lane) {
+template <int W> __device__ __forceinline__ u32x4 frag_across(const unsigned short* t, int c32, int ks, int lane) {
     const int l = lane & 15, half = (lane >> 4) & 1, h = lane >> 5;
-    const unsigned short* p = t + across(16 * ks + 8 * h + (l >> 2), c32) + 16 * half + 4 * (l & 3);
+    const unsigned short* p = t + across<W>(16 * ks + 8 * h + (l >> 2), c32) + 16 * half + 4 * (l & 3);
     union { s16x4 s[2]; u32x4 u; } v;
     v.s[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)p);
-    v.s[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p + 4 * 128));
+    v.s[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p + 4 * W));
     return v.u;
 }
 
-// Block statistics and codes of 8 of a block's 32 values; the four lanes that hold the block sit side by side (lane & ~3).  Every lane of the four must arrive.
-__device__ __forceinline__ void encode8(const float (&f)[8], bool is_signed, u32x2& codes, unsigned& scale) {
-    int mag = 0, pos = 0;      // float bits as integers order as the magnitudes do; an infinity or NaN is >= 0x7f800000
+// the largest of the four lanes side by side (lane & ~3), in each of them
+__device__ __forceinline__ unsigned max_of_4(unsigned x) {
+    x = max(x, (unsigned)__builtin_amdgcn_mov_dpp((int)x, 0xb1, 0xf, 0xf, true));      // lanes 1 0 3 2
+    return max(x, (unsigned)__builtin_amdgcn_mov_dpp((int)x, 0x4e, 0xf, 0xf, true));   // lanes 2 3 0 1
+}
+
+// A block's largest magnitude and the value that sets its step (the largest positive one of an unsigned checkpoint), as bits of its type.  Magnitudes are compared as integers:
+// a value's bits without the sign order as the values do, and an infinity or NaN is at least the infinity's.
+struct Block { unsigned mag, top; };
+template <int T, int N> __device__ __forceinline__ Block block_of(const Raw8<T> (&v)[N], bool is_signed) {
+    Block b;
+    if constexpr (T == LT_F32) {
+        unsigned mag = 0;
+        int pos = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const int b = (int)as_bits(f[i]);
-        mag = max(mag, b & 0x7fffffff);
-        pos = max(pos, b);
+        for (int i = 0; i < 8 * N; ++i) {
+            const unsigned u = v[i >> 3].q[(i & 7) >> 2][i & 3];
+            mag = max(mag, u & 0x7fffffffu);
+            pos = max(pos, (int)u);
+        }
+        b = Block{mag, is_signed ? mag : (unsigned)pos};
+    } else {
+        u16x2 m = {0, 0};
+        s16x2 p = {0, 0};
+#pragma unroll
+        for (int i = 0; i < 4 * N; ++i) {
+            const unsigned u = v[i >> 2].q[0][i & 3], c = u & 0x7fff7fffu;
+            m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, c));
+            p = __builtin_elementwise_max(p, __builtin_bit_cast(s16x2, u));
+        }
+        b.mag = max((unsigned)m[0], (unsigned)m[1]);
+        b.top = is_signed ? b.mag : (unsigned)max((int)p[0], (int)p[1]);
     }
-    mag = max(mag, __shfl_xor(mag, 1)); mag = max(mag, __shfl_xor(mag, 2));
-    pos = max(pos, __shfl_xor(pos, 1)); pos = max(pos, __shfl_xor(pos, 2));
-    const int a = is_signed ? mag : pos;
+    return b;
+}
+
+struct Step { float inv; unsigned scale; bool bad; };
+template <int T> __device__ __forceinline__ Step step_of(const Block& b, bool is_signed) {
+    const bool bad = b.mag >= (T == LT_F32 ? 0x7f800000u : T == LT_BF16 ? 0x7f80u : 0x7c00u);
+    const unsigned top = T == LT_F32 ? b.top : T == LT_BF16 ? b.top << 16 : as_bits(half_float(b.top));
     // 127 = 1.984375 * 2^6 (fraction bits 0x7e0000), 255 = 1.9921875 * 2^7 (0x7f0000)
-    const int e = max((a >> 23) - 127 - (is_signed ? 6 : 7) + ((a & 0x7fffff) > (is_signed ? 0x7e0000 : 0x7f0000) ? 1 : 0), -126);
-    const bool bad = mag >= 0x7f800000;
-    const float inv = as_float(bad ? 0 : (127 - e) << 23);
-    unsigned c[8];
+    const int e = max((int)(top >> 23) - 127 - (is_signed ? 6 : 7) + ((top & 0x7fffffu) > (is_signed ? 0x7e0000u : 0x7f0000u) ? 1 : 0), -126);
+    return Step{as_float(bad ? 0u : (unsigned)(127 - e) << 23), bad ? 255u : (unsigned)(e + 127), bad};
+}
+
+template <int T> __device__ __forceinline__ u32x2 codes_of(const Raw8<T>& v, const Step& s, bool is_signed) {
+    float f[8];
+    to_floats<T>(v, f);
+    u32x2 codes;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const int q = (int)rintf(f[i] * inv);
-        c[i] = is_signed ? (unsigned)q & 255u : (f[i] > 0.0f ? (unsigned)max(q, 1) : 0u);
+    for (int g = 0; g < 2; ++g) {
+        unsigned c = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            float u = f[4 * g + i] * s.inv;
+            if (is_signed) u = rintf(u) + 128.0f;                                              // (the top bit flipped back below)
+            else u = fmaxf(u, __builtin_amdgcn_fmed3f(ceilf(f[4 * g + i]), 0.0f, 1.0f));       // a positive value, however small, keeps at least code 1
+            c = __builtin_amdgcn_cvt_pk_u8_f32(u, i, c);                                       // rounds to nearest, ties to even; below zero: 0
+        }
+        codes[g] = s.bad ? 0x01010101u : is_signed ? c ^ 0x80808080u : c;
     }
-#pragma unroll
-    for (int g = 0; g < 2; ++g) codes[g] = bad ? 0x01010101u : (c[4 * g] | c[4 * g + 1] << 8 | c[4 * g + 2] << 16 | c[4 * g + 3] << 24);
-    scale = bad ? 255u : (unsigned)(e + 127);
+    return codes;
+}
+
+// Codes and scale byte of 8 of a block's 32 values; the four lanes that hold the block sit side by side, and all of them must arrive
+template <int T> __device__ __forceinline__ void encode8(const Raw8<T>& v, bool is_signed, u32x2& codes, unsigned& scale) {
+    const Raw8<T> one[1] = {v};
+    Block b = block_of<T, 1>(one, is_signed);
+    b.mag = max_of_4(b.mag);
+    b.top = max_of_4(b.top);
+    const Step s = step_of<T>(b, is_signed);
+    codes = codes_of<T>(v, s, is_signed);
+    scale = s.scale;
 }
 
 // the eight values behind codes: (u - off) * step in one exact fused multiply-add (u the code byte, its top bit flipped where signed); scale byte 255 makes step infinite
@@ -119,6 +169,81 @@ __device__ __forceinline__ void decode8(u32x2 codes, unsigned scale, bool is_sig
     }
 }
 
+// The end of a Y tile: a wave's TP x 32 rows, TO x 32 outputs from o0 on.  32 rows at a time through the wave's own window of LDS: rounded outputs in, whole row pieces out
+// (16 bytes a lane) with their checkpoint.
+template <int TO, int T> struct Window { static constexpr int row = 32 * TO * Bytes<T>::v + 16, bytes = 32 * row; };
+template <int T, bool DX, int TO, int TP>
+__device__ __forceinline__ void write_rows(const DenseRows& a, const f32x16 (&acc)[TO][TP], char* win, long p0, int o0, int lane) {
+    constexpr int RS = Window<TO, T>::row, LPR = 4 * TO;      // lanes a row (8 outputs each)
+    const int h = lane >> 5;
+#pragma unroll
+    for (int k = 0; k < TP; ++k) {
+#pragma unroll
+        for (int i = 0; i < TO; ++i)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                float v[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    v[e] = acc[i][k][4 * g + e];
+                    if (!DX && a.relu) v[e] = __builtin_elementwise_maximum(v[e], 0.0f);      // (a NaN stays, -0 becomes 0)
+                }
+                char* dst = win + (lane & 31) * RS + (32 * i + 8 * g + 4 * h) * Bytes<T>::v;
+                if constexpr (T == LT_F32) *reinterpret_cast<u32x4*>(dst) = u32x4{as_bits(v[0]), as_bits(v[1]), as_bits(v[2]), as_bits(v[3])};
+                else *reinterpret_cast<u32x2*>(dst) = u32x2{pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3])};
+            }
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll 1
+        for (int pass = 0; pass < 32 * LPR / 64; ++pass) {      // (unrolled it takes registers that the products' loop then spills)
+            const int at = pass * 64 + lane, row = at / LPR, c = 8 * (at % LPR);
+            const long p = p0 + 32 * k + row;
+            const int o = o0 + c;
+            Raw8<T> v;
+            v.q[0] = *reinterpret_cast<const u32x4*>(win + row * RS + c * Bytes<T>::v);
+            if constexpr (T == LT_F32) v.q[1] = *reinterpret_cast<const u32x4*>(win + row * RS + c * 4 + 16);
+            if (p < a.n && o < a.o) store8<T>(static_cast<char*>(a.y) + p * a.ldy * Bytes<T>::v, o, a.o, v);
+            if (!DX && a.codes) {
+                if (o + 8 > a.o) {      // (columns beyond the layer's outputs are coded 0)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        if (o + e >= a.o) {
+                            if constexpr (T == LT_F32) v.q[e >> 2][e & 3] = 0;
+                            else v.q[0][e >> 1] &= (e & 1) ? 0x0000ffffu : 0xffff0000u;
+                        }
+                }
+                u32x2 codes; unsigned scale;
+                encode8<T>(v, a.is_signed != 0, codes, scale);
+                const int o32 = (a.o + 31) & ~31;
+                if (p < a.n && o < o32) {
+                    *reinterpret_cast<u32x2*>(a.codes + p * o32 + o) = codes;
+                    if ((c & 31) == 0) a.scales[p * (o32 >> 5) + (o >> 5)] = (uint8_t)scale;
+                }
+            }
+        }
+        __builtin_amdgcn_wave_barrier();
+    }
+}
+
+template <int T> __device__ __forceinline__ float bias_at(const DenseRows& a, int o) {
+    if (!a.bias || o >= a.o) return 0.0f;
+    if constexpr (T == LT_F32) return static_cast<const float*>(a.bias)[o];
+    else if constexpr (T == LT_BF16) return as_float((unsigned)static_cast<const unsigned short*>(a.bias)[o] << 16);
+    else return (float)static_cast<const _Float16*>(a.bias)[o];
+}
+
+// accumulators begin with the bias of their output (in LDS: the wave's first output's on), or with zero
+template <bool DX, int TO, int TP> __device__ __forceinline__ void begin(f32x16 (&acc)[TO][TP], const float* bias, int lane) {
+#pragma unroll
+    for (int i = 0; i < TO; ++i) {
+        f32x16 b = {0};
+        if (!DX)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) b[r] = bias[32 * i + (r & 3) + 8 * (r >> 2) + 4 * (lane >> 5)];
+#pragma unroll
+        for (int k = 0; k < TP; ++k) acc[i][k] = b;
+    }
+}
+
 // ------------------------------------------------------------------------------------------------------------------------------ Y = act(A B + bias)
 // One workgroup = BP rows x BO outputs, 4 waves of (BP / 2) x (BO / 2); D[output][row] so that a lane's accumulators are runs of 4 outputs of ONE row.  The reduction runs
 // in steps of BK staged through LDS: the next step's elements travel into registers while this step's products run.
@@ -129,9 +254,7 @@ __global__ __launch_bounds__(256, 2) void k_dense_rows(DenseRows a) {
     constexpr int TP = BP / 64, TO = BO / 64;                      // 32-wide tiles of a wave
     constexpr int XC = BP * BK / 8 / 256, WC = BO * BK / 8 / 256;  // 8-element chunks a thread stages
     constexpr int XPLANE = BP * BK, WPLANE = BO * BK;
-    constexpr int RS = (BO / 2) * Bytes<T>::v + 16;                // epilogue: bytes of a row in a wave's LDS window of 32 rows
-    constexpr int STAGE = PARTS * (XPLANE + WPLANE) * 2, OUT = 4 * 32 * RS;
-    static_assert(!DX || BO == 128, "the across layout has rows of 128 columns");
+    constexpr int STAGE = PARTS * (XPLANE + WPLANE) * 2, OUT = 4 * Window<TO, T>::bytes;
     __shared__ __attribute__((aligned(16))) char lds[STAGE > OUT ? STAGE : OUT];
     __shared__ float bias[BO];
     unsigned short* xt = reinterpret_cast<unsigned short*>(lds);
@@ -143,17 +266,9 @@ __global__ __launch_bounds__(256, 2) void k_dense_rows(DenseRows a) {
     const long p0 = pt * BP;
     const int o0 = (int)(j % ot) * BO;
     if (p0 >= a.n) return;
-    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const int wp = (wave >> 1) * (BP / 2), wo = (wave & 1) * (BO / 2);
-    if (t < BO) {
-        float b = 0.0f;
-        if (!DX && a.bias && o0 + t < a.o) {
-            if constexpr (T == LT_F32) b = static_cast<const float*>(a.bias)[o0 + t];
-            else if constexpr (T == LT_BF16) b = as_float((unsigned)static_cast<const unsigned short*>(a.bias)[o0 + t] << 16);
-            else b = (float)static_cast<const _Float16*>(a.bias)[o0 + t];
-        }
-        bias[t] = b;
-    }
+    if (!DX && t < BO) bias[t] = bias_at<T>(a, o0 + t);
 
     const int r32 = (a.r + 31) & ~31;
     Raw8<T> xr[XC], wr[WC];
@@ -193,20 +308,17 @@ __global__ __launch_bounds__(256, 2) void k_dense_rows(DenseRows a) {
         for (int i = 0; i < WC; ++i) {
             const int c = t + 256 * i;
             if (!DX) stage8<T>(wt + along<BK>(c / (BK / 8), c % (BK / 8)), WPLANE, wr[i]);
-            else stage8<T>(wt + across(c / (BO / 8), (c % (BO / 8)) >> 2) + 8 * (c & 3), WPLANE, wr[i]);
+            else stage8<T>(wt + across<BO>(c / (BO / 8), (c % (BO / 8)) >> 2) + 8 * (c & 3), WPLANE, wr[i]);
         }
     };
 
     f32x16 acc[TO][TP];
-#pragma unroll
-    for (int i = 0; i < TO; ++i)
-#pragma unroll
-        for (int k = 0; k < TP; ++k) acc[i][k] = f32x16{0};
     load(0);
     for (int k0 = 0; k0 < a.r; k0 += BK) {
         if (k0) __syncthreads();
         stage();
         __syncthreads();
+        if (k0 == 0) begin<DX>(acc, bias + wo, lane);
         if (k0 + BK < a.r) load(k0 + BK);
 #pragma unroll
         for (int ks = 0; ks < BK / 16; ++ks) {
@@ -220,7 +332,7 @@ __global__ __launch_bounds__(256, 2) void k_dense_rows(DenseRows a) {
                 u32x4 w[PARTS];
 #pragma unroll
                 for (int q = 0; q < PARTS; ++q)
-                    w[q] = DX ? frag_across(wt + q * WPLANE, (wo >> 5) + i, ks, lane) : frag_along<BK>(wt + q * WPLANE, wo + 32 * i, ks, lane);
+                    w[q] = DX ? frag_across<BO>(wt + q * WPLANE, (wo >> 5) + i, ks, lane) : frag_along<BK>(wt + q * WPLANE, wo + 32 * i, ks, lane);
 #pragma unroll
                 for (int k = 0; k < TP; ++k) acc[i][k] = product<T, PARTS, PARTS>(w, x[k], acc[i][k]);
             }
@@ -228,155 +340,413 @@ __global__ __launch_bounds__(256, 2) void k_dense_rows(DenseRows a) {
     }
     __syncthreads();
 
-    // 32 rows at a time through the wave's own window of LDS: rounded outputs in, whole row pieces out (16 bytes a lane) with their checkpoint
-    char* win = lds + wave * 32 * RS;
-    const int h = lane >> 5;
+    write_rows<T, DX, TO, TP>(a, acc, lds + wave * Window<TO, T>::bytes, p0 + wp, o0 + wo, lane);
+}
+
+// The weights as matrix operands for k_dense_tall: [32-wide tile][16 reduction elements][lane][8], zeros beyond the layer
+template <int T, bool DX> __global__ __launch_bounds__(256) void k_dense_fragments(DenseRows a, u32x4* wf, int tiles, int steps) {
+    const int id = blockIdx.x * 256 + threadIdx.x;
+    const int lane = id & 63, ks = (id >> 6) % steps, tile = (id >> 6) / steps;
+    if (tile >= tiles) return;
+    const int i = 32 * tile + (lane & 31), r0 = 16 * ks + 8 * (lane >> 5);
+    u32x4 v = {0, 0, 0, 0};
+    if (i < a.o) {
+        if (!DX) {
+            v = load8<T>(static_cast<const char*>(a.w) + (long)i * a.ldw * 2, r0, a.r).q[0];
+        } else {
+            const unsigned short* w = static_cast<const unsigned short*>(a.w) + i;
 #pragma unroll
-    for (int k = 0; k < TP; ++k) {
+            for (int e = 0; e < 8; ++e)
+                if (r0 + e < a.r) v[e >> 1] |= (unsigned)w[(long)(r0 + e) * a.ldw] << (16 * (e & 1));
+        }
+    }
+    wf[id] = v;
+}
+
+constexpr int TALL_ROWS = 128;
+// eight 16-bit elements moved down by `n` (0 or less: not at all; 8 or more: nothing is left), zeros behind them
+__device__ __forceinline__ u32x4 drop16(u32x4 v, int n) {
+    unsigned long long lo = v[0] | (unsigned long long)v[1] << 32, hi = v[2] | (unsigned long long)v[3] << 32;
+    const int s = 16 * max(n, 0);
+    const unsigned long long l = s == 0 ? lo : s < 64 ? lo >> s | hi << (64 - s) : s < 128 ? hi >> (s - 64) : 0, u = s < 64 ? hi >> s : 0;
+    return u32x4{(unsigned)l, (unsigned)(l >> 32), (unsigned)u, (unsigned)(u >> 32)};
+}
+// place of the 16-byte chunk c of a row of CH chunks: 16 rows x one chunk fall on all banks
+template <int CH> __device__ __forceinline__ int tall_at(int row, int c) { return (row * CH + (c ^ (CH == 8 ? (row >> 1) & 7 : row & 15))) * 8; }
+
+// What k_dense_tall makes: the input gradient, or Y alone, or Y with its checkpoint behind a ReLU / without one
+enum TallMode { TALL_DX = 0, TALL_Y = 1, TALL_RELU_KEEP = 2, TALL_KEEP = 3 };
+
+// 32 rows x 64 outputs of Y from their accumulators.  A lane has outputs (r & 3) + 8 (r >> 2) + 4 h of row i; halves of the wave swap packed pairs so that it holds 16 neighbouring
+// outputs (16 h on): the block's largest value is one more swap away, 16 codes are one 16-byte word.  Everything leaves through `win` (2.5 KB of LDS for each wave) in
+// pieces of 64 bytes of a row: the address unit takes one such piece a cycle, and 16 bytes of 64 rows cost it 64 cycles where 64 bytes of 16 rows cost 16 (stored straight
+// from the lanes, results and codes took 270 us more for 786 432 x 512).
+struct Out { char* y; uint8_t* codes; uint8_t* scales; long ldy; int o32, rows, o; };      // at the first row and output; rows that are there, outputs from the first on
+template <int T, int MODE> __device__ __forceinline__ void write_rows64(const DenseRows& a, const f32x16& a0, const f32x16& a1, const Out& out, int lane, char* win) {
+    constexpr bool KEEP = MODE == TALL_RELU_KEEP || MODE == TALL_KEEP, SIGNED = MODE == TALL_KEEP;
+    constexpr int RS = 80;      // bytes of a row in the window (64 and a step to the next banks)
+    const int h = lane >> 5, i = lane & 31;
+    u32x4 c[2];
+    unsigned scales = 0;
 #pragma unroll
-        for (int i = 0; i < TO; ++i)
+    for (int tile = 0; tile < 2; ++tile) {
+        const f32x16& acc = tile ? a1 : a0;
+        unsigned d[4][2];
 #pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                float v[4];
+        for (int g = 0; g < 4; ++g) {
+            float v[4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    v[e] = acc[i][k][4 * g + e] + bias[wo + 32 * i + 8 * g + 4 * h + e];
-                    if (!DX && a.relu) v[e] = v[e] < 0.0f ? 0.0f : v[e];      // (a NaN stays)
-                }
-                char* dst = win + (lane & 31) * RS + (32 * i + 8 * g + 4 * h) * Bytes<T>::v;
-                if constexpr (T == LT_F32) {
-                    *reinterpret_cast<u32x4*>(dst) = u32x4{as_bits(v[0]), as_bits(v[1]), as_bits(v[2]), as_bits(v[3])};
-                } else {
-                    *reinterpret_cast<u32x2*>(dst) = u32x2{pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3])};
-                }
+            for (int e = 0; e < 4; ++e) {
+                v[e] = acc[4 * g + e];
+                if (MODE == TALL_RELU_KEEP || (MODE == TALL_Y && a.relu)) v[e] = __builtin_elementwise_maximum(v[e], 0.0f);      // (a NaN stays, -0 becomes 0)
             }
+            d[g][0] = pack2<T>(v[0], v[1]);
+            d[g][1] = pack2<T>(v[2], v[3]);
+        }
+        Raw8<T> half[2];
+#pragma unroll
+        for (int g = 0; g < 2; ++g)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const auto s = __builtin_amdgcn_permlane32_swap(d[g][j], d[g + 2][j], false, false);
+                half[g].q[0][j] = s[0];
+                half[g].q[0][2 + j] = s[1];
+            }
+        char* mine = win + i * RS + 32 * h;
+        *reinterpret_cast<u32x4*>(mine) = half[0].q[0];
+        *reinterpret_cast<u32x4*>(mine + 16) = half[1].q[0];
+        if (KEEP) {
+            const int have = out.o - 32 * tile - 16 * h;
+            if (out.o < 64)      // (columns beyond the layer's outputs are coded 0)
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                    if (e >= have) half[e >> 3].q[0][(e & 7) >> 1] &= (e & 1) ? 0x0000ffffu : 0xffff0000u;
+            u16x2 m = {0, 0};      // magnitudes as integers; behind a ReLU there is no sign: the bits themselves (a NaN's with it)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const unsigned u = half[e >> 2].q[0][e & 3] & (SIGNED ? 0x7fff7fffu : 0xffffffffu);
+                m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, u));
+            }
+            Block b;
+            b.mag = max((unsigned)m[0], (unsigned)m[1]);
+            const auto s = __builtin_amdgcn_permlane32_swap(b.mag, b.mag, false, false);
+            b.mag = b.top = max(s[0], s[1]);
+            const Step st = step_of<T>(b, SIGNED);
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const u32x2 q = codes_of<T>(half[e], st, SIGNED);
+                c[tile][2 * e] = q[0];
+                c[tile][2 * e + 1] = q[1];
+            }
+            scales |= st.scale << (8 * tile);
+        }
         __builtin_amdgcn_wave_barrier();
-        constexpr int LPR = BO / 16;                       // lanes a row (8 outputs each)
+        const int o = 32 * tile + 8 * (lane & 3);
 #pragma unroll
-        for (int pass = 0; pass < 32 * LPR / 64; ++pass) {
-            const int row = pass * (64 / LPR) + lane / LPR, c = 8 * (lane % LPR);
-            const long p = p0 + wp + 32 * k + row;
-            const int o = o0 + wo + c;
+        for (int j = 0; j < 2; ++j) {
+            const int row = 16 * j + (lane >> 2);
             Raw8<T> v;
-            v.q[0] = *reinterpret_cast<const u32x4*>(win + row * RS + c * Bytes<T>::v);
-            if constexpr (T == LT_F32) v.q[1] = *reinterpret_cast<const u32x4*>(win + row * RS + c * 4 + 16);
-            const bool in = p < a.n && o < a.o;
-            if (in) store8<T>(static_cast<char*>(a.y) + p * a.ldy * Bytes<T>::v, o, a.o, v);
-            if (!DX && a.codes) {
-                float f[8];
-                to_floats<T>(v, f);
+            v.q[0] = *reinterpret_cast<const u32x4*>(win + row * RS + 16 * (lane & 3));
+            char* y = out.y + row * out.ldy;
+            if (out.o >= 64) {
+                if (row < out.rows) __builtin_memcpy(y + 2 * o, &v.q[0], 16);
+            } else if (row < out.rows) store8<T>(y, o, out.o, v);
+        }
+        __builtin_amdgcn_wave_barrier();
+    }
+    if (KEEP) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) if (o + e >= a.o) f[e] = 0.0f;
-                u32x2 codes; unsigned scale;
-                encode8(f, a.is_signed != 0, codes, scale);
-                const int o32 = (a.o + 31) & ~31;
-                if (p < a.n && o < o32) {
-                    *reinterpret_cast<u32x2*>(a.codes + p * o32 + o) = codes;
-                    if ((c & 31) == 0) a.scales[p * (o32 >> 5) + (o >> 5)] = (uint8_t)scale;
-                }
-            }
+        for (int tile = 0; tile < 2; ++tile) *reinterpret_cast<u32x4*>(win + i * RS + 32 * tile + 16 * h) = c[tile];
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const int row = 16 * j + (lane >> 2), o = 16 * (lane & 3);
+            const u32x4 v = *reinterpret_cast<const u32x4*>(win + row * RS + o);
+            if (row < out.rows && o < ((out.o + 31) & ~31)) __builtin_memcpy(out.codes + row * out.o32 + o, &v, 16);
+        }
+        if (h == 0 && i < out.rows) {
+            uint8_t* s = out.scales + i * (out.o32 >> 5);
+            s[0] = (uint8_t)scales;
+            if (out.o > 32) s[1] = (uint8_t)(scales >> 8);
         }
         __builtin_amdgcn_wave_barrier();
     }
 }
 
+// The 16-bit types' form for many rows.  What bounds it is HBM (a 512-wide layer: 2.5 KB a row against 0.5 MFLOP), then L2 (the weights are read once for each 128 rows) and the
+// address units (see write_rows64).  Two workgroups stay on each compute unit and flow through their work, 128 rows x 256 outputs at a time: while a piece of the rows
+// (128 x COLS columns) is multiplied out of one LDS buffer, the next one — the next work item's first, too — is on its way in registers, goes to the other buffer, and the
+// piece after that is asked for before results are written; the other workgroup multiplies meanwhile.  A wave takes 128 rows x 64 outputs, so a fragment of the rows is
+// read once from LDS for each wave, and a fragment of the weights once from L2 for the workgroup.  Items of the same rows are neighbours on one XCD.  COLS: 128, or 64 for
+// layers that read no more.  786 432 x 512 x 512 bfloat16: 690 us with the checkpoint (2.0 GB: 2.9 TB/s), 570 us without, 620 us as the input gradient.  Tried and slower:
+// steps of 64 columns with one step under way (940 us); all columns of 64 rows at once, the weights read twice as often (750); weights kept in LDS and rows straight to
+// registers as operands (915: 16 bytes of 32 rows a load, address units full).
+template <int T, int MODE, int COLS>
+__global__ __launch_bounds__(256, 2) void k_dense_tall(DenseRows a, const u32x4* wf, int passes) {
+    constexpr bool DX = MODE == TALL_DX;
+    constexpr int TP = 4, TO = 2, AHEAD = 2, BO = 256, NT = 256, CH = COLS / 8, RP = NT / CH, NC = TALL_ROWS / RP, BUFFER = TALL_ROWS * COLS;
+    extern __shared__ __attribute__((aligned(16))) unsigned short lds[];
+    char* wins = reinterpret_cast<char*>(lds + 2 * BUFFER);
+    float* bias = reinterpret_cast<float*>(wins + 4 * 2560);
+    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+    const int steps = (a.r + 63) / 64 * 4, pieces = (a.r + COLS - 1) / COLS, r32 = (a.r + 31) & ~31, o32 = (a.o + 31) & ~31;
+    if (!DX) for (int i = t; i < passes * BO; i += NT) bias[i] = bias_at<T>(a, i);
+    // work item j of XCD x: rows of tile x + 8 (j / passes), outputs of pass j % passes; a workgroup takes every (gridDim / 8)-th
+    const long tiles = (a.n + TALL_ROWS - 1) / TALL_ROWS;
+    const int xcd = blockIdx.x & 7, first_item = blockIdx.x >> 3, stride_item = gridDim.x >> 3;
+    const long items = xcd < tiles ? (tiles - xcd + 7) / 8 * passes : 0;
+    const long mine = first_item < items ? (items - first_item + stride_item - 1) / stride_item : 0, count = mine * pieces;
+
+    // where the sequence of pieces stands: the loads run ahead of the products
+    struct At { long tile; int pass, piece; };
+    auto next = [&](At& x) {
+        if (++x.piece == pieces) {
+            x.piece = 0;
+            x.pass += stride_item;
+            x.tile += 8 * (x.pass / passes);
+            x.pass %= passes;
+        }
+    };
+    // the thread's 16-byte chunk of every RP-th row of a piece.  Rows behind the last are the last again (their results are not written), a chunk that hangs over the row's end is read
+    // from 8 elements before it and moved (stage): no branches, the loads travel together
+    const int row = t / CH, col = 8 * (t % CH);
+    const long stride = a.lda * 2;
+    unsigned short* place = lds + tall_at<CH>(row, t % CH);
+    Raw8<T> v[NC];
+    u32x2 q[NC];
+    int held = 0;      // the piece that the registers hold
+    auto load = [&](const At& x) {
+        const long p0 = x.tile * TALL_ROWS;
+        const int k = x.piece * COLS + col, last = (int)min(a.n - 1 - p0, (long)(TALL_ROWS - 1));
+        const char* base = static_cast<const char*>(a.a) + p0 * stride;
+        const unsigned at = 2 * min(k, a.r - 8);
+        held = x.piece;
+#pragma unroll
+        for (int i = 0; i < NC; ++i) v[i].q[0] = load16(base + ((unsigned)min(row + i * RP, last) * (unsigned)stride + at));
+        if (DX && a.open) {
+            const uint8_t* open = a.open + p0 * r32;
+            const unsigned at8 = min(k, r32 - 8);
+#pragma unroll
+            for (int i = 0; i < NC; ++i) q[i] = *reinterpret_cast<const u32x2*>(open + ((unsigned)min(row + i * RP, last) * (unsigned)r32 + at8));
+        }
+    };
+    auto stage = [&](int b) {
+        if ((held + 1) * COLS > a.r) {      // the row ends in this piece
+            const int over = held * COLS + col - (a.r - 8);      // elements that the chunk was read too early by; 8 and more: nothing of it is in the row
+#pragma unroll
+            for (int i = 0; i < NC; ++i) v[i].q[0] = drop16(v[i].q[0], over);
+        }
+#pragma unroll
+        for (int i = 0; i < NC; ++i) {
+            if (DX && a.open) close8<T>(v[i], q[i]);
+            *reinterpret_cast<u32x4*>(place + b * BUFFER + i * RP * COLS) = v[i].q[0];
+        }
+    };
+
+    f32x16 acc[TO][TP];
+    At in{xcd + 8 * (long)(first_item / passes), first_item % passes, 0}, now = in;
+    const int frow = lane & 31, fx = CH == 8 ? (frow >> 1) & 7 : frow & 15;      // a fragment's row in its 32, what its chunks are crossed with
+    const unsigned wlane = 16 * lane;
+    // The weights' fragments are one stream over all pieces, AHEAD steps in front of the products: loads come back in the order they were asked for, so a piece's first fragments
+    // are asked for before the rows of the piece after it — behind those they would wait for HBM
+    u32x4 w[AHEAD][TO];
+    auto weights_of = [&](const At& x) { return reinterpret_cast<const char*>(wf) + ((size_t)(x.pass * (BO / 32) + wave * TO) * steps + x.piece * (COLS / 16)) * 1024; };
+    auto weights = [&](const char* wl, int step, u32x4 (&to)[TO]) {
+#pragma unroll
+        for (int i = 0; i < TO; ++i) to[i] = *reinterpret_cast<const u32x4*>(wl + (size_t)(i * steps + step) * 1024 + wlane);
+    };
+    if (count > 0) {
+        load(in);
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) weights(weights_of(in), u, w[u]);
+        next(in);
+        stage(0);
+    }
+    if (count > 1) { load(in); next(in); }
+    __syncthreads();
+    for (long s = 0; s < count; ++s) {
+        const int b = (int)s & 1, o0 = now.pass * BO + wave * 64, size = min(steps - now.piece * (COLS / 16), COLS / 16);
+        const char* wl = weights_of(now);
+        At after = now;
+        if (s + 1 < count) next(after);
+        const char* wn = weights_of(after);
+        asm volatile("" ::: "memory");      // (the bias and the weights of a one-piece layer are the same in every round: kept in registers they spill)
+        if (now.piece == 0) begin<DX>(acc, bias + o0, lane);
+        const unsigned short* x0 = lds + b * BUFFER + frow * COLS;
+        auto rows_at = [&](int step, u32x4 (&x)[TP]) {
+            const unsigned short* xs = x0 + (((2 * step + (lane >> 5)) ^ fx) * 8);
+#pragma unroll
+            for (int k = 0; k < TP; ++k) x[k] = *reinterpret_cast<const u32x4*>(xs + 32 * k * COLS);
+        };
+        u32x4 x[2][TP];
+        rows_at(0, x[0]);
+#pragma unroll 1
+        for (int s0 = 0; s0 < size; s0 += AHEAD) {      // (a multiple of 4)
+#pragma unroll
+            for (int u = 0; u < AHEAD; ++u) {
+                const int st = s0 + u;
+                rows_at(st + 1 < size ? st + 1 : st, x[(u + 1) & 1]);       // (the last ones again: no branch)
+#pragma unroll
+                for (int i = 0; i < TO; ++i)
+#pragma unroll
+                    for (int k = 0; k < TP; ++k) acc[i][k] = mfma<T>(w[u][i], x[u & 1][k], acc[i][k]);
+                const bool here = st + AHEAD < size;
+                weights(here ? wl : wn, here ? st + AHEAD : st + AHEAD - size, w[u]);
+                __builtin_amdgcn_sched_barrier(0);      // (left alone, the compiler moves these loads down to their use)
+            }
+        }
+        if (s + 1 < count) stage(b ^ 1);
+        if (s + 2 < count) { load(in); next(in); }
+        if (now.piece == pieces - 1 && o0 < a.o) {
+            const long p0 = now.tile * TALL_ROWS;
+#pragma unroll
+            for (int k = 0; k < TP; ++k) {
+                const long p = p0 + 32 * k;
+                const Out out{static_cast<char*>(a.y) + (p * a.ldy + o0) * 2, a.codes + p * o32 + o0, a.scales + p * (o32 >> 5) + (o0 >> 5), 2 * a.ldy, o32, (int)min(a.n - p, 32L), a.o - o0};
+                write_rows64<T, MODE>(a, acc[0][k], acc[1][k], out, lane, wins + 2560 * wave);
+            }
+        }
+        now = after;
+        __syncthreads();
+    }
+}
+
 // --------------------------------------------------------------------------------------------------------------------------------- dW = dZ^T X, db
-// One workgroup = 128 outputs x 128 input columns over its piece of the rows, 4 waves of 64 x 64; BR rows a step.  Both operands lie with the REDUCTION index as the row, as
+// One workgroup = a square tile of outputs x input columns over its piece of the rows, BR rows a step.  Both operands lie with the REDUCTION index as the row, as
 // they do in memory, and are turned by the transposing LDS read.  The pieces' sums go to `part` and are added in order by k_dense_weights_sum: no atomics, the same
 // bits every time.
-template <int T>
-__global__ __launch_bounds__(256, 2) void k_dense_weights(DenseWeights a) {
-    constexpr int PARTS = T == LT_F32 ? 3 : 1, BR = T == LT_F32 ? 32 : 64;
-    constexpr int PLANE = BR * 128, NC = BR * 16 / 256;
-    __shared__ __attribute__((aligned(16))) unsigned short lds[(PARTS + 1) * PLANE];
-    unsigned short* zt = lds;
-    unsigned short* xt = lds + PARTS * PLANE;
-    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-    const int kt = (a.k + 127) / 128, ot = (a.o + 127) / 128, tiles = kt * ot;
+//
+// W = 128: 4 waves, two workgroups on a compute unit; W = 256: 16 waves, half as many reads of either operand.  A wave takes 64 x 64.
+template <int T, int W>
+__global__ __launch_bounds__(W * W / 64, W == 256 ? 4 : 2) void k_dense_weights(DenseWeights a) {
+    constexpr int PARTS = T == LT_F32 ? 3 : 1, BR = T == LT_F32 ? 32 : 64, NT = W * W / 64, TO = 2, TK = 2;
+    constexpr int RT = W / 8, RP = NT / RT, NC = BR / RP;      // threads a row of a tile, rows at a time, 8-column chunks a thread stages
+    constexpr int PLANE = BR * W, BUFFER = (PARTS + 1) * PLANE;
+    __shared__ __attribute__((aligned(16))) unsigned short lds[2 * BUFFER];
+    static_assert(NC >= 1 && NC <= BR / 16, "a chunk for each step of 16 rows at most");
+    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+    const int kt = (a.k + W - 1) / W, ot = (a.o + W - 1) / W, tiles = kt * ot;
     const long j = blockIdx.x >> 3;
     const int split = (int)(j / tiles) * 8 + (blockIdx.x & 7);
     if (split >= a.splits) return;
-    const int tile = (int)(j % tiles), k0 = (tile % kt) * 128, o0 = (tile / kt) * 128;
+    const int tile = (int)(j % tiles), k0 = (tile % kt) * W, o0 = (tile / kt) * W;
     const long steps = (a.n + BR - 1) / BR;
     const long s0 = steps * split / a.splits, s1 = steps * (split + 1) / a.splits;
     const int k32 = (a.k + 31) & ~31, o32 = (a.o + 31) & ~31;
-    const int cc = 8 * (t & 15);                       // the thread's 8 columns of either tile (the same in every step), rows t / 16 + 16 i
-    const bool sums = a.db != nullptr && k0 == 0;
+    // the thread's 8 columns of either tile are the same in every step; its rows: t / RT + RP * i.  Addresses are a scalar base that moves with the steps and 32-bit offsets
+    const int cc = 8 * (t % RT), row = t / RT;
+    // (columns beyond the outputs or inputs: any, their sums are not written)
+    const int zc = o0 + cc < a.o ? o0 + cc : 0, xc0 = k0 + cc < k32 ? k0 + cc : 0;
+    const unsigned zo = (unsigned)(row * (int)a.lddy + zc) * Bytes<T>::v, oo = row * o32 + zc, co = row * k32 + xc0, so = row * (k32 >> 5) + (xc0 >> 5);
+    const char* zb = static_cast<const char*>(a.dy) + s0 * BR * a.lddy * Bytes<T>::v;
+    const uint8_t *ob = a.open + s0 * BR * o32, *cb = a.x.codes + s0 * BR * k32, *sb = a.x.scales + s0 * BR * (k32 >> 5);
+    const long rows = a.n - s0 * BR;
+    const bool whole = (a.o & 7) == 0;          // every 8-column chunk of dY is whole or absent
 
     Raw8<T> zr[NC];
     u32x2 cr[NC], xc[NC];
     unsigned xs[NC];
-    auto load = [&](long step) {
-#pragma unroll
-        for (int i = 0; i < NC; ++i) {
-            const long p = step * BR + (t >> 4) + 16 * i;
-            const bool in = p < a.n;
-            zr[i] = in ? load8<T>(static_cast<const char*>(a.dy) + p * a.lddy * Bytes<T>::v, o0 + cc, a.o) : zero8<T>();
-            cr[i] = u32x2{0x01010101u, 0x01010101u};
-            if (a.open && in && o0 + cc < o32) cr[i] = *reinterpret_cast<const u32x2*>(a.open + p * o32 + o0 + cc);
-            const bool inx = in && k0 + cc < k32;
-            xc[i] = inx ? *reinterpret_cast<const u32x2*>(a.x.codes + p * k32 + k0 + cc) : u32x2{0, 0};
-            xs[i] = inx ? a.x.scales[p * (k32 >> 5) + ((k0 + cc) >> 5)] : 256u;      // (256: beyond the rows or columns)
-        }
+    auto load_whole = [&](long step, int i) {   // (step counts from s0) every row and chunk is there: straight code, the loads travel together
+        const long at = step * BR + RP * i;
+        const char* z = zb + at * a.lddy * Bytes<T>::v;
+        zr[i].q[0] = load16(z + zo);
+        if constexpr (T == LT_F32) zr[i].q[1] = load16(z + zo + 16);
+        if (a.open) cr[i] = *reinterpret_cast<const u32x2*>(ob + at * o32 + oo);
+        xc[i] = *reinterpret_cast<const u32x2*>(cb + at * k32 + co);
+        xs[i] = (sb + at * (k32 >> 5))[so];
     };
-    // the bias gradient is one sum over all rows, with nothing to average an error out: 64 bits from one step to the next (and within a step for float32, whose terms fill fp32)
-    double bs[8] = {0., 0., 0., 0., 0., 0., 0., 0.};
-    auto stage = [&]() {
-        float few[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    auto load = [&](long step, int i) {
+        const long at = step * BR + RP * i;
+        const bool in = at + row < rows;
+        zr[i] = in ? load8<T>(zb + at * a.lddy * Bytes<T>::v + zo, 0, a.o - zc) : zero8<T>();
+        if (a.open && in) cr[i] = *reinterpret_cast<const u32x2*>(ob + at * o32 + oo);
+        xc[i] = in ? *reinterpret_cast<const u32x2*>(cb + at * k32 + co) : u32x2{0, 0};
+        xs[i] = in ? (sb + at * (k32 >> 5))[so] : 127u;
+    };
+    auto stage = [&](unsigned short* zt, int i) {
+        unsigned short* xt = zt + PARTS * PLANE;
+        const int at = across<W>(row + RP * i, (t % RT) >> 2) + 8 * (t & 3);
+        if (a.open) close8<T>(zr[i], cr[i]);
+        stage8<T>(zt + at, PLANE, zr[i]);
+        float f[8];
+        decode8(xc[i], xs[i], a.x.is_signed != 0, f);
+        u32x4 v;
 #pragma unroll
-        for (int i = 0; i < NC; ++i) {
-            const int at = across((t >> 4) + 16 * i, (t & 15) >> 2) + 8 * (t & 3);
-            close8<T>(zr[i], cr[i]);
-            stage8<T>(zt + at, PLANE, zr[i]);
-            if (sums) {
-                float f[8];
-                to_floats<T>(zr[i], f);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    if constexpr (T == LT_F32) bs[e] += (double)f[e];
-                    else few[e] += f[e];
-                }
-            }
-            float f[8];
-            decode8(xc[i], xs[i] & 255u, a.x.is_signed != 0, f);
-            u32x4 v;
-#pragma unroll
-            for (int e = 0; e < 4; ++e)      // a value has at most 8 significant bits: its upper 16 bits are all of it
-                v[e] = T == LT_F16 ? pack2<LT_F16>(f[2 * e], f[2 * e + 1])
-                                   : __builtin_amdgcn_perm(as_bits(f[2 * e + 1]), as_bits(f[2 * e]), 0x07060302u);
-            if (xs[i] == 256u) v = u32x4{0, 0, 0, 0};
-            *reinterpret_cast<u32x4*>(xt + at) = v;
-        }
-        if (T != LT_F32 && sums)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) bs[e] += (double)few[e];
+        for (int e = 0; e < 4; ++e)      // a value has at most 8 significant bits: its upper 16 bits are all of it
+            v[e] = T == LT_F16 ? pack2<LT_F16>(f[2 * e], f[2 * e + 1]) : __builtin_amdgcn_perm(as_bits(f[2 * e + 1]), as_bits(f[2 * e]), 0x07060302u);
+        *reinterpret_cast<u32x4*>(xt + at) = v;
     };
 
-    const int wo = (wave >> 1) * 2, wk = (wave & 1) * 2;      // the wave's first 32-wide tile of either side
-    f32x16 acc[2][2];
+    const int wo = (wave / (W / 64)) * TO, wk = (wave % (W / 64)) * TK;      // the wave's first 32-wide tile of either side
+    f32x16 acc[TO][TK];
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < TO; ++i)
 #pragma unroll
-        for (int k = 0; k < 2; ++k) acc[i][k] = f32x16{0};
-    if (s0 < s1) load(s0);
-    for (long s = s0; s < s1; ++s) {
-        if (s > s0) __syncthreads();
-        stage();
+        for (int k = 0; k < TK; ++k) acc[i][k] = f32x16{0};
+    // The bias gradient falls off the fragments (a lane has 8 rows of one output), in the waves of the first column tile.  It is one sum over all rows with nothing to average an
+    // error out: added up in 64 bits
+    const bool sums = a.db != nullptr && k0 == 0 && wk == 0;
+    double bs[TO] = {0.0, 0.0};
+    auto multiply = [&](const unsigned short* zt, int ks) {
+        const unsigned short* xt = zt + PARTS * PLANE;
+        u32x4 x[TK][1];
+#pragma unroll
+        for (int k = 0; k < TK; ++k) x[k][0] = frag_across<W>(xt, wk + k, ks, lane);
+#pragma unroll
+        for (int i = 0; i < TO; ++i) {
+            u32x4 z[PARTS];
+#pragma unroll
+            for (int q = 0; q < PARTS; ++q) z[q] = frag_across<W>(zt + q * PLANE, wo + i, ks, lane);
+#pragma unroll
+            for (int k = 0; k < TK; ++k) acc[i][k] = product<T, PARTS, 1>(z, x[k], acc[i][k]);
+            if (sums)
+#pragma unroll
+                for (int q = 0; q < PARTS; ++q) {
+                    Raw8<T == LT_F16 ? LT_F16 : LT_BF16> v;
+                    v.q[0] = z[q];
+                    float f[8];
+                    to_floats<T == LT_F16 ? LT_F16 : LT_BF16>(v, f);
+                    bs[i] += (double)(((f[0] + f[1]) + (f[2] + f[3])) + ((f[4] + f[5]) + (f[6] + f[7])));
+                }
+        }
+    };
+    // One barrier a step: while a step's products run, the next one's elements — already in registers — are masked, decoded and written to the other buffer, a chunk between
+    // 16 rows of products and the next, and the chunk's registers are asked for the step after that: a load has a whole step to arrive
+    const long count = s1 - s0;
+    if (count > 0) {
+#pragma unroll
+        for (int i = 0; i < NC; ++i) load(0, i);
+#pragma unroll
+        for (int i = 0; i < NC; ++i) {
+            stage(lds, i);
+            if (count > 1) load(1, i);
+        }
         __syncthreads();
-        if (s + 1 < s1) load(s + 1);
+        long s = 0;
+        const long full = whole ? rows / BR - 2 : -1;      // steps whose next but one is whole
+        for (; s + 2 < count && s < full; ++s) {
+            const int b = (int)s & 1;
 #pragma unroll
-        for (int ks = 0; ks < BR / 16; ++ks) {
-            u32x4 x[2][1];
-#pragma unroll
-            for (int k = 0; k < 2; ++k) x[k][0] = frag_across(xt, wk + k, ks, lane);
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                u32x4 z[PARTS];
-#pragma unroll
-                for (int q = 0; q < PARTS; ++q) z[q] = frag_across(zt + q * PLANE, wo + i, ks, lane);
-#pragma unroll
-                for (int k = 0; k < 2; ++k) acc[i][k] = product<T, PARTS, 1>(z, x[k], acc[i][k]);
+            for (int i = 0; i < BR / 16; ++i) {
+                if (i < NC) {
+                    stage(lds + (b ^ 1) * BUFFER, i);
+                    load_whole(s + 2, i);
+                }
+                multiply(lds + b * BUFFER, i);
             }
+            __syncthreads();
+        }
+        for (; s < count; ++s) {
+            const int b = (int)s & 1;
+#pragma unroll
+            for (int i = 0; i < BR / 16; ++i) {
+                if (i < NC && s + 1 < count) {
+                    stage(lds + (b ^ 1) * BUFFER, i);
+                    if (s + 2 < count) load(s + 2, i);
+                }
+                multiply(lds + b * BUFFER, i);
+            }
+            __syncthreads();
         }
     }
     const bool last = a.splits == 1;
@@ -385,9 +755,9 @@ __global__ __launch_bounds__(256, 2) void k_dense_weights(DenseWeights a) {
         else static_cast<unsigned short*>(to)[at] = (unsigned short)pack2<T == LT_F32 ? LT_F16 : T>(v, 0.0f);
     };
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < TO; ++i)
 #pragma unroll
-        for (int k = 0; k < 2; ++k)
+        for (int k = 0; k < TK; ++k)
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
                 const int o = o0 + 32 * (wo + i) + (r & 3) + 8 * (r >> 2) + 4 * (lane >> 5), c = k0 + 32 * (wk + k) + (lane & 31);
@@ -396,20 +766,16 @@ __global__ __launch_bounds__(256, 2) void k_dense_weights(DenseWeights a) {
                     else a.part[((long)split * a.o + o) * a.k + c] = acc[i][k][r];
                 }
             }
-    if (sums) {      // 16 threads hold sums of the same 8 columns
-        __syncthreads();
-        double* f = reinterpret_cast<double*>(lds);
+    if (sums)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) f[(t >> 4) * 128 + cc + e] = bs[e];
-        __syncthreads();
-        if (t < 128 && o0 + t < a.o) {
-            double s = 0.0;
-#pragma unroll
-            for (int i = 0; i < 16; ++i) s += f[i * 128 + t];
-            if (last) put(a.db, o0 + t, (float)s);
-            else a.bias_part[(long)split * a.o + o0 + t] = s;
+        for (int i = 0; i < TO; ++i) {
+            const double s = bs[i] + __shfl_xor(bs[i], 32);
+            const int o = o0 + 32 * (wo + i) + lane;
+            if (lane < 32 && o < a.o) {
+                if (last) put(a.db, o, (float)s);
+                else a.bias_part[(long)split * a.o + o] = s;
+            }
         }
-    }
 }
 
 template <int T> __global__ __launch_bounds__(256) void k_dense_weights_sum(DenseWeights a) {
@@ -437,10 +803,8 @@ template <int T> __global__ __launch_bounds__(256) void k_checkpoint(const char*
         const bool in = i < total;
         const long p = in ? i / cpr : 0;
         const int c = 8 * (int)(in ? i - p * cpr : 0);
-        float f[8];
-        to_floats<T>(in ? load8<T>(x + p * ld * Bytes<T>::v, c, k) : zero8<T>(), f);
         u32x2 q; unsigned s;
-        encode8(f, is_signed != 0, q, s);
+        encode8<T>(in ? load8<T>(x + p * ld * Bytes<T>::v, c, k) : zero8<T>(), is_signed != 0, q, s);
         if (in) {
             *reinterpret_cast<u32x2*>(codes + 8 * i) = q;
             if ((c & 31) == 0) scales[i >> 2] = (uint8_t)s;
@@ -461,17 +825,71 @@ template <int T> __global__ __launch_bounds__(256) void k_checkpoint_values(Chec
     }
 }
 
-template <int T> hipError_t dense_rows(bool dx, const DenseRows& a, hipStream_t s) {
-    const long pt = (a.n + 127) / 128, ot = (a.o + 127) / 128;
-    const dim3 grid((unsigned)((pt + 7) / 8 * 8 * ot));
-    if (dx) hipLaunchKernelGGL((k_dense_rows<T, true, 128, 128>), grid, dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((k_dense_rows<T, false, 128, 128>), grid, dim3(256), 0, s, a);
+// Which form Y = act(A B + bias) runs in, and the fragments' memory: the tall form for the 16-bit types once its tiles of 128 rows give every compute unit one (rows of 8
+// elements at least: it reads whole chunks; and as long as the biases of all passes fit LDS beside the two buffers).  A pass makes 256 outputs.
+struct RowsPlan { bool tall; int passes, steps; };
+RowsPlan rows_plan(int type, long n, int r, int o) {
+    RowsPlan p{};
+    p.passes = (o + 255) / 256;
+    p.tall = type != LT_F32 && n >= 256 * TALL_ROWS && r >= 8 && p.passes <= 8;
+    p.steps = (r + 63) / 64 * 4;
+    return p;
+}
+
+template <int T, int MODE, int COLS> hipError_t dense_tall(const DenseRows& a, const RowsPlan& p, u32x4* wf, hipStream_t s) {
+    const int tiles = p.passes * 8;
+    const size_t bytes = 4 * (size_t)TALL_ROWS * COLS + 4 * 2560 + p.passes * 256 * 4;
+    // (once for each device and kernel: more LDS than the default 64 KB)
+    int dev = 0;
+    hipError_t e = hipGetDevice(&dev);
+    if (e != hipSuccess) return e;
+    static std::atomic<unsigned long long> set{0};
+    if (dev > 63 || !(set.load(std::memory_order_acquire) >> dev & 1)) {
+        e = hipFuncSetAttribute(reinterpret_cast<const void*>(&k_dense_tall<T, MODE, COLS>), hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
+        if (e != hipSuccess) return e;
+        if (dev <= 63) set.fetch_or(1ull << dev, std::memory_order_release);
+    }
+    hipLaunchKernelGGL((k_dense_fragments<T, MODE == TALL_DX>), dim3((unsigned)(tiles * (p.steps / 4))), dim3(256), 0, s, a, wf, tiles, p.steps);
+    hipLaunchKernelGGL((k_dense_tall<T, MODE, COLS>), dim3(512), dim3(256), bytes, s, a, wf, p.passes);
+    return hipGetLastError();
+}
+template <int T, int MODE> hipError_t dense_tall(const DenseRows& a, const RowsPlan& p, u32x4* wf, hipStream_t s) {
+    return a.r <= 64 ? dense_tall<T, MODE, 64>(a, p, wf, s) : dense_tall<T, MODE, 128>(a, p, wf, s);
+}
+
+template <int T, bool DX> hipError_t dense_rows(const DenseRows& a, void* ws, hipStream_t s) {
+    const RowsPlan p = rows_plan(T, a.n, a.r, a.o);
+    if constexpr (T != LT_F32) {
+        if (p.tall) {
+            u32x4* wf = static_cast<u32x4*>(ws);
+            if constexpr (DX) return dense_tall<T, TALL_DX>(a, p, wf, s);
+            else return !a.codes ? dense_tall<T, TALL_Y>(a, p, wf, s) : a.relu ? dense_tall<T, TALL_RELU_KEEP>(a, p, wf, s) : dense_tall<T, TALL_KEEP>(a, p, wf, s);
+        }
+    }
+    const long pt = ((a.n + 127) / 128 + 7) / 8 * 8;
+    hipLaunchKernelGGL((k_dense_rows<T, DX, 128, 128>), dim3((unsigned)(pt * ((a.o + 127) / 128))), dim3(256), 0, s, a);
     return hipGetLastError();
 }
 
+// The weight gradient's tile and how many pieces the rows are cut into (functions of the sizes alone)
+struct WeightsPlan { int width, tiles, splits; };
+WeightsPlan weights_plan(int type, long n, int k, int o) {
+    WeightsPlan p;
+    const long t4 = (long)((k + 127) / 128) * ((o + 127) / 128), t8 = (long)((k + 255) / 256) * ((o + 255) / 256);
+    p.width = 2 * 4 * t8 <= 3 * t4 ? 256 : 128;
+    p.tiles = (int)(p.width == 256 ? t8 : t4);
+    const long steps = type == LT_F32 ? (n + 31) / 32 : (n + 63) / 64, fill = p.width == 256 ? 256 : 512;      // one or two workgroups for each of the 256 compute units
+    long s = fill / p.tiles;
+    if (s > steps) s = steps;
+    p.splits = (int)(s < 1 ? 1 : s);
+    return p;
+}
+
 template <int T> hipError_t dense_weights(const DenseWeights& a, hipStream_t s) {
-    const long tiles = (long)((a.k + 127) / 128) * ((a.o + 127) / 128);
-    hipLaunchKernelGGL((k_dense_weights<T>), dim3((unsigned)((a.splits + 7) / 8 * 8 * tiles)), dim3(256), 0, s, a);
+    const WeightsPlan p = weights_plan(T, a.n, a.k, a.o);
+    const dim3 grid((unsigned)((p.splits + 7) / 8 * 8 * p.tiles));
+    if (p.width == 256) hipLaunchKernelGGL((k_dense_weights<T, 256>), grid, dim3(1024), 0, s, a);
+    else hipLaunchKernelGGL((k_dense_weights<T, 128>), grid, dim3(256), 0, s, a);
     if (a.splits > 1) {
         const long m = (long)a.o * a.k + a.o;
         hipLaunchKernelGGL((k_dense_weights_sum<T>), dim3((unsigned)((m + 255) / 256)), dim3(256), 0, s, a);
@@ -486,15 +904,16 @@ unsigned chunk_grid(long n, int k) {
 
 }  // namespace
 
-int dense_weight_splits(long n, int k, int o, int type) {
-    const long tiles = (long)((k + 127) / 128) * ((o + 127) / 128), steps = (n + (type == LT_F32 ? 31 : 63)) / (type == LT_F32 ? 32 : 64);
-    long s = 1024 / tiles;      // four workgroups for each of the 256 compute units
-    if (s > steps) s = steps;
-    return (int)(s < 1 ? 1 : s);
+int dense_weight_splits(int type, long n, int k, int o) { return weights_plan(type, n, k, o).splits; }
+
+size_t dense_rows_bytes(int type, long n, int r, int o) {
+    const RowsPlan p = rows_plan(type, n, r, o);
+    return p.tall ? (size_t)p.passes * 8 * p.steps * 1024 : 0;
 }
 
-hipError_t launch_dense_rows(int type, bool input_gradient, const DenseRows& a, hipStream_t s) {
-    return type == LT_F32 ? dense_rows<LT_F32>(input_gradient, a, s) : type == LT_BF16 ? dense_rows<LT_BF16>(input_gradient, a, s) : dense_rows<LT_F16>(input_gradient, a, s);
+hipError_t launch_dense_rows(int type, bool input_gradient, const DenseRows& a, void* ws, hipStream_t s) {
+    if (input_gradient) return type == LT_F32 ? dense_rows<LT_F32, true>(a, ws, s) : type == LT_BF16 ? dense_rows<LT_BF16, true>(a, ws, s) : dense_rows<LT_F16, true>(a, ws, s);
+    return type == LT_F32 ? dense_rows<LT_F32, false>(a, ws, s) : type == LT_BF16 ? dense_rows<LT_BF16, false>(a, ws, s) : dense_rows<LT_F16, false>(a, ws, s);
 }
 
 hipError_t launch_dense_weights(int type, const DenseWeights& a, hipStream_t s) {

@@ -16,7 +16,9 @@ typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+typedef short s16x2 __attribute__((ext_vector_type(2)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 
 template <int T> struct Bytes { static constexpr int v = T == LT_F32 ? 4 : 2; };
@@ -24,6 +26,8 @@ template <int T> struct Bytes { static constexpr int v = T == LT_F32 ? 4 : 2; };
 // (by value: __builtin_bit_cast of a vector's element reads element 0)
 __device__ __forceinline__ float as_float(unsigned u) { return __builtin_bit_cast(float, u); }
 __device__ __forceinline__ unsigned as_bits(float f) { return __builtin_bit_cast(unsigned, f); }
+
+__device__ __forceinline__ float half_float(unsigned bits) { return (float)__builtin_bit_cast(_Float16, (unsigned short)bits); }
 
 // eight consecutive elements of a row as they lie in memory: 16 bytes (16-bit types) or 32 (float32)
 template <int T> struct Raw8 { u32x4 q[T == LT_F32 ? 2 : 1]; };

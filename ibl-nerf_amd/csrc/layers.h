@@ -26,7 +26,8 @@ struct DenseRows {
     long n; int r, o;
     int relu, is_signed;
 };
-hipError_t launch_dense_rows(int type, bool input_gradient, const DenseRows& a, hipStream_t s);
+size_t dense_rows_bytes(int type, long n, int r, int o);      // scratch memory of the launch
+hipError_t launch_dense_rows(int type, bool input_gradient, const DenseRows& a, void* ws, hipStream_t s);
 
 // dW [o][k] = sum_p dZ[p][o] X[p][k], db [o] = sum_p dZ[p][o];  dZ = dY where `open` is nonzero (or everywhere: null)
 struct DenseWeights {
@@ -40,7 +41,7 @@ struct DenseWeights {
     long n; int k, o;
     int splits;
 };
-int dense_weight_splits(long n, int k, int o, int type);      // how many pieces the rows are cut into (a function of the sizes alone: results repeat bit for bit)
+int dense_weight_splits(int type, long n, int k, int o);      // how many pieces the rows are cut into (a function of the sizes alone: results repeat bit for bit)
 hipError_t launch_dense_weights(int type, const DenseWeights& a, hipStream_t s);
 
 hipError_t launch_checkpoint(int type, const void* x, long ld, long n, int k, int is_signed, uint8_t* codes, uint8_t* scales, hipStream_t s);

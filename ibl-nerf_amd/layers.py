@@ -20,7 +20,7 @@ import torch
 from . import binding as B
 
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
-MAX_COLUMNS = 65536
+MAX_COLUMNS, MAX_STRIDE = 65536, 1 << 24
 
 
 def _type(t, what):
@@ -53,9 +53,14 @@ def _rows(t, what):
     k = t.shape[-1]
     if t.dim() != 2:
         t = t.reshape(-1, k) if t.numel() else t.new_empty((0, k))
-    if (k > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < k):
+    if (k > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and not k <= t.stride(0) <= MAX_STRIDE):
         t = t.contiguous()
     return t, (t.stride(0) if t.shape[0] > 1 else k)
+
+
+def _workspace(size, device):
+    """Scratch memory of one call from torch's allocator: reused in stream order, a captured graph's from the graph's own pool."""
+    return (torch.empty((size,), dtype=torch.uint8, device=device), size) if size else (None, 0)
 
 
 class Checkpoint:
@@ -130,9 +135,10 @@ def dense_forward(x, weight, bias=None, relu=False, keep=True):
         bias = bias.detach().contiguous()
     y = torch.empty((n, o), dtype=x.dtype, device=x.device)
     codes, scales = _codes_like(x, n, o) if keep else (None, None)
+    ws, ws_bytes = _workspace(lib.iblnerf_dense_forward_workspace(t, n, k, o), x.device)
     with guard:
         B.check_layers(lib.iblnerf_dense_forward(stream, t, x.data_ptr(), ld, n, k, w.data_ptr(), ldw, o, None if bias is None else bias.data_ptr(), int(bool(relu)), y.data_ptr(), o,
-                                                 codes.data_ptr() if keep else None, scales.data_ptr() if keep else None))
+                                                 codes.data_ptr() if keep else None, scales.data_ptr() if keep else None, None if ws is None else ws.data_ptr(), ws_bytes))
     return y.reshape(lead + (o,)), (Checkpoint(codes, scales, o, not relu) if keep else None)
 
 
@@ -162,11 +168,11 @@ def dense_backward(dy, x, weight, relu=None, need_dx=True, need_dw=True, need_db
     dx = torch.empty((n, k), dtype=dy.dtype, device=dev) if need_dx else None
     dw = torch.empty((o, k), dtype=grad_dtype, device=dev) if need_dw or need_db else None
     db = torch.empty((o,), dtype=grad_dtype, device=dev) if need_db else None
-    ws = torch.empty((lib.iblnerf_dense_backward_workspace(t, n, k, o),), dtype=torch.uint8, device=dev) if dw is not None else None
+    ws, ws_bytes = _workspace(lib.iblnerf_dense_backward_workspace(t, n, k, o), dev)
     with guard:
         B.check_layers(lib.iblnerf_dense_backward(stream, t, dy.data_ptr(), ld, n, k, o, x.codes.data_ptr(), x.scales.data_ptr(), int(x.signed), None if relu is None else relu.codes.data_ptr(),
                                                   w.data_ptr(), ldw, None if dx is None else dx.data_ptr(), k, _TYPES[grad_dtype], None if dw is None else dw.data_ptr(),
-                                                  None if db is None else db.data_ptr(), None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel()))
+                                                  None if db is None else db.data_ptr(), None if ws is None else ws.data_ptr(), ws_bytes))
     return (None if dx is None else dx.reshape(lead + (k,))), (dw if need_dw else None), db
 
 
@@ -227,7 +233,7 @@ def _lookup(table, index, scale, rows_per_index, out):
         out = torch.empty(shape, dtype=table.dtype, device=table.device)
     else:
         _same(out, table, "out", table.dtype)
-        if out.dim() != 2 or tuple(out.shape) != (n * per, d) or (d > 1 and out.stride(1) != 1) or (out.shape[0] > 1 and out.stride(0) < d):
+        if out.dim() != 2 or tuple(out.shape) != (n * per, d) or (d > 1 and out.stride(1) != 1) or (out.shape[0] > 1 and not d <= out.stride(0) <= MAX_STRIDE):
             raise ValueError("out must be [%d, %d] with unit stride along a row, got %s strides %s" % (n * per, d, tuple(out.shape), tuple(out.stride())))
     ld_out = out.stride(0) if out.dim() == 2 and out.shape[0] > 1 else d
     with guard:

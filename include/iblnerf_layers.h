@@ -8,8 +8,8 @@
  *     captured graph needs one of its own).  Calls from several threads, on several streams and devices are independent; the stream must belong to the current device, and
  *     the tensors must lie on it.
  *   - iblnerf_layers_last_error() has the message of the calling thread's last failure.
- *   - `dtype` is the type T of every tensor of the call but indices, codes and scale bytes; sums are held in fp32 and rounded once.  Row strides ("ld_") are in elements
- *     and at least the row's length; pointers need the alignment of their element type (codes: 8 bytes, workspace: 16 bytes).
+ *   - `dtype` is the type T of every tensor of the call but indices, codes and scale bytes; sums are held in fp32 and rounded once.  Row strides ("ld_") are in elements,
+ *     at least the row's length and at most 2^24; pointers need the alignment of their element type (codes: 8 bytes, workspace: 16 bytes).
  *   - inputs and outputs of a call may not overlap.
  *   - results depend on the inputs alone: the same call gives the same bits. */
 #ifndef IBLNERF_LAYERS_H
@@ -35,8 +35,9 @@ int iblnerf_checkpoint_values(void* stream, const uint8_t* d_codes, const uint8_
 /* y [n, o] = x [n, k] w^T + bias (w [o, k] as nn.Linear holds it; bias [o] or NULL), negative values to 0 if relu; with d_codes / d_scales (both or neither) also y's
  * checkpoint, unsigned if relu, else signed.  float32 products are taken in six bfloat16 products of the operands' exact three-part splits (about fp32's own accuracy; an
  * operand that is infinite or beyond 3.39e38 gives NaN). */
+size_t iblnerf_dense_forward_workspace(int dtype, int64_t n, int k, int o);
 int iblnerf_dense_forward(void* stream, int dtype, const void* d_x, int64_t ld_x, int64_t n, int k, const void* d_w, int64_t ld_w, int o, const void* d_bias, int relu,
-                          void* d_y, int64_t ld_y, uint8_t* d_codes, uint8_t* d_scales);
+                          void* d_y, int64_t ld_y, uint8_t* d_codes, uint8_t* d_scales, void* d_workspace, size_t workspace_bytes);
 
 /* The backward of that layer from the checkpoint of its input (d_x_codes / d_x_scales, x_is_signed) and, under a ReLU, of its output (d_y_codes; NULL: no ReLU):
  *   dZ = dY where the output's code is not 0 (elsewhere 0, whatever dY holds there);  dX [n, k] = dZ w;  dW [o, k] = dZ^T X;  db [o] = sum over the rows of dZ

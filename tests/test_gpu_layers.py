@@ -133,6 +133,25 @@ def test_dense_backward(n, k, o, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,k,o", [(33001, 70, 130), (32900, 40, 24), (40000, 3, 300), (33000, 200, 512)])
+def test_dense_many_rows(n, k, o, dtype):
+    """more row tiles than compute units: the forms for many rows, ragged in every size"""
+    g = gen(n + k + o)
+    x, w, b = randn(g, n, k, dtype=dtype), randn(g, o, k, dtype=dtype, scale=k ** -0.5), randn(g, o, dtype=dtype)
+    y, kept = L.dense_forward(x, w, b, relu=True)
+    R.close(y, (x.double() @ w.double().t() + b.double()).clamp_min(0), x.double().abs() @ w.double().abs().t() + b.double().abs(), k, dtype)
+    again = L.checkpoint(y, signed=False)                   # (held to the definition above)
+    assert torch.equal(kept.codes, again.codes) and torch.equal(kept.scales, again.scales)
+    dy = randn(g, n, o, dtype=dtype)
+    kx = L.checkpoint(x)
+    dx, dw, db = L.dense_backward(torch.where(y > 0, dy, torch.full_like(dy, float("nan"))), kx, w, relu=kept)
+    dz, xv = torch.where(y > 0, dy, torch.zeros_like(dy)).double(), kx.values().double()
+    R.close(dx, dz @ w.double(), dz.abs() @ w.double().abs(), o, dtype)
+    R.close(dw, dz.t() @ xv, dz.abs().t() @ xv.abs(), n // 4, dtype)
+    R.close(db, dz.sum(0), dz.abs().sum(0), n // 4, dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_dense_long_reduction(dtype):
     """many rows: the pieces of the weight gradient and their sum; 70 001 rows, more than one launch tile of each kind"""
     g = gen(11)

@@ -51,7 +51,7 @@ def refused(lib, rc, word):
 
 def test_c_checkpoint_refuses(lib):
     good = dict(dtype=0, x=P, ld=8, n=4, k=8, s=0, codes=P, scales=P)
-    for bad in (dict(dtype=3), dict(dtype=-1), dict(x=None), dict(ld=7), dict(n=-1), dict(n=1 << 31), dict(k=0), dict(k=65537), dict(codes=None), dict(scales=None),
+    for bad in (dict(dtype=3), dict(dtype=-1), dict(x=None), dict(ld=7), dict(ld=(1 << 24) + 1), dict(n=-1), dict(n=1 << 31), dict(k=0), dict(k=65537), dict(codes=None), dict(scales=None),
                 dict(codes=C.c_void_p((1 << 20) + 4)), dict(x=C.c_void_p((1 << 20) + 2))):
         a = dict(good, **bad)
         refused(lib, lib.iblnerf_checkpoint(None, a["dtype"], a["x"], a["ld"], a["n"], a["k"], a["s"], a["codes"], a["scales"]), "checkpoint")
@@ -64,7 +64,10 @@ def test_c_dense_refuses(lib):
     for bad in (dict(dtype=9), dict(x=None), dict(ldx=7), dict(n=-1), dict(k=0), dict(o=0), dict(o=1 << 17), dict(w=None), dict(ldw=7), dict(y=None), dict(ldy=4), dict(codes=None),
                 dict(scales=None), dict(b=C.c_void_p((1 << 20) + 1)), dict(codes=C.c_void_p((1 << 20) + 1)), dict(n=2147482000, o=65536, ldy=65536)):
         a = dict(good, **bad)
-        refused(lib, lib.iblnerf_dense_forward(None, a["dtype"], a["x"], a["ldx"], a["n"], a["k"], a["w"], a["ldw"], a["o"], a["b"], 1, a["y"], a["ldy"], a["codes"], a["scales"]), "dense_forward")
+        refused(lib, lib.iblnerf_dense_forward(None, a["dtype"], a["x"], a["ldx"], a["n"], a["k"], a["w"], a["ldw"], a["o"], a["b"], 1, a["y"], a["ldy"], a["codes"], a["scales"], P, 1 << 40), "dense_forward")
+    need = lib.iblnerf_dense_forward_workspace(1, 100000, 512, 512)
+    assert need > 0
+    refused(lib, lib.iblnerf_dense_forward(None, 1, P, 512, 100000, 512, P, 512, 512, P, 1, P, 512, P, P, P, need - 1), "workspace")
     good = dict(dtype=1, dy=P, ldy=5, n=400, k=8, o=5, xc=P, xs=P, yc=P, w=P, ldw=8, dx=P, ldx=8, gt=1, dw=P, db=P, ws=P, bytes=1 << 30)
     for bad in (dict(dtype=9), dict(dy=None), dict(ldy=4), dict(n=-1), dict(k=0), dict(o=0), dict(xc=None), dict(xs=None), dict(w=None), dict(ldw=7), dict(ldx=7), dict(gt=2), dict(dw=None),
                 dict(yc=C.c_void_p((1 << 20) + 1)), dict(ws=None), dict(bytes=8), dict(db=C.c_void_p((1 << 20) + 1))):
