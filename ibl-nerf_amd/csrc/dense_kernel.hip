@@ -21,10 +21,10 @@ namespace ibl {
 
 namespace {
 
-// eight elements into the matrix-operand planes in LDS: 16-bit types as they are, float32 as its three bfloat16 parts
-template <int T> __device__ __forceinline__ void stage8(unsigned short* dst, int plane, const Raw8<T>& v) {
+// eight elements as matrix operands: 16-bit types as they are, float32 as its three bfloat16 parts
+template <int T> struct Parts { static constexpr int n = T == LT_F32 ? 3 : 1; };
+template <int T> __device__ __forceinline__ void parts_of(const Raw8<T>& v, u32x4 (&part)[Parts<T>::n]) {
     if constexpr (T == LT_F32) {
-        u32x4 part[3];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             float x = as_float(v.q[i >> 1][2 * (i & 1)]), y = as_float(v.q[i >> 1][2 * (i & 1) + 1]);
@@ -36,11 +36,16 @@ template <int T> __device__ __forceinline__ void stage8(unsigned short* dst, int
                 y -= as_float(h & 0xffff0000u);
             }
         }
-#pragma unroll
-        for (int q = 0; q < 3; ++q) *reinterpret_cast<u32x4*>(dst + q * plane) = part[q];
     } else {
-        *reinterpret_cast<u32x4*>(dst) = v.q[0];
+        part[0] = v.q[0];
     }
+}
+// ... into their planes in LDS
+template <int T> __device__ __forceinline__ void stage8(unsigned short* dst, int plane, const Raw8<T>& v) {
+    u32x4 part[Parts<T>::n];
+    parts_of<T>(v, part);
+#pragma unroll
+    for (int q = 0; q < Parts<T>::n; ++q) *reinterpret_cast<u32x4*>(dst + q * plane) = part[q];
 }
 
 template <int T> __device__ __forceinline__ f32x16 mfma(u32x4 a, u32x4 b, f32x16 c) {
@@ -341,6 +346,105 @@ __global__ __launch_bounds__(256, 2) void k_dense_rows(DenseRows a) {
     __syncthreads();
 
     write_rows<T, DX, TO, TP>(a, acc, lds + wave * Window<TO, T>::bytes, p0 + wp, o0 + wo, lane);
+}
+
+// The form for few rows, where one latency after the other is what a call costs: a workgroup makes 32 rows x 32 outputs, each of its 4 waves over a quarter of the reduction, straight
+// from global memory (operands in the order they lie there, 4 steps asked for at once), and the quarters meet in LDS once.
+template <int T, bool DX>
+__global__ __launch_bounds__(256) void k_dense_few(DenseRows a) {
+    constexpr int U = 4, RS = 36;
+    __shared__ __attribute__((aligned(16))) float sums[4 * 32 * RS];
+    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), i = lane & 31, h = lane >> 5;
+    const int ot = (a.o + 31) >> 5, o0 = (int)(blockIdx.x % ot) * 32;
+    const long p0 = (long)(blockIdx.x / ot) * 32;
+    const int steps = (a.r + 15) >> 4, quarter = (steps + 3) >> 2, s1 = min(steps, (wave + 1) * quarter), r32 = (a.r + 31) & ~31;
+    const long p = min(p0 + i, a.n - 1);                 // (rows and outputs beyond the last: the last again, not written)
+    const int o = min(o0 + i, a.o - 1);
+    const char* x = static_cast<const char*>(a.a) + p * a.lda * Bytes<T>::v;
+    const char* w = static_cast<const char*>(a.w) + (DX ? (long)o : o * a.ldw) * Bytes<T>::v;
+    const bool whole = (a.r & 7) == 0;                   // every 8-element chunk of the reduction is whole or absent
+    f32x16 acc = {0};
+    for (int s0 = wave * quarter; s0 < s1; s0 += U) {
+        Raw8<T> xv[U], wv[U];
+        u32x2 q[U];
+        if (whole) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int k = min(16 * (s0 + u) + 8 * h, a.r - 8);
+                xv[u].q[0] = load16(x + (long)k * Bytes<T>::v);
+                if constexpr (T == LT_F32) xv[u].q[1] = load16(x + (long)k * 4 + 16);
+                q[u] = u32x2{0x01010101u, 0x01010101u};
+                if (DX && a.open) q[u] = *reinterpret_cast<const u32x2*>(a.open + p * r32 + k);
+                if (!DX) {
+                    wv[u].q[0] = load16(w + (long)k * Bytes<T>::v);
+                    if constexpr (T == LT_F32) wv[u].q[1] = load16(w + (long)k * 4 + 16);
+                } else {
+                    wv[u] = zero8<T>();
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        if constexpr (T == LT_F32) wv[u].q[e >> 2][e & 3] = *reinterpret_cast<const unsigned*>(w + (k + e) * a.ldw * 4);
+                        else wv[u].q[0][e >> 1] |= (unsigned)*reinterpret_cast<const unsigned short*>(w + (k + e) * a.ldw * 2) << (16 * (e & 1));
+                    }
+                }
+            }
+        } else {
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int k = 16 * (s0 + u) + 8 * h;
+                xv[u] = load8<T>(x, k, a.r);
+                q[u] = u32x2{0x01010101u, 0x01010101u};
+                if (DX && a.open && k < r32) q[u] = *reinterpret_cast<const u32x2*>(a.open + p * r32 + k);
+                if (!DX) {
+                    wv[u] = load8<T>(w, k, a.r);
+                } else {
+                    wv[u] = zero8<T>();
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        if (k + e < a.r) {
+                            if constexpr (T == LT_F32) wv[u].q[e >> 2][e & 3] = *reinterpret_cast<const unsigned*>(w + (k + e) * a.ldw * 4);
+                            else wv[u].q[0][e >> 1] |= (unsigned)*reinterpret_cast<const unsigned short*>(w + (k + e) * a.ldw * 2) << (16 * (e & 1));
+                        }
+                }
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (s0 + u >= s1) break;
+            if (DX) close8<T>(xv[u], q[u]);
+            if (16 * (s0 + u) + 8 * h >= a.r) xv[u] = wv[u] = zero8<T>();
+            u32x4 xp[Parts<T>::n], wp[Parts<T>::n];
+            parts_of<T>(xv[u], xp);
+            parts_of<T>(wv[u], wp);
+            acc = product<T, Parts<T>::n, Parts<T>::n>(wp, xp, acc);
+        }
+    }
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+        *reinterpret_cast<u32x4*>(sums + (wave * 32 + i) * RS + 8 * g + 4 * h) = u32x4{as_bits(acc[4 * g]), as_bits(acc[4 * g + 1]), as_bits(acc[4 * g + 2]), as_bits(acc[4 * g + 3])};
+    __syncthreads();
+    if (t >= 128) return;
+    const int row = t >> 2, c = 8 * (t & 3);
+    float f[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        float v = DX ? 0.0f : bias_at<T>(a, o0 + c + e);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) v += sums[(q * 32 + row) * RS + c + e];
+        if (!DX && a.relu) v = __builtin_elementwise_maximum(v, 0.0f);
+        f[e] = !DX && o0 + c + e >= a.o ? 0.0f : v;      // (columns beyond the layer's outputs are coded 0)
+    }
+    const Raw8<T> v = from_floats<T>(f);
+    const bool in = p0 + row < a.n;
+    if (in && o0 + c < a.o) store8<T>(static_cast<char*>(a.y) + (p0 + row) * a.ldy * Bytes<T>::v, o0 + c, a.o, v);
+    if (!DX && a.codes) {
+        u32x2 codes; unsigned scale;
+        encode8<T>(v, a.is_signed != 0, codes, scale);
+        const int o32 = (a.o + 31) & ~31;
+        if (in) {
+            *reinterpret_cast<u32x2*>(a.codes + (p0 + row) * o32 + o0 + c) = codes;
+            if (c == 0) a.scales[(p0 + row) * (o32 >> 5) + (o0 >> 5)] = (uint8_t)scale;
+        }
+    }
 }
 
 // The weights as matrix operands for k_dense_tall: [32-wide tile][16 reduction elements][lane][8], zeros beyond the layer
@@ -787,7 +891,7 @@ template <int T> __global__ __launch_bounds__(256) void k_dense_weights_sum(Dens
     if (bias) {
         for (int q = 0; q < a.splits; ++q) s += a.bias_part[(long)q * a.o + at];
     } else {
-#pragma unroll 8
+#pragma unroll 16
         for (int q = 0; q < a.splits; ++q) s += (double)a.part[q * nw + at];
     }
     void* to = bias ? a.db : a.dw;
@@ -824,6 +928,8 @@ template <int T> __global__ __launch_bounds__(256) void k_checkpoint_values(Chec
         store8<T>(out + p * ld * Bytes<T>::v, c, k, from_floats<T>(f));
     }
 }
+
+constexpr long FEW_TILES = 64;
 
 // Which form Y = act(A B + bias) runs in, and the fragments' memory: the tall form for the 16-bit types once its tiles of 128 rows give every compute unit one (rows of 8
 // elements at least: it reads whole chunks; and as long as the biases of all passes fit LDS beside the two buffers).  A pass makes 256 outputs.
@@ -866,6 +972,11 @@ template <int T, bool DX> hipError_t dense_rows(const DenseRows& a, void* ws, hi
             else return !a.codes ? dense_tall<T, TALL_Y>(a, p, wf, s) : a.relu ? dense_tall<T, TALL_RELU_KEEP>(a, p, wf, s) : dense_tall<T, TALL_KEEP>(a, p, wf, s);
         }
     }
+    // few tiles of 128 x 128: small ones instead
+    if (((a.n + 127) / 128) * ((a.o + 127) / 128) <= FEW_TILES) {
+        hipLaunchKernelGGL((k_dense_few<T, DX>), dim3((unsigned)(((a.n + 31) / 32) * ((a.o + 31) / 32))), dim3(256), 0, s, a);
+        return hipGetLastError();
+    }
     const long pt = ((a.n + 127) / 128 + 7) / 8 * 8;
     hipLaunchKernelGGL((k_dense_rows<T, DX, 128, 128>), dim3((unsigned)(pt * ((a.o + 127) / 128))), dim3(256), 0, s, a);
     return hipGetLastError();
@@ -876,11 +987,13 @@ struct WeightsPlan { int width, tiles, splits; };
 WeightsPlan weights_plan(int type, long n, int k, int o) {
     WeightsPlan p;
     const long t4 = (long)((k + 127) / 128) * ((o + 127) / 128), t8 = (long)((k + 255) / 256) * ((o + 255) / 256);
-    p.width = 2 * 4 * t8 <= 3 * t4 ? 256 : 128;
+    // 256 x 256 where that computes at most half as much again beyond the layer's edges and each of the 256 compute units has some steps to do; pieces of two steps at least
+    // (1 003 x 539 -> 512: 18 us; 25 in 256-wide tiles, 24 in pieces of one step)
+    const long steps = type == LT_F32 ? (n + 31) / 32 : (n + 63) / 64;
+    p.width = 2 * 4 * t8 <= 3 * t4 && steps * t8 >= 4 * 256 ? 256 : 128;
     p.tiles = (int)(p.width == 256 ? t8 : t4);
-    const long steps = type == LT_F32 ? (n + 31) / 32 : (n + 63) / 64, fill = p.width == 256 ? 256 : 512;      // one or two workgroups for each of the 256 compute units
-    long s = fill / p.tiles;
-    if (s > steps) s = steps;
+    long s = (p.width == 256 ? 256 : 512) / p.tiles;      // one workgroup a compute unit, or two
+    if (s > steps / 2) s = steps / 2;
     p.splits = (int)(s < 1 ? 1 : s);
     return p;
 }

@@ -16,7 +16,7 @@ namespace ibl {
 namespace {
 
 constexpr int SMALL = 4096;          // positions that one workgroup sorts in LDS
-constexpr int TILE = 4096;           // positions a workgroup of the large sort takes
+constexpr int TILE = 2048;           // positions a workgroup of the large sort takes
 constexpr int BINS = 512;            // at most 9 bits a pass
 
 __device__ __forceinline__ long index_at(const void* index, int index64, long i) {
@@ -60,9 +60,10 @@ template <int T> __global__ __launch_bounds__(256) void k_lookup(Lookup a) {
 
 // ------------------------------------------------------------------------------------------------------------------------------------------------ sorting
 // Lanes of the wave whose digit equals this lane's (only lanes with `in` count)
-__device__ __forceinline__ unsigned long long peers(unsigned digit, int bits, bool in) {
+__device__ __forceinline__ unsigned long long peers(unsigned digit, bool in) {
     unsigned long long m = __ballot(in);
-    for (int b = 0; b < bits; ++b) {
+#pragma unroll
+    for (int b = 0; b < 9; ++b) {      // (a shorter digit's upper bits are equal in all lanes)
         const bool one = (digit >> b) & 1;
         const unsigned long long v = __ballot(one);
         m &= one ? v : ~v;
@@ -71,8 +72,8 @@ __device__ __forceinline__ unsigned long long peers(unsigned digit, int bits, bo
 }
 
 // One stable pass over `rounds` x 64 keys of each wave: the key's rank among the wave's keys of the same digit, the wave's digit counts in hist[wave][BINS]
-template <int WAVES> __device__ __forceinline__ unsigned rank_in_wave(unsigned digit, int bits, bool in, unsigned* hist, int wave, int lane) {
-    const unsigned long long m = peers(digit, bits, in);
+template <int WAVES> __device__ __forceinline__ unsigned rank_in_wave(unsigned digit, bool in, unsigned* hist, int wave, int lane) {
+    const unsigned long long m = peers(digit, in);
     unsigned before = 0;
     if (in) before = hist[wave * BINS + digit];
     const unsigned lower = __popcll(m & ((1ull << lane) - 1));
@@ -103,7 +104,7 @@ __global__ __launch_bounds__(1024) void k_sort_small(LookupGrad a, int passes, i
             const bool in = i < n;
             k[q] = in ? lk[i] : 0;
             p[q] = in ? lp[i] : 0;
-            r[q] = rank_in_wave<16>((k[q] >> shift) & mask, bits, in, hist, wave, lane);
+            r[q] = rank_in_wave<16>((k[q] >> shift) & mask, in, hist, wave, lane);
         }
         __syncthreads();
         // the waves' counts of a digit become exclusive sums; base = the digit's total
@@ -195,17 +196,18 @@ __global__ __launch_bounds__(256) void k_sort_scatter(LookupGrad a, const unsign
 #pragma unroll
         for (int q = 0; q < BINS / 64; ++q) { base[t * (BINS / 64) + q] = x; x += v[q]; }
     }
+    constexpr int Q = TILE / 256;
     const long i0 = (long)blockIdx.x * TILE + (long)wave * (TILE / 4);
-    unsigned k[16], p[16], r[16];
+    unsigned k[Q], p[Q], r[Q];
 #pragma unroll
-    for (int q = 0; q < 16; ++q) {
+    for (int q = 0; q < Q; ++q) {
         const long i = i0 + 64 * q + lane;
         const bool in = i < a.n;
         k[q] = in ? (keys ? keys[i] : key_at(a, i)) : 0;
         p[q] = in ? (pos ? pos[i] : (unsigned)i) : 0;
     }
 #pragma unroll
-    for (int q = 0; q < 16; ++q) r[q] = rank_in_wave<4>((k[q] >> shift) & (bins - 1), bits, i0 + 64 * q + lane < a.n, hist, wave, lane);
+    for (int q = 0; q < Q; ++q) r[q] = rank_in_wave<4>((k[q] >> shift) & (bins - 1), i0 + 64 * q + lane < a.n, hist, wave, lane);
     __syncthreads();
     for (int i = t; i < bins; i += 256) {
         unsigned s = base[i] + counts[(size_t)i * gridDim.x + blockIdx.x];
@@ -214,7 +216,7 @@ __global__ __launch_bounds__(256) void k_sort_scatter(LookupGrad a, const unsign
     }
     __syncthreads();
 #pragma unroll
-    for (int q = 0; q < 16; ++q)
+    for (int q = 0; q < Q; ++q)
         if (i0 + 64 * q + lane < a.n) {
             const unsigned at = hist[wave * BINS + ((k[q] >> shift) & (bins - 1))] + r[q];
             keys_out[at] = k[q];
@@ -282,42 +284,103 @@ template <int T> __global__ __launch_bounds__(256) void k_lookup_sum(LookupGrad 
     else put_sum<T>(a, cur, c, s);
 }
 
-// One workgroup a piece: if a run begins in it and goes on, the run's partial sums — its own and those of the pieces it comes into — are added up: each thread a column and
-// every G-th piece, then the G sums in order.
+// Runs that begin in a piece and go on: the run's partial sums — its own and those of the pieces it comes into — are added up.  A wave looks at one piece; a short run (the usual
+// case: it ends in the next piece) is its own work, lane by column; a long one is done by the workgroup: each thread a column and every G-th piece, then the G sums in order.
+template <int T> __device__ __forceinline__ void put_one(const LookupGrad& a, unsigned token, int c, float s) {
+    const size_t at = (size_t)token * a.d + c;
+    s *= a.scale;
+    if constexpr (T == LT_F32) static_cast<float*>(a.dtable)[at] = s;
+    else static_cast<unsigned short*>(a.dtable)[at] = (unsigned short)pack2<T>(s, 0.0f);
+}
 template <int T> __global__ __launch_bounds__(256) void k_lookup_join(LookupGrad a, const unsigned* keys, long pieces, int len, const float* part) {
+    constexpr long SHORT = 16;
     __shared__ float sums[256];
-    const long piece = blockIdx.x, rows = a.n * a.per, i0 = piece * len, i1 = i0 + len;
-    if (i1 >= rows) return;
-    const unsigned tok = keys[(i1 - 1) / a.per];
-    if (tok == (unsigned)a.v || keys[i1 / a.per] != tok) return;
-    if (i0 > 0 && keys[(i0 - 1) / a.per] == tok) return;      // the run began in an earlier piece
-    long lo = i1 / a.per, hi = a.n;                           // first entry behind the run
-    while (lo < hi) {
-        const long m = (lo + hi) >> 1;
-        if (keys[m] <= tok) lo = m + 1; else hi = m;
-    }
-    const long more = (lo * a.per - 1) / len - piece;         // pieces that the run comes into
-    const int w = 8 * ((a.d + 7) >> 3);
-    const float* first = part + (size_t)piece * 2 * w;
-    for (int c0 = 0; c0 < a.d; c0 += 256) {
-        const int cols = a.d - c0 < 256 ? a.d - c0 : 256, g = 256 / cols;
-        const int c = threadIdx.x % cols, y = threadIdx.x / cols;
-        float s = 0.0f;
-        if (y < g) {
-            if (y == 0) s = first[w + c0 + c];
-            const float* p = first + 2 * w + c0 + c;
-#pragma unroll 4
-            for (long q = y; q < more; q += g) s += p[(size_t)q * 2 * w];
+    __shared__ unsigned token[4];
+    __shared__ int goes_on[4];      // pieces that the run comes into, where it is a long one
+    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), w = 8 * ((a.d + 7) >> 3);
+    const long rows = a.n * a.per, piece = (long)blockIdx.x * 4 + wave, i0 = piece * len, i1 = i0 + len;
+    long more = 0;
+    unsigned tok = 0;
+    if (i1 < rows) {
+        tok = keys[(i1 - 1) / a.per];
+        if (tok != (unsigned)a.v && keys[i1 / a.per] == tok && !(i0 > 0 && keys[(i0 - 1) / a.per] == tok)) {      // (else: no run goes on, or it began in an earlier piece)
+            more = 1;
+            if (i1 + len < rows && keys[(i1 + len) / a.per] == tok) {      // further than the next piece: where the run ends
+                long lo = (i1 + len) / a.per, hi = a.n;
+                while (lo < hi) {
+                    const long m = (lo + hi) >> 1;
+                    if (keys[m] <= tok) lo = m + 1; else hi = m;
+                }
+                more = (lo * a.per - 1) / len - piece;
+            }
         }
-        sums[threadIdx.x] = s;
+    }
+    const float* first = part + (size_t)piece * 2 * w;
+    if (more > 0 && more <= SHORT)
+        for (int c = lane; c < a.d; c += 64) {
+            float s = first[w + c];
+            for (long q = 0; q < more; ++q) s += first[(size_t)(q + 1) * 2 * w + c];
+            put_one<T>(a, tok, c, s);
+        }
+    if (lane == 0) { token[wave] = tok; goes_on[wave] = more > SHORT ? (int)more : 0; }
+    __syncthreads();
+    for (int y = 0; y < 4; ++y) {
+        const int n = goes_on[y];
+        if (n == 0) continue;
+        const float* from = part + (size_t)((long)blockIdx.x * 4 + y) * 2 * w;
+        for (int c0 = 0; c0 < a.d; c0 += 256) {
+            const int cols = a.d - c0 < 256 ? a.d - c0 : 256, g = 256 / cols, c = t % cols, z = t / cols;
+            float s = 0.0f;
+            if (z < g) {
+                if (z == 0) s = from[w + c0 + c];
+                const float* p = from + 2 * w + c0 + c;
+#pragma unroll 4
+                for (int q = z; q < n; q += g) s += p[(size_t)q * 2 * w];
+            }
+            sums[t] = s;
+            __syncthreads();
+            if (t < cols) {
+                float r = 0.0f;
+                for (int q = 0; q < g; ++q) r += sums[q * cols + t];
+                put_one<T>(a, token[y], c0 + t, r);
+            }
+            __syncthreads();
+        }
+    }
+}
+
+// Few positions (at most 4 096 sorted by one workgroup, at most 8 192 rows, a table of at most 4 096 tokens): one workgroup a token, which finds its rows by two 64-way searches of
+// the sorted keys and writes its gradient, zeros too — no pieces, no clearing, one launch behind the sort.
+__device__ __forceinline__ int below(const unsigned* keys, int n, unsigned token, int lane) {      // positions whose key is less than `token`
+    const int some = __popcll(__ballot(64 * lane < n && keys[min(64 * lane, n - 1)] < token));
+    if (some == 0) return 0;
+    const int i = 64 * (some - 1) + lane;
+    return 64 * (some - 1) + __popcll(__ballot(i < n && keys[min(i, n - 1)] < token));
+}
+template <int T> __global__ __launch_bounds__(256) void k_lookup_token(LookupGrad a, const unsigned* keys, const unsigned* pos) {
+    __shared__ float sums[256 * 8];
+    const int t = threadIdx.x, lane = t & 63, n = (int)a.n, per = (int)a.per, cpr = (a.d + 7) >> 3;
+    const unsigned token = blockIdx.x;
+    const int first = below(keys, n, token, lane) * per, last = below(keys, n, token + 1, lane) * per;
+    for (int c0 = 0; c0 < cpr; c0 += 256) {
+        const int chunks = cpr - c0 < 256 ? cpr - c0 : 256, g = 256 / chunks, y = t / chunks, c = 8 * (c0 + t % chunks);
+        float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        if (y < g)
+#pragma unroll 4
+            for (int i = first + y; i < last; i += g) {
+                const int e = i / per;
+                float f[8];
+                to_floats<T>(load8<T>(static_cast<const char*>(a.dout) + ((long)pos[e] * per + (i - e * per)) * a.ld_dout * Bytes<T>::v, c, a.d), f);
+#pragma unroll
+                for (int x = 0; x < 8; ++x) s[x] += f[x];
+            }
+#pragma unroll
+        for (int x = 0; x < 8; ++x) sums[8 * t + x] = s[x];
         __syncthreads();
-        if (threadIdx.x < cols) {
+        for (int z = t; z < 8 * chunks; z += 256) {
             float r = 0.0f;
-            for (int q = 0; q < g; ++q) r += sums[q * cols + threadIdx.x];
-            r *= a.scale;
-            const size_t at = (size_t)tok * a.d + c0 + threadIdx.x;
-            if constexpr (T == LT_F32) static_cast<float*>(a.dtable)[at] = r;
-            else static_cast<unsigned short*>(a.dtable)[at] = (unsigned short)pack2<T>(r, 0.0f);
+            for (int q = 0; q < g; ++q) r += sums[q * 8 * chunks + z];
+            if (8 * c0 + z < a.d) put_one<T>(a, token, 8 * c0 + z, r);
         }
         __syncthreads();
     }
@@ -363,6 +426,11 @@ template <int T> hipError_t lookup_backward(const LookupGrad& a, hipStream_t s) 
     char* ws = static_cast<char*>(a.ws);
     auto u = [&](size_t at) { return reinterpret_cast<unsigned*>(ws + at); };
     const size_t zero = (size_t)a.v * a.d * Bytes<T>::v;
+    if (a.n > 0 && p.tiles == 0 && p.rows <= 8192 && a.v <= 4096) {
+        hipLaunchKernelGGL(k_sort_small, dim3(1), dim3(1024), 0, s, a, p.passes, p.bits, u(p.keys), u(p.pos), (size_t)0);
+        hipLaunchKernelGGL((k_lookup_token<T>), dim3((unsigned)a.v), dim3(256), 0, s, a, u(p.keys), u(p.pos));
+        return hipGetLastError();
+    }
     if (a.n == 0 || p.tiles == 0) {
         // a table of up to 64 KB is cleared by the sorting workgroup, a larger one by a launch of its own
         const bool own = a.n > 0 && zero <= 65536;
@@ -384,7 +452,7 @@ template <int T> hipError_t lookup_backward(const LookupGrad& a, hipStream_t s) 
     const long threads = p.pieces * ((a.d + 7) / 8);
     float* part = reinterpret_cast<float*>(ws + p.part);
     hipLaunchKernelGGL((k_lookup_sum<T>), dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, s, a, u(p.keys), u(p.pos), p.pieces, p.len, part);
-    if (p.pieces > 1) hipLaunchKernelGGL((k_lookup_join<T>), dim3((unsigned)p.pieces), dim3(256), 0, s, a, u(p.keys), p.pieces, p.len, part);
+    if (p.pieces > 1) hipLaunchKernelGGL((k_lookup_join<T>), dim3((unsigned)((p.pieces + 3) / 4)), dim3(256), 0, s, a, u(p.keys), p.pieces, p.len, part);
     return hipGetLastError();
 }
 

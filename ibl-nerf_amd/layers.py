@@ -21,6 +21,9 @@ from . import binding as B
 
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 MAX_COLUMNS, MAX_STRIDE = 65536, 1 << 24
+# the current stream's handle without a Stream object around it (these calls cost microseconds, and so do a small layer's kernels)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda device: torch.cuda.current_stream(device).cuda_stream)
+_SAME_DEVICE = contextlib.nullcontext()
 
 
 def _type(t, what):
@@ -34,9 +37,8 @@ def _on(t):
     """(library, stream, guard): the tensor's device made current for the call where it is not."""
     if not t.is_cuda:
         raise B.IblNerfError("the layer operators have no CPU path: got a tensor on %s" % t.device)
-    lib, dev = B.load_library(), t.device.index
-    guard = contextlib.nullcontext() if dev == torch.cuda.current_device() else torch.cuda.device(dev)
-    return lib, torch.cuda.current_stream(dev).cuda_stream, guard
+    dev = t.get_device()
+    return B.load_library(), _raw_stream(dev), _SAME_DEVICE if dev == torch.cuda.current_device() else torch.cuda.device(dev)
 
 
 def _same(t, like, what, dtype=None):
@@ -47,11 +49,14 @@ def _same(t, like, what, dtype=None):
 
 
 def _rows(t, what):
-    """t [..., k] as [n, k] with unit stride along a row and its row stride in elements."""
-    if t.dim() < 1 or not 1 <= t.shape[-1] <= MAX_COLUMNS:
-        raise ValueError("%s must be [..., k] with 1 <= k <= %d, got %s" % (what, MAX_COLUMNS, tuple(t.shape)))
-    k = t.shape[-1]
-    if t.dim() != 2:
+    """t [..., k] as [n, k] with unit stride along a row, and its row stride in elements."""
+    shape = t.shape
+    if len(shape) == 2 and 1 <= shape[1] <= MAX_COLUMNS and t.is_contiguous():
+        return t, shape[1]
+    if len(shape) < 1 or not 1 <= shape[-1] <= MAX_COLUMNS:
+        raise ValueError("%s must be [..., k] with 1 <= k <= %d, got %s" % (what, MAX_COLUMNS, tuple(shape)))
+    k = shape[-1]
+    if len(shape) != 2:
         t = t.reshape(-1, k) if t.numel() else t.new_empty((0, k))
     if (k > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and not k <= t.stride(0) <= MAX_STRIDE):
         t = t.contiguous()
@@ -61,6 +66,10 @@ def _rows(t, what):
 def _workspace(size, device):
     """Scratch memory of one call from torch's allocator: reused in stream order, a captured graph's from the graph's own pool."""
     return (torch.empty((size,), dtype=torch.uint8, device=device), size) if size else (None, 0)
+
+
+def _address(t):
+    return None if t is None else t.data_ptr()
 
 
 class Checkpoint:
@@ -92,6 +101,13 @@ class Checkpoint:
         return out
 
 
+def _made(codes, scales, columns, signed):
+    """A Checkpoint of buffers that a kernel has just written."""
+    c = Checkpoint.__new__(Checkpoint)
+    c.codes, c.scales, c.columns, c.signed = codes, scales, columns, bool(signed)
+    return c
+
+
 def _codes_like(x, n, columns):
     blocks = (columns + 31) // 32
     return torch.empty((n, 32 * blocks), dtype=torch.uint8, device=x.device), torch.empty((n, blocks), dtype=torch.uint8, device=x.device)
@@ -101,19 +117,19 @@ def checkpoint(x, signed=True):
     """The 8-bit checkpoint of x [..., k] (rows flattened).  signed=False: negative entries become zero."""
     t = _type(x, "x")
     lib, stream, guard = _on(x)
-    x, ld = _rows(x.detach(), "x")
+    x, ld = _rows(x, "x")
     n, k = x.shape
     codes, scales = _codes_like(x, n, k)
     with guard:
         B.check_layers(lib.iblnerf_checkpoint(stream, t, x.data_ptr(), ld, n, k, int(bool(signed)), codes.data_ptr(), scales.data_ptr()))
-    return Checkpoint(codes, scales, k, signed)
+    return _made(codes, scales, k, signed)
 
 
 def _weight(weight, k, like, dtype):
     if weight.dim() != 2 or weight.shape[1] != k:
         raise ValueError("a layer of %d inputs takes a weight [o, %d], got %s" % (k, k, tuple(weight.shape)))
     _same(weight, like, "weight", dtype)
-    return _rows(weight.detach(), "weight")
+    return _rows(weight, "weight")
 
 
 def dense_forward(x, weight, bias=None, relu=False, keep=True):
@@ -122,7 +138,7 @@ def dense_forward(x, weight, bias=None, relu=False, keep=True):
     t = _type(x, "x")
     lib, stream, guard = _on(x)
     lead = x.shape[:-1]
-    x, ld = _rows(x.detach(), "x")
+    x, ld = _rows(x, "x")
     n, k = x.shape
     w, ldw = _weight(weight, k, x, x.dtype)
     o = w.shape[0]
@@ -132,14 +148,14 @@ def dense_forward(x, weight, bias=None, relu=False, keep=True):
         if tuple(bias.shape) != (o,):
             raise ValueError("the bias of a layer of %d outputs is [%d], got %s" % (o, o, tuple(bias.shape)))
         _same(bias, x, "bias", x.dtype)
-        bias = bias.detach().contiguous()
+        bias = bias.contiguous()
     y = torch.empty((n, o), dtype=x.dtype, device=x.device)
     codes, scales = _codes_like(x, n, o) if keep else (None, None)
     ws, ws_bytes = _workspace(lib.iblnerf_dense_forward_workspace(t, n, k, o), x.device)
     with guard:
-        B.check_layers(lib.iblnerf_dense_forward(stream, t, x.data_ptr(), ld, n, k, w.data_ptr(), ldw, o, None if bias is None else bias.data_ptr(), int(bool(relu)), y.data_ptr(), o,
-                                                 codes.data_ptr() if keep else None, scales.data_ptr() if keep else None, None if ws is None else ws.data_ptr(), ws_bytes))
-    return y.reshape(lead + (o,)), (Checkpoint(codes, scales, o, not relu) if keep else None)
+        B.check_layers(lib.iblnerf_dense_forward(stream, t, x.data_ptr(), ld, n, k, w.data_ptr(), ldw, o, _address(bias), int(bool(relu)), y.data_ptr(), o, _address(codes), _address(scales),
+                                                 _address(ws), ws_bytes))
+    return (y if len(lead) == 1 else y.reshape(lead + (o,))), (_made(codes, scales, o, not relu) if keep else None)
 
 
 def dense_backward(dy, x, weight, relu=None, need_dx=True, need_dw=True, need_db=True, grad_dtype=None):
@@ -148,7 +164,7 @@ def dense_backward(dy, x, weight, relu=None, need_dx=True, need_dw=True, need_db
     t = _type(dy, "dy")
     lib, stream, guard = _on(dy)
     lead = dy.shape[:-1]
-    dy, ld = _rows(dy.detach(), "dy")
+    dy, ld = _rows(dy, "dy")
     n, o = dy.shape
     if not isinstance(x, Checkpoint) or x.rows != n:
         raise ValueError("x must be the Checkpoint of the layer's %d input rows" % n)
@@ -170,10 +186,10 @@ def dense_backward(dy, x, weight, relu=None, need_dx=True, need_dw=True, need_db
     db = torch.empty((o,), dtype=grad_dtype, device=dev) if need_db else None
     ws, ws_bytes = _workspace(lib.iblnerf_dense_backward_workspace(t, n, k, o), dev)
     with guard:
-        B.check_layers(lib.iblnerf_dense_backward(stream, t, dy.data_ptr(), ld, n, k, o, x.codes.data_ptr(), x.scales.data_ptr(), int(x.signed), None if relu is None else relu.codes.data_ptr(),
-                                                  w.data_ptr(), ldw, None if dx is None else dx.data_ptr(), k, _TYPES[grad_dtype], None if dw is None else dw.data_ptr(),
-                                                  None if db is None else db.data_ptr(), None if ws is None else ws.data_ptr(), ws_bytes))
-    return (None if dx is None else dx.reshape(lead + (k,))), (dw if need_dw else None), db
+        B.check_layers(lib.iblnerf_dense_backward(stream, t, dy.data_ptr(), ld, n, k, o, x.codes.data_ptr(), x.scales.data_ptr(), int(x.signed),
+                                                  None if relu is None else relu.codes.data_ptr(), w.data_ptr(), ldw, _address(dx), k, _TYPES[grad_dtype], _address(dw), _address(db),
+                                                  _address(ws), ws_bytes))
+    return (dx if dx is None or len(lead) == 1 else dx.reshape(lead + (k,))), (dw if need_dw else None), db
 
 
 class _Dense(torch.autograd.Function):
@@ -222,7 +238,7 @@ def _lookup(table, index, scale, rows_per_index, out):
     lib, stream, guard = _on(table)
     if table.dim() != 2 or table.shape[0] < 1:
         raise ValueError("table must be [v, d] with at least one row, got %s" % (tuple(table.shape),))
-    tab, ld = _rows(table.detach(), "table")
+    tab, ld = _rows(table, "table")
     v, d = tab.shape
     idx, bits = _index(index, table)
     n, per = idx.numel(), int(rows_per_index)
@@ -246,7 +262,7 @@ def lookup_backward(dout, index, v, scale=1.0, rows_per_index=1):
     count nowhere.  The same inputs give the same bits."""
     t = _type(dout, "dout")
     lib, stream, guard = _on(dout)
-    dout, ld = _rows(dout.detach(), "dout")
+    dout, ld = _rows(dout, "dout")
     idx, bits = _index(index, dout)
     n, per, d = idx.numel(), int(rows_per_index), dout.shape[1]
     if per < 1 or int(v) < 1 or n * per != dout.shape[0]:
