@@ -143,6 +143,25 @@ def is_generic_arch(arch):
     return not is_member_of_built(arch) and 1 <= D <= 32 and D != 5 and 2 <= W <= 4096 and W % 2 == 0 and 0 <= L <= 24 and 0 <= Lv <= 24
 
 
+def bake_view_code(sd, code):
+    """The network of ONE view of a network trained with a code for each view (layers.network_query): `code` [c] as the network receives it (scaled) is a constant of every
+    sample, so its columns of views_linears.0 — the last c — go into that layer's bias, and what is left is an IBLNeRF that renders as any other.  numpy arrays or torch
+    tensors in, same kind out."""
+    w, b = sd["views_linears.0.weight"], sd["views_linears.0.bias"]
+    c = int(code.shape[0])
+    if code.ndim != 1 or not 0 < c < int(w.shape[1]):
+        raise ValueError("a view's code is [c] with fewer than views_linears.0's %d columns, got %s" % (int(w.shape[1]), tuple(code.shape)))
+    out = OrderedDict(sd)
+    if isinstance(w, np.ndarray):
+        out["views_linears.0.bias"] = (b.astype(np.float64) + w[:, -c:].astype(np.float64) @ np.asarray(code, np.float64)).astype(b.dtype)
+        out["views_linears.0.weight"] = np.ascontiguousarray(w[:, :-c])
+    else:
+        out["views_linears.0.bias"] = (b.detach().double() + w.detach()[:, -c:].double() @ code.detach().to(w.device).double()).to(b.dtype)
+        out["views_linears.0.weight"] = w.detach()[:, :-c].contiguous()
+    arch_of(out)                                  # (what is left has to be an IBLNeRF)
+    return out
+
+
 def weights_checksum(sd):
     """blob_checksum of a state dict of ANY architecture: of the built-shape blob it is uploaded as when it is a member of the built architecture (what the fixtures
     have always recorded), of its own flattening (arch_blob) otherwise."""

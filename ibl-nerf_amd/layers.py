@@ -2,7 +2,7 @@
 of each ray) with the table's gradient by sorted tokens.  include/iblnerf_layers.h is the C boundary; csrc/dense_kernel.hip and csrc/lookup_kernel.hip say what bounds
 them.
 
-They train what the fused backward (training.py) is not built for: networks outside the 8 x 256 shape, layer by layer (`network_forward` below,
+They train what the fused backward (training.py) is not built for: networks outside the 8 x 256 shape, layer by layer (`network_query` below,
 model.fused_network_query, training.render_rays_train).
 
     y, kept = dense(x, weight, bias, relu=True)        autograd; keeps 1.03 bytes an activation instead of x and y
@@ -192,6 +192,22 @@ def dense_backward(dy, x, weight, relu=None, need_dx=True, need_dw=True, need_db
     return (dx if dx is None or len(lead) == 1 else dx.reshape(lead + (k,))), (dw if need_dw else None), db
 
 
+def _leaves(*tensors, capturing=None):
+    """A leaf's gradient is accumulated on the stream of the first live graph that reads the leaf.  Under stream capture an EAGER graph that still lives would pull its stream into
+    the captured backward pass, where nothing can be reported and the process ends; so eager graphs sign the accumulation node (it lives as long as they do: called behind the
+    operator that holds it), and a capture that meets the sign is refused."""
+    for t in tensors:
+        if t is not None and t.requires_grad and t.is_leaf:
+            if capturing is None:
+                with _on(t)[2] if t.is_cuda else _SAME_DEVICE:
+                    capturing = t.is_cuda and torch.cuda.is_current_stream_capturing()
+            sign = t.view_as(t).grad_fn.next_functions[0][0].metadata
+            if not capturing:
+                sign["eager"] = True
+            elif "eager" in sign:
+                raise RuntimeError("a graph is being captured while an eager result of the same leaf (%s) is alive: delete that result (or its loss) first" % (tuple(t.shape),))
+
+
 class _Dense(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, relu, x_codes, x_scales, x_signed):
@@ -219,10 +235,13 @@ class _Dense(torch.autograd.Function):
 def dense(x, weight, bias=None, relu=False, kept=None):
     """dense_forward with autograd -> (y, Checkpoint of y).  kept: the Checkpoint of x that an earlier layer has written (None: one is made here, signed) — the backward pass
     reads the checkpoints of x and, under a ReLU, of y, so neither tensor is held for it.  Parameters may be float32 beside 16-bit activations: they are cast for the
-    products, and their gradients are float32 sums.  First derivatives only."""
+    products, and their gradients are float32 sums.  First derivatives only.
+    A backward pass may be captured into a graph while no eager result of the same leaves is alive (RuntimeError otherwise)."""
     if kept is not None and (kept.columns != x.shape[-1] or kept.rows * kept.columns != x.numel()):
         raise ValueError("kept is a checkpoint of [%d, %d], x is %s" % (kept.rows, kept.columns, tuple(x.shape)))
     y, codes, scales = _Dense.apply(x, weight, bias, bool(relu), *((None, None, True) if kept is None else (kept.codes, kept.scales, kept.signed)))
+    if y.requires_grad:
+        _leaves(x, weight, bias)
     return y, Checkpoint(codes, scales, weight.shape[0], not relu)
 
 
@@ -293,5 +312,109 @@ def lookup(table, index, scale=1.0, rows_per_index=1, out=None):
     index grows by that factor.  A negative index is a row without a code (zeros, no gradient); one beyond the table reads NaN.  Differentiable in the table; `out`
     ([n, d], rows may be strided: a slice of a wider input) is written instead of a new tensor, without autograd."""
     if out is None and torch.is_grad_enabled() and table.requires_grad:
-        return _Lookup.apply(table, index, float(scale), int(rows_per_index))
+        rows = _Lookup.apply(table, index, float(scale), int(rows_per_index))
+        _leaves(table)
+        return rows
     return _lookup(table, index, scale, rows_per_index, out)
+
+
+# ------------------------------------------------------------------------------------------------------------- a network layer by layer
+def encode(x, freqs):
+    """[x, sin(2^0 x), cos(2^0 x), ..., sin(2^(freqs-1) x), cos(2^(freqs-1) x)] of x [n, 3] (positional_embedder.py:21-34): the products with powers of two are exact, the angles of
+    the high frequencies large — sine and cosine in 64 bits, rounded once (as csrc/generic_mlp.hip)."""
+    if freqs == 0:
+        return x
+    a = (x[:, None, :] * torch.exp2(torch.arange(freqs, device=x.device, dtype=x.dtype))[None, :, None]).double()
+    e = torch.stack([torch.sin(a), torch.cos(a)], 2).to(x.dtype)              # [n, freqs, 2, 3]
+    return torch.cat([x, e.reshape(x.shape[0], 6 * freqs)], -1)
+
+
+def _linear(params, name):
+    return params[name + ".weight"], params[name + ".bias"]
+
+
+def network_query(inputs, viewdirs, network_fn, codes=None, views=None, code_scale=1.0, dtype=torch.float32):
+    """IBLNeRF.forward (ibl_nerf.py:154-208) of a network of ANY depth and width, with autograd, on `dense`: inputs [..., 3] points, viewdirs [n, 3] one direction for each row
+    of points (or None: the density alone, :175-176), `network_fn` a torch module with the reference's parameter names -> raw [..., 18] float32 (or [..., 1]).  What is held for
+    the backward pass is one 8-bit checkpoint of each activation.
+    codes [v, c] and views [n] (int): a code for each training view (photographs differ in exposure and white balance), code_scale * codes[view], beside the direction's
+    encoding of every sample of the ray: views_linears.0 then takes c more columns (checkpoint.bake_view_code makes the network of one view for rendering); the codes
+    receive their gradient by sorted views.  (Such a network queried without its codes is refused by its width, unless c is a multiple of 6: then its shapes are those of a
+    network with more frequencies.)
+    dtype: the type of the layers between the encodings and the heads (float32, bfloat16, float16); parameters stay what they are, heads are float32."""
+    params = dict(network_fn.named_parameters())
+    if getattr(network_fn, "is_color_independent_to_direction", False):
+        raise NotImplementedError("colour-independent networks run on the fused kernels only")
+    if (codes is None) != (views is None):
+        raise ValueError("codes and views come together")
+    lead, flat = inputs.shape[:-1], inputs.reshape(-1, 3)
+    W, ch = params["positions_linears.0.weight"].shape
+    depth = 1 + max(int(k.split(".")[1]) for k in params if k.startswith("positions_linears."))
+    e = encode(flat, (ch - 3) // 6).to(dtype)
+    h, kept = dense(e, *_linear(params, "positions_linears.0"), relu=True)
+    for i in range(1, depth):
+        if i == 5:                                                              # cat([x, h]) behind layer 4 (:168)
+            h, kept = torch.cat([e, h], -1), None
+        h, kept = dense(h, *_linear(params, "positions_linears.%d" % i), relu=True, kept=kept)
+
+    def head(x, names, kept_x):                                                 # the narrow outputs of one activation, float32
+        w = [params[n + ".weight"] for n in names]
+        b = [params[n + ".bias"] for n in names]
+        y = dense(x.float(), w[0] if len(w) == 1 else torch.cat(w), b[0] if len(b) == 1 else torch.cat(b), kept=kept_x)[0]
+        if len(names) > 1 and y.requires_grad:
+            _leaves(*w, *b)
+        return y
+
+    if viewdirs is None:
+        return head(h, ("sigma_linear",), kept).reshape(lead + (1,))
+    sigma_rough = head(h, ("sigma_linear", "roughness_linear"), kept)
+
+    def branch(x, kept_x, feature, out):
+        f, k = dense(x, *_linear(params, feature), relu=True, kept=kept_x)
+        return head(f, (out,), k)
+
+    albedo = branch(h, kept, "albedo_feature_linear", "albedo_linear")
+    irradiance = branch(h, kept, "irradiance_feature_linear", "irradiance_linear")
+    feature, _ = dense(h, *_linear(params, "feature_linear"), kept=kept)
+    rays, samples = viewdirs.shape[0], flat.shape[0] // max(viewdirs.shape[0], 1)
+    if rays * samples != flat.shape[0]:
+        raise ValueError("%d points do not divide among %d directions" % (flat.shape[0], rays))
+    n_code = 0 if codes is None else codes.shape[1]
+    chv = params["views_linears.0.weight"].shape[1] - W - n_code
+    if chv < 3 or (chv - 3) % 6:
+        raise ValueError("views_linears.0 takes %d columns: %d features, %d code columns and no positional encoding's width beside them" % (params["views_linears.0.weight"].shape[1], W, n_code))
+    ev = encode(viewdirs.reshape(-1, 3).to(flat.dtype), (chv - 3) // 6).to(dtype)
+    parts = [feature, ev[:, None].expand(rays, samples, chv).reshape(-1, chv)]
+    if codes is not None:
+        if views.numel() != rays:
+            raise ValueError("views has %d entries for %d rays" % (views.numel(), rays))
+        parts.append(lookup(codes, views.reshape(-1), code_scale, rows_per_index=samples).to(dtype) if samples else codes.new_zeros((0, n_code), dtype=dtype))
+    h2, kept2 = dense(torch.cat(parts, -1), *_linear(params, "views_linears.0"), relu=True)
+    out = [sigma_rough[:, :1], albedo, sigma_rough[:, 1:], irradiance, head(h2, ("radiance_linear",), kept2)]
+    out += [branch(h2, kept2, "additional_radiance_feature_linear.%d" % k, "additional_radiance_linear.%d" % k) for k in range(3)]
+    return torch.cat(out, -1).reshape(lead + (18,))
+
+
+def network_gradients(inputs, viewdirs, draw, network_fn, dtype=torch.float32, points=1 << 20):
+    """{parameter name: dL/d parameter} of network_query from dL/d raw (draw [n, S, 18]), `points` samples at a time (14 checkpoints of a 512-wide network: 7 KB a sample)."""
+    named = dict(network_fn.named_parameters())
+    names, params = list(named), list(named.values())
+    total = None
+    step = max(1, points // max(1, inputs.shape[1]))
+    for i in range(0, inputs.shape[0], step):
+        with torch.enable_grad():
+            held = [p.detach().requires_grad_(True) for p in params]
+            raw = network_query(inputs[i:i + step], viewdirs[i:i + step], _Named(dict(zip(names, held))), dtype=dtype)
+        grads = torch.autograd.grad(raw, held, draw[i:i + step].contiguous())
+        total = list(grads) if total is None else [a.add_(b) for a, b in zip(total, grads)]
+    return dict(zip(names, total if total is not None else [torch.zeros_like(p) for p in params]))
+
+
+class _Named:
+    """Parameters by name, as network_query asks a module for them."""
+
+    def __init__(self, params):
+        self._params = params
+
+    def named_parameters(self):
+        return self._params.items()

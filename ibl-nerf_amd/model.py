@@ -24,7 +24,7 @@ class IBLNeRF:
         # The kernels are built for D=8, W=256, multires 10 / 4; a SMALLER network is evaluated as the member of that architecture computing the same function
         # (checkpoint.embed_architecture, applied at upload): D <= 8 (not 5: the reference's own forward fails there), W <= 256, multires <= 10, multires_views <= 4.
         # Round 6: anything LARGER (D <= 32, even W <= 4096, multires / multires_views <= 24) runs on csrc/generic_mlp.hip — layer by layer in exact fp32 on the matrix
-        # cores, every sample of every query, no backward: correct and slow (checkpoint.is_generic_arch; iblnerf_upload_weights_arch).
+        # cores, every sample of every query: correct and slow (checkpoint.is_generic_arch; iblnerf_upload_weights_arch); its gradients come layer by layer too (layers.py).
         shape_ok = (input_ch - 3) % 6 == 0 and (input_ch_views - 3) % 6 == 0 and input_ch >= 3 and input_ch_views >= 3
         arch = (int(D), int(W), (int(input_ch) - 3) // 6, (int(input_ch_views) - 3) // 6) if shape_ok else None
         ok = tuple(skips) == (4,) and coarse_radiance_number == 3 and shape_ok and (ck.is_member_of_built(arch) or (ck.is_generic_arch(arch) and not is_color_independent_to_direction))
@@ -169,12 +169,27 @@ def network_query_fn(inputs, viewdirs, network_fn, renderer=None, which=0):
 TRUNK_PARAMS = tuple("positions_linears.%d.%s" % (i, k) for i in range(8) for k in ("weight", "bias")) + ("sigma_linear.weight", "sigma_linear.bias")
 
 
+def layered(network_fn):
+    """Does a gradient-carrying query of this network run layer by layer (layers.network_query)?  True for one that the fused kernels cannot hold."""
+    try:
+        trunk = network_fn.positions_linears
+        W, ch = trunk[0].weight.shape
+        chv = network_fn.views_linears[0].weight.shape[1] - W
+    except (AttributeError, IndexError, TypeError):
+        return False
+    return (ch - 3) % 6 == 0 and (chv - 3) % 6 == 0 and not ck.is_member_of_built((len(trunk), W, (ch - 3) // 6, (chv - 3) // 6)) and not _ci(network_fn)
+
+
 def fused_trunk_query(inputs, network_fn):
     """`network_query_fn(inputs, None, network_fn)` (the trunk-only query, ibl_nerf.py:175-176) WITH autograd, both directions on the
     fused kernels: forward = the trunk query, backward = iblnerf_trunk_backward (the forward is recomputed there with the pass bits
     kept, as under activation checkpointing), which hands dL/dinputs and the gradients of positions_linears.0-7 / sigma_linear back
-    to torch.  `network_fn` is the torch module whose parameters carry those names (the reference's IBLNeRF).  First derivatives only."""
+    to torch.  `network_fn` is the torch module whose parameters carry those names (the reference's IBLNeRF).  First derivatives only.
+    A network outside the built shape runs layer by layer (layers.network_query)."""
     import torch
+    if layered(network_fn):
+        from . import layers
+        return layers.network_query(inputs, None, network_fn)
     named = dict(network_fn.named_parameters())
     params = [named[k] for k in TRUNK_PARAMS]
 
@@ -248,10 +263,15 @@ def fused_trunk_features2(inputs, viewdirs, network_fn):
 ALL_PARAMS = tuple(n + s for n, _, _ in ck.SCHEMA for s in (".weight", ".bias"))
 
 
-def fused_network_query(inputs, viewdirs, network_fn):
+def fused_network_query(inputs, viewdirs, network_fn, codes=None, views=None, code_scale=1.0, layer_dtype=None):
     """`network_query_fn(inputs, viewdirs, network_fn)` WITH autograd, the whole network on the fused kernels in both directions: forward =
-    the precise network query, backward = iblnerf_network_backward (dL/d raw rows in; dL/dinputs and all 46 parameter gradients out)."""
+    the precise network query, backward = iblnerf_network_backward (dL/d raw rows in; dL/dinputs and all 46 parameter gradients out).
+    A network outside the built shape, and any network with a code for each view (codes, views, code_scale: layers.network_query), runs layer by layer from 8-bit
+    checkpoints, its layers in layer_dtype (float32 by default)."""
     import torch
+    if codes is not None or layer_dtype is not None or layered(network_fn):
+        from . import layers
+        return layers.network_query(inputs, viewdirs, network_fn, codes=codes, views=views, code_scale=code_scale, dtype=layer_dtype or torch.float32)
     named = dict(network_fn.named_parameters())
     params = [named[k] for k in ALL_PARAMS]
 
@@ -278,6 +298,8 @@ def fused_query(inputs, viewdirs, network_fn):
     import torch
     import torch.nn.functional as F
     n = network_fn
+    if layered(n):
+        return fused_trunk_query(inputs, n) if viewdirs is None else fused_network_query(inputs, viewdirs, n)
     if viewdirs is not None and not _ci(n) and len(n.views_linears) == 1 and inputs.dim() == 3 and set(ALL_PARAMS) == set(dict(n.named_parameters())):
         return fused_network_query(inputs, viewdirs, n)                                # every layer, both directions
     if viewdirs is not None and not _ci(n) and len(n.views_linears) == 1 and inputs.dim() == 3:

@@ -44,28 +44,29 @@ COMPACT_MIN_POINTS = 131072
 LIVE_REL = 1e-7
 
 
-def network_backward_live(r, pts, rays_d, draw, which):
+def network_backward_live(r, pts, rays_d, draw, which, backward=None):
     """Renderer.network_backward on the samples that carry a gradient only.  A sample whose density is not positive has alpha = 0: its weight is exactly zero and the ReLU in
     front of the density is dead, so its whole row of dL/d raw is EXACTLY zero (iblnerf_composite_direct_backward) — nine in ten samples on a scene with surfaces — and a
     zero row adds exactly nothing to any parameter gradient.  Those rows — and the rows below LIVE_REL of the pass's largest — are dropped (one mask, one nonzero — the
     step's only host synchronisation — three gathers) and the
     fused backward runs on the rest as a batch of one-sample "rays": the same kernels, a third of the points (round 6: "training evaluates every
     sample").  Parameter gradients agree with the whole batch's to fp32 round-off of the weight-gradient sums (another grouping of the same terms); dL/d pts is not returned
-    (a training step's rays are constants)."""
+    (a training step's rays are constants).  backward: another (pts, rays_d, draw) -> (dL/d pts or None, gradients) than the fused one (a network that runs layer by layer)."""
     torch = __import__("torch")
+    backward = backward or (lambda p, d, u: r.network_backward(p, d, u, which))
     n, S = int(pts.shape[0]), int(pts.shape[1])
     if n * S < COMPACT_MIN_POINTS:
-        return r.network_backward(pts, rays_d, draw, which)
+        return backward(pts, rays_d, draw)
     rows = draw.reshape(n * S, -1)
     mag = rows.abs().amax(-1)
     idx = (~(mag <= LIVE_REL * mag.max())).nonzero().reshape(-1)      # (an all-zero upstream gradient: every row is dropped; a NaN row is kept, so that it shows)
     if idx.numel() > 0.7 * n * S:                      # fog: (almost) everything is live
-        return r.network_backward(pts, rays_d, draw, which)
+        return backward(pts, rays_d, draw)
     if idx.numel() == 0:
         idx = torch.zeros((1,), dtype=torch.long, device=rows.device)      # (an all-zero upstream gradient: one dead sample keeps the call's shape; its gradients are zeros)
     pts_c = pts.reshape(n * S, 3)[idx].reshape(-1, 1, 3).contiguous()
     rd_c = rays_d.reshape(n, 3)[idx // S].contiguous()
-    return r.network_backward(pts_c, rd_c, rows[idx].reshape(-1, 1, rows.shape[-1]).contiguous(), which)
+    return backward(pts_c, rd_c, rows[idx].reshape(-1, 1, rows.shape[-1]).contiguous())
 
 # parameters that still receive gradients under forward_freezed (ibl_nerf.py:113-131)
 UNFROZEN = ("albedo_feature_linear.", "albedo_linear.", "irradiance_feature_linear.", "irradiance_linear.", "roughness_linear.")
@@ -472,10 +473,11 @@ def render_rays_train(r, rays_o, rays_d, near, far, net_c, net_f, lut, *, approx
     pnames = []
     for nm, arch in zip(named, archs):
         want = None if arch is None else [n + t for n, _, _ in ck.arch_schema(*arch) for t in (".weight", ".bias")]
-        if want is None or set(nm) != set(want) or arch[0] > 8 or arch[0] == 5 or arch[1] > 256 or arch[2] > 10 or arch[3] > 4:
-            raise NotImplementedError("the fused backward is built for the IBLNeRF architecture (46 parameters per network at netdepth 8; netdepth <= 8 and != 5, "
-                                      "netwidth <= 256, multires <= 10, multires_views <= 4)")
-        pnames.append([k for k in ALL_PARAMS if k in nm])
+        if want is None or set(nm) != set(want) or not (ck.is_member_of_built(arch) or ck.is_generic_arch(arch)):
+            raise NotImplementedError("the backward is built for the IBLNeRF architecture (46 parameters per network at netdepth 8): fused for netdepth <= 8 and != 5, netwidth <= 256, "
+                                      "multires <= 10, multires_views <= 4, layer by layer for larger networks (netdepth <= 32, even netwidth <= 4096, multires, multires_views <= 24)")
+        # (a network outside the built shape: its forward on the layer-by-layer render path, its gradients from 8-bit checkpoints of a second forward, layers.network_gradients)
+        pnames.append([k for k in ALL_PARAMS if k in nm] if ck.is_member_of_built(arch) else want)
     params = [nm[k] for nm, ks in zip(named, pnames) for k in ks]
     ci = bool(r.opt.color_independent_to_direction)      # (the context's streams carry the identity in place of the unused layers: iblnerf_network_backward)
     frozen = [bool(getattr(net, "freeze_radiance", False)) for net in (net_c, net_f)]
@@ -624,7 +626,11 @@ def render_rays_train(r, rays_o, rays_d, near, far, net_c, net_f, lut, *, approx
                     gn = gn.reshape(n, 3)
                     aux_add("normal_mlp", r.aux_backward("normal_mlp", qpts, (gn * fac) if fac.dim() == 2 else (gn[:, None, :] * fac)))
                 r.last_backward_ok = None
-                _, grads = network_backward_live(r, pts, sv["rd"], draw, which)
+                layered = None
+                if not ck.is_member_of_built(archs[which]):
+                    from . import layers
+                    layered = lambda p, d, u, net=(net_c, net_f)[which]: (None, layers.network_gradients(p, d, u, net))      # noqa: E731
+                _, grads = network_backward_live(r, pts, sv["rd"], draw, which, layered)
                 if incident_gradient and consts is not None and not frozen[which]:      # (forward_freezed computes sigma and every radiance under no_grad: nothing to carry)
                     # the reflected ray of this pass (:438-440): x_surface + reflected_dir * z_vals_constant (the coarse grid, jitter included, :694), queried on the
                     # pass's own network (:451); raw2outputs_simple composites radiance and the three coarse radiances on the live weights
@@ -640,11 +646,11 @@ def render_rays_train(r, rays_o, rays_d, near, far, net_c, net_f, lut, *, approx
                     dm[:, 7:19] = denv.reshape(n, 12)
                     rdraw = r.composite_direct_backward(rraw, sv["zc"], rdir, dm, None, full=True)
                     r.last_backward_ok = None
-                    _, g2 = r.network_backward(rpts, rdir, rdraw, which)
+                    _, g2 = (layered or (lambda p, d, u: r.network_backward(p, d, u, which)))(rpts, rdir, rdraw)
                     grads = {k: grads[k] + g2[k] for k in grads}
                 if getattr(r, "last_backward_ok", None) is not None:
                     oks.append(r.last_backward_ok)
-                if archs[which] != ck.SHIPPED_ARCH:
+                if archs[which] != ck.SHIPPED_ARCH and layered is None:
                     grads = ck.unembed_gradients(grads, archs[which])
                 for k in pnames[which]:
                     gk = grads[k]

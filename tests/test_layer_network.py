@@ -1,0 +1,127 @@
+"""A network layer by layer (layers.network_query) on the CPU: its wiring against the plain module, with plain products in the places of the kernels; the codes of the views; what it
+refuses; the sign that an eager graph leaves on its leaves."""
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from ibl_nerf_amd import checkpoint as ck, layers  # noqa: E402
+from torch_ref import RefShaped, embed  # noqa: E402
+
+
+def plain_dense(x, weight, bias=None, relu=False, kept=None):
+    y = x @ weight.to(x.dtype).T + bias.to(x.dtype)
+    y = torch.relu(y) if relu else y
+    assert kept is None or torch.equal(kept.to(x.dtype), x)          # (the checkpoint that is handed on is the one of this very input)
+    return y, y.detach()
+
+
+def plain_lookup(table, index, scale=1.0, rows_per_index=1):
+    return (scale * table[index.long()]).repeat_interleave(rows_per_index, 0)
+
+
+@pytest.fixture()
+def plain(monkeypatch):
+    monkeypatch.setattr(layers, "dense", plain_dense)
+    monkeypatch.setattr(layers, "lookup", plain_lookup)
+
+
+def with_codes(net, c, seed):
+    """The module with c more columns in views_linears.0 and a table of 5 codes."""
+    g = torch.Generator().manual_seed(seed)
+    old = net.views_linears[0]
+    new = torch.nn.Linear(old.in_features + c, old.out_features).to(old.weight.dtype)
+    with torch.no_grad():
+        new.weight.copy_(torch.cat([old.weight, 0.3 * torch.randn(old.out_features, c, generator=g, dtype=old.weight.dtype)], 1))
+        new.bias.copy_(old.bias)
+    net.views_linears[0] = new
+    return torch.randn(5, c, generator=g, dtype=old.weight.dtype)
+
+
+ARCHS = [(8, 256, 10, 4), (2, 6, 3, 0), (6, 32, 0, 2), (10, 48, 12, 5)]
+
+
+@pytest.mark.parametrize("arch", ARCHS)
+@pytest.mark.parametrize("coded", [False, True])
+def test_wiring(plain, arch, coded):
+    net = RefShaped(ck.synthetic_arch_state_dict(3, arch), arch).double()
+    codes = with_codes(net, 7, 11) if coded else None
+    g = torch.Generator().manual_seed(5)
+    pts, dirs = torch.rand(4, 3, 3, generator=g, dtype=torch.float64) * 2 - 1, torch.randn(4, 3, generator=g, dtype=torch.float64)
+    views = torch.tensor([2, 0, 4, 2])
+    e, d = embed(pts.reshape(-1, 3), arch[2]), embed(dirs.repeat_interleave(3, 0), arch[3])
+    if coded:
+        d = torch.cat([d, 0.5 * codes[views].repeat_interleave(3, 0)], -1)
+        got = layers.network_query(pts, dirs, net, codes=codes, views=views, code_scale=0.5, dtype=torch.float64)
+    else:
+        got = layers.network_query(pts, dirs, net, dtype=torch.float64)
+    want = net(e, d).reshape(4, 3, 18).detach()
+    # the heads run in float32: the feature layers' outputs rounded once (2^-24), products of up to 256 terms summed in float32
+    assert (got - want).abs().max() <= 300 * 2.0 ** -23 * max(1.0, float(want.abs().max())) and got.dtype == torch.float32
+    sigma = layers.network_query(pts, None, net, dtype=torch.float64)
+    assert sigma.shape == (4, 3, 1) and (sigma[..., 0] - got[..., 0]).abs().max() <= 300 * 2.0 ** -23 * max(1.0, float(want.abs().max()))      # (another order of the same sum)
+
+
+def test_encode():
+    x = torch.rand(50, 3, dtype=torch.float64) * 4 - 2
+    for k in (0, 1, 4, 24):
+        assert layers.encode(x, k).shape == (50, 3 + 6 * k) and (layers.encode(x, k) - embed(x, k)).abs().max() <= 1e-15 * 2.0 ** k
+    x32 = x.float()                # float32 points: one rounding of the true sine
+    e = layers.encode(x32, 12)
+    assert e.dtype == torch.float32 and (e.double() - embed(x32.double(), 12)).abs().max() <= 2.0 ** -24 + 1e-11
+
+
+def test_bake_view_code():
+    arch = (6, 32, 4, 2)
+    net = RefShaped(ck.synthetic_arch_state_dict(3, arch), arch).double()
+    codes = with_codes(net, 7, 2)
+    e, d = torch.randn(9, 27, dtype=torch.float64), torch.randn(9, 15, dtype=torch.float64)
+    want = net(e, torch.cat([d, 0.25 * codes[3].expand(9, 7)], -1))
+    sd = ck.bake_view_code(net.state_dict(), 0.25 * codes[3])
+    one = RefShaped(arch=arch).double()
+    one.load_state_dict(sd)
+    assert ck.arch_of(sd) == arch and (one(e, d) - want).abs().max() <= 1e-13
+    sn = ck.bake_view_code({k: v.numpy() for k, v in net.state_dict().items()}, (0.25 * codes[3]).numpy())
+    assert all(isinstance(v, np.ndarray) and np.allclose(v, sd[k].numpy(), rtol=0, atol=1e-14) for k, v in sn.items())
+    for bad in (codes, torch.zeros(0), torch.zeros(54), codes[0, :5]):
+        with pytest.raises(ValueError):
+            ck.bake_view_code(net.state_dict(), bad)
+
+
+def test_refuses(plain):
+    arch = (2, 16, 2, 1)
+    net = RefShaped(ck.synthetic_arch_state_dict(3, arch), arch)
+    p, d, codes = torch.zeros(4, 3, 3), torch.zeros(4, 3), torch.zeros(5, 7)
+    with pytest.raises(ValueError, match="together"):
+        layers.network_query(p, d, net, codes=codes)
+    with pytest.raises(ValueError, match="together"):
+        layers.network_query(p, d, net, views=torch.zeros(4, dtype=torch.int32))
+    with pytest.raises(ValueError, match="columns"):
+        layers.network_query(p, d, net, codes=codes, views=torch.zeros(4, dtype=torch.int32))          # (the network has no columns for a code)
+    with_codes(net, 7, 1)
+    with pytest.raises(ValueError, match="columns"):
+        layers.network_query(p, d, net)
+    with pytest.raises(ValueError, match="entries"):
+        layers.network_query(p, d, net, codes=codes, views=torch.zeros(5, dtype=torch.int32))
+    with pytest.raises(ValueError, match="divide"):
+        layers.network_query(p, torch.zeros(5, 3), net, codes=codes, views=torch.zeros(5, dtype=torch.int32))
+    net.is_color_independent_to_direction = True
+    with pytest.raises(NotImplementedError):
+        layers.network_query(p, d, net)
+
+
+def test_an_eager_graph_signs_its_leaves():
+    w, b = torch.nn.Parameter(torch.zeros(3)), torch.zeros(3)
+    layers._leaves(w, b, None, capturing=True)                  # nothing alive
+    layers._leaves(w, b, None, capturing=False)
+    layers._leaves(w, capturing=True)                           # (the sign went with the node: no graph holds it)
+    y = (w * 2).sum()
+    layers._leaves(w, capturing=False)
+    with pytest.raises(RuntimeError, match="alive"):
+        layers._leaves(w, capturing=True)
+    layers._leaves(b, capturing=True)
+    del y
+    layers._leaves(w, capturing=True)
+    z = w * 2
+    layers._leaves(w, capturing=True)                           # a graph made within the capture is no eager one
+    del z
