@@ -350,13 +350,12 @@ __global__ __launch_bounds__(256, 2) void k_dense_rows(DenseRows a) {
 
 // The form for few rows, where one latency after the other is what a call costs: a workgroup makes 32 rows x 32 outputs, each of its 4 waves over a quarter of the reduction, straight
 // from global memory (operands in the order they lie there, 4 steps asked for at once), and the quarters meet in LDS once.
-template <int T, bool DX>
-__global__ __launch_bounds__(256) void k_dense_few(DenseRows a) {
-    constexpr int U = 4, RS = 36;
-    __shared__ __attribute__((aligned(16))) float sums[4 * 32 * RS];
+constexpr int FEW_ROW = 36, FEW_LDS = 4 * 32 * FEW_ROW;      // floats
+template <int T, bool DX> __device__ __forceinline__ void dense_few(const DenseRows& a, unsigned block, float* sums) {
+    constexpr int U = 4, RS = FEW_ROW;
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), i = lane & 31, h = lane >> 5;
-    const int ot = (a.o + 31) >> 5, o0 = (int)(blockIdx.x % ot) * 32;
-    const long p0 = (long)(blockIdx.x / ot) * 32;
+    const int ot = (a.o + 31) >> 5, o0 = (int)(block % ot) * 32;
+    const long p0 = (long)(block / ot) * 32;
     const int steps = (a.r + 15) >> 4, quarter = (steps + 3) >> 2, s1 = min(steps, (wave + 1) * quarter), r32 = (a.r + 31) & ~31;
     const long p = min(p0 + i, a.n - 1);                 // (rows and outputs beyond the last: the last again, not written)
     const int o = min(o0 + i, a.o - 1);
@@ -445,6 +444,11 @@ __global__ __launch_bounds__(256) void k_dense_few(DenseRows a) {
             if (c == 0) a.scales[(p0 + row) * (o32 >> 5) + (o0 >> 5)] = (uint8_t)scale;
         }
     }
+}
+
+template <int T, bool DX> __global__ __launch_bounds__(256) void k_dense_few(DenseRows a) {
+    __shared__ __attribute__((aligned(16))) float sums[FEW_LDS];
+    dense_few<T, DX>(a, blockIdx.x, sums);
 }
 
 // The weights as matrix operands for k_dense_tall: [32-wide tile][16 reduction elements][lane][8], zeros beyond the layer
@@ -721,17 +725,18 @@ __global__ __launch_bounds__(256, 2) void k_dense_tall(DenseRows a, const u32x4*
 // bits every time.
 //
 // W = 128: 4 waves, two workgroups on a compute unit; W = 256: 16 waves, half as many reads of either operand.  A wave takes 64 x 64.
-template <int T, int W>
-__global__ __launch_bounds__(W * W / 64, W == 256 ? 4 : 2) void k_dense_weights(DenseWeights a) {
-    constexpr int PARTS = T == LT_F32 ? 3 : 1, BR = T == LT_F32 ? 32 : 64, NT = W * W / 64, TO = 2, TK = 2;
+template <int T, int W> struct WeightsTile {
+    static constexpr int PARTS = T == LT_F32 ? 3 : 1, BR = T == LT_F32 ? 32 : 64, PLANE = BR * W, BUFFER = (PARTS + 1) * PLANE;
+};
+template <int T, int W> __device__ __forceinline__ void dense_weights_tile(const DenseWeights& a, unsigned block, unsigned short* lds) {
+    constexpr int PARTS = WeightsTile<T, W>::PARTS, BR = WeightsTile<T, W>::BR, NT = W * W / 64, TO = 2, TK = 2;
     constexpr int RT = W / 8, RP = NT / RT, NC = BR / RP;      // threads a row of a tile, rows at a time, 8-column chunks a thread stages
-    constexpr int PLANE = BR * W, BUFFER = (PARTS + 1) * PLANE;
-    __shared__ __attribute__((aligned(16))) unsigned short lds[2 * BUFFER];
+    constexpr int PLANE = WeightsTile<T, W>::PLANE, BUFFER = WeightsTile<T, W>::BUFFER;
     static_assert(NC >= 1 && NC <= BR / 16, "a chunk for each step of 16 rows at most");
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const int kt = (a.k + W - 1) / W, ot = (a.o + W - 1) / W, tiles = kt * ot;
-    const long j = blockIdx.x >> 3;
-    const int split = (int)(j / tiles) * 8 + (blockIdx.x & 7);
+    const long j = block >> 3;
+    const int split = (int)(j / tiles) * 8 + (block & 7);
     if (split >= a.splits) return;
     const int tile = (int)(j % tiles), k0 = (tile % kt) * W, o0 = (tile / kt) * W;
     const long steps = (a.n + BR - 1) / BR;
@@ -818,12 +823,22 @@ __global__ __launch_bounds__(W * W / 64, W == 256 ? 4 : 2) void k_dense_weights(
     // 16 rows of products and the next, and the chunk's registers are asked for the step after that: a load has a whole step to arrive
     const long count = s1 - s0;
     if (count > 0) {
+        if (whole && rows >= 2 * BR && count > 1) {
 #pragma unroll
-        for (int i = 0; i < NC; ++i) load(0, i);
+            for (int i = 0; i < NC; ++i) load_whole(0, i);
 #pragma unroll
-        for (int i = 0; i < NC; ++i) {
-            stage(lds, i);
-            if (count > 1) load(1, i);
+            for (int i = 0; i < NC; ++i) {
+                stage(lds, i);
+                load_whole(1, i);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < NC; ++i) load(0, i);
+#pragma unroll
+            for (int i = 0; i < NC; ++i) {
+                stage(lds, i);
+                if (count > 1) load(1, i);
+            }
         }
         __syncthreads();
         long s = 0;
@@ -882,6 +897,19 @@ __global__ __launch_bounds__(W * W / 64, W == 256 ? 4 : 2) void k_dense_weights(
         }
 }
 
+template <int T, int W> __global__ __launch_bounds__(W * W / 64, W == 256 ? 4 : 2) void k_dense_weights(DenseWeights a) {
+    __shared__ __attribute__((aligned(16))) unsigned short lds[2 * WeightsTile<T, W>::BUFFER];
+    dense_weights_tile<T, W>(a, blockIdx.x, lds);
+}
+
+// Both gradients of few rows in one launch: neither fills the chip, and they read the same dY.  The weight tiles, which take longer, come first.
+template <int T> __global__ __launch_bounds__(256, 2) void k_dense_backward_few(DenseRows x, DenseWeights w, unsigned weight_blocks) {
+    __shared__ __attribute__((aligned(16))) unsigned short lds[2 * WeightsTile<T, 128>::BUFFER];
+    static_assert(sizeof(lds) >= FEW_LDS * sizeof(float), "one memory for both");
+    if (blockIdx.x < weight_blocks) dense_weights_tile<T, 128>(w, blockIdx.x, lds);
+    else dense_few<T, true>(x, blockIdx.x - weight_blocks, reinterpret_cast<float*>(lds));
+}
+
 template <int T> __global__ __launch_bounds__(256) void k_dense_weights_sum(DenseWeights a) {
     const long nw = (long)a.o * a.k, i = (long)blockIdx.x * 256 + threadIdx.x;
     if (i >= nw + (a.db ? a.o : 0)) return;
@@ -929,7 +957,10 @@ template <int T> __global__ __launch_bounds__(256) void k_checkpoint_values(Chec
     }
 }
 
+// few tiles of 128 x 128: small ones instead
 constexpr long FEW_TILES = 64;
+bool few_rows(const DenseRows& a) { return ((a.n + 127) / 128) * ((a.o + 127) / 128) <= FEW_TILES; }
+unsigned few_blocks(const DenseRows& a) { return (unsigned)(((a.n + 31) / 32) * ((a.o + 31) / 32)); }
 
 // Which form Y = act(A B + bias) runs in, and the fragments' memory: the tall form for the 16-bit types once its tiles of 128 rows give every compute unit one (rows of 8
 // elements at least: it reads whole chunks; and as long as the biases of all passes fit LDS beside the two buffers).  A pass makes 256 outputs.
@@ -972,9 +1003,8 @@ template <int T, bool DX> hipError_t dense_rows(const DenseRows& a, void* ws, hi
             else return !a.codes ? dense_tall<T, TALL_Y>(a, p, wf, s) : a.relu ? dense_tall<T, TALL_RELU_KEEP>(a, p, wf, s) : dense_tall<T, TALL_KEEP>(a, p, wf, s);
         }
     }
-    // few tiles of 128 x 128: small ones instead
-    if (((a.n + 127) / 128) * ((a.o + 127) / 128) <= FEW_TILES) {
-        hipLaunchKernelGGL((k_dense_few<T, DX>), dim3((unsigned)(((a.n + 31) / 32) * ((a.o + 31) / 32))), dim3(256), 0, s, a);
+    if (few_rows(a)) {
+        hipLaunchKernelGGL((k_dense_few<T, DX>), dim3(few_blocks(a)), dim3(256), 0, s, a);
         return hipGetLastError();
     }
     const long pt = ((a.n + 127) / 128 + 7) / 8 * 8;
@@ -998,10 +1028,16 @@ WeightsPlan weights_plan(int type, long n, int k, int o) {
     return p;
 }
 
-template <int T> hipError_t dense_weights(const DenseWeights& a, hipStream_t s) {
+// (x: the input gradient where that is asked for too and runs in the few-rows form, or null)
+template <int T> hipError_t dense_weights(const DenseWeights& a, const DenseRows* x, hipStream_t s) {
     const WeightsPlan p = weights_plan(T, a.n, a.k, a.o);
     const dim3 grid((unsigned)((p.splits + 7) / 8 * 8 * p.tiles));
-    if (p.width == 256) hipLaunchKernelGGL((k_dense_weights<T, 256>), grid, dim3(1024), 0, s, a);
+    if (x && p.width == 128) {
+        hipLaunchKernelGGL((k_dense_backward_few<T>), dim3(grid.x + few_blocks(*x)), dim3(256), 0, s, *x, a, grid.x);
+    } else if (x) {
+        hipLaunchKernelGGL((k_dense_few<T, true>), dim3(few_blocks(*x)), dim3(256), 0, s, *x);
+        hipLaunchKernelGGL((k_dense_weights<T, 256>), grid, dim3(1024), 0, s, a);
+    } else if (p.width == 256) hipLaunchKernelGGL((k_dense_weights<T, 256>), grid, dim3(1024), 0, s, a);
     else hipLaunchKernelGGL((k_dense_weights<T, 128>), grid, dim3(256), 0, s, a);
     if (a.splits > 1) {
         const long m = (long)a.o * a.k + a.o;
@@ -1029,8 +1065,15 @@ hipError_t launch_dense_rows(int type, bool input_gradient, const DenseRows& a, 
     return type == LT_F32 ? dense_rows<LT_F32, false>(a, ws, s) : type == LT_BF16 ? dense_rows<LT_BF16, false>(a, ws, s) : dense_rows<LT_F16, false>(a, ws, s);
 }
 
-hipError_t launch_dense_weights(int type, const DenseWeights& a, hipStream_t s) {
-    return type == LT_F32 ? dense_weights<LT_F32>(a, s) : type == LT_BF16 ? dense_weights<LT_BF16>(a, s) : dense_weights<LT_F16>(a, s);
+hipError_t launch_dense_backward(int type, const DenseRows* x, const DenseWeights* w, void* ws, hipStream_t s) {
+    const bool together = x && w && x->n > 0 && few_rows(*x);
+    if (x && x->n > 0 && !together) {
+        const hipError_t e = launch_dense_rows(type, true, *x, ws, s);
+        if (e != hipSuccess) return e;
+    }
+    if (!w) return hipSuccess;
+    const DenseRows* both = together ? x : nullptr;
+    return type == LT_F32 ? dense_weights<LT_F32>(*w, both, s) : type == LT_BF16 ? dense_weights<LT_BF16>(*w, both, s) : dense_weights<LT_F16>(*w, both, s);
 }
 
 hipError_t launch_checkpoint(int type, const void* x, long ld, long n, int k, int is_signed, uint8_t* codes, uint8_t* scales, hipStream_t s) {

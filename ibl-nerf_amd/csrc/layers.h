@@ -42,7 +42,8 @@ struct DenseWeights {
     int splits;
 };
 int dense_weight_splits(int type, long n, int k, int o);      // how many pieces the rows are cut into (a function of the sizes alone: results repeat bit for bit)
-hipError_t launch_dense_weights(int type, const DenseWeights& a, hipStream_t s);
+// both gradients of a layer, or one (null: not asked for); ws is the input gradient's scratch memory
+hipError_t launch_dense_backward(int type, const DenseRows* x, const DenseWeights* w, void* ws, hipStream_t s);
 
 hipError_t launch_checkpoint(int type, const void* x, long ld, long n, int k, int is_signed, uint8_t* codes, uint8_t* scales, hipStream_t s);
 hipError_t launch_checkpoint_values(int type, const Checkpoint8& c, long n, int k, void* out, long ld, hipStream_t s);

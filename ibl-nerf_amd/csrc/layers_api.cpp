@@ -96,18 +96,13 @@ int iblnerf_dense_backward(void* stream, int dtype, const void* d_dy, int64_t ld
     const size_t need = iblnerf_dense_backward_workspace(dtype, n, k, o);
     if (bad_workspace(d_workspace, workspace_bytes, need))
         return fail(IBLNERF_ERR_INVALID, "dense_backward: a workspace of %zu bytes is needed, %zu given", need, d_workspace ? workspace_bytes : (size_t)0);
-    if (d_dx && n > 0) {
-        DenseRows a{};
-        a.a = d_dy; a.lda = ld_dy; a.w = d_w; a.ldw = ld_w; a.open = d_y_codes; a.y = d_dx; a.ldy = ld_dx; a.n = n; a.r = o; a.o = k;
-        const int rc = done("dense_backward (input)", launch_dense_rows(dtype, true, a, d_workspace, (hipStream_t)stream));
-        if (rc) return rc;
-    }
-    if (!d_dw) return IBLNERF_OK;
+    DenseRows a{};
+    a.a = d_dy; a.lda = ld_dy; a.w = d_w; a.ldw = ld_w; a.open = d_y_codes; a.y = d_dx; a.ldy = ld_dx; a.n = n; a.r = o; a.o = k;
     DenseWeights w{};
     w.dy = d_dy; w.lddy = ld_dy; w.open = d_y_codes; w.x = Checkpoint8{d_x_codes, d_x_scales, x_is_signed != 0}; w.dw = d_dw; w.db = d_db; w.grad32 = grad_dtype == IBLNERF_FLOAT32;
     w.splits = dense_weight_splits(dtype, n, k, o);
     w.bias_part = static_cast<double*>(d_workspace); w.part = reinterpret_cast<float*>(w.bias_part + (size_t)w.splits * o); w.n = n; w.k = k; w.o = o;
-    return done("dense_backward (weights)", launch_dense_weights(dtype, w, (hipStream_t)stream));
+    return done("dense_backward", launch_dense_backward(dtype, d_dx ? &a : nullptr, d_dw ? &w : nullptr, d_workspace, (hipStream_t)stream));
 }
 
 static bool bad_lookup(int dtype, int64_t v, int d, const void* index, int bits, int64_t n, int64_t per) {

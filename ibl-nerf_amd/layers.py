@@ -219,11 +219,14 @@ class _Dense(torch.autograd.Function):
         ctx.relu, ctx.x_signed, ctx.has_bias, ctx.type, ctx.bias_dtype = relu, x_signed, bias is not None, x.dtype, None if bias is None else bias.dtype
         ctx.save_for_backward(weight, x_codes, x_scales, *((kept.codes, kept.scales) if relu else ()))
         ctx.mark_non_differentiable(kept.codes, kept.scales)
+        ctx.set_materialize_grads(False)                       # (or zeros of the codes' size would be written for them)
         return y, kept.codes, kept.scales
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy, _codes, _scales):
+        if dy is None:
+            return (None,) * 7
         weight, xc, xs, *out = ctx.saved_tensors
         k, o = weight.shape[1], weight.shape[0]
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
