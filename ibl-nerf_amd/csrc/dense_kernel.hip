@@ -17,6 +17,8 @@
 #include "layer_elems.h"
 #include "layers.h"
 
+#include <type_traits>
+
 namespace ibl {
 
 namespace {
@@ -70,7 +72,8 @@ template <int BK> __device__ __forceinline__ int along(int i, int c) {
     return i * BK + ((c ^ ((i / (16 / C)) % C)) * 8);
 }
 // "across": one row of W columns for each reduction index; the 64-byte chunk c of row p at place c ^ (p & 3): the transposing read below takes 4 rows x 64 bytes at once
-template <int W> __device__ __forceinline__ int across(int p, int c32) { return p * W + ((c32 ^ (p & 3)) * 32); }
+// (rows of one chunk lie side by side as they are)
+template <int W> __device__ __forceinline__ int across(int p, int c32) { return p * W + ((c32 ^ (p & 3 & (W / 32 - 1))) * 32); }
 
 // Operand fragments of step ks (16 reduction elements): lane (i = lane & 31, h = lane >> 5) holds elements 8 h .. 8 h + 7 of column / row i of the 32-wide tile
 template <int BK> __device__ __forceinline__ u32x4 frag_along(const unsigned short* t, int row0, int ks, int lane) {
@@ -348,6 +351,22 @@ __global__ __launch_bounds__(256, 2) void k_dense_rows(DenseRows a) {
     write_rows<T, DX, TO, TP>(a, acc, lds + wave * Window<TO, T>::bytes, p0 + wp, o0 + wo, lane);
 }
 
+// outputs o .. o + 7 of row p, and their codes (four neighbouring lanes hold a block; rows and outputs beyond the last are not written)
+template <int T, bool DX> __device__ __forceinline__ void finish8(const DenseRows& a, long p, int o, const float (&f)[8]) {
+    const Raw8<T> v = from_floats<T>(f);
+    const bool in = p < a.n;
+    if (in && o < a.o) store8<T>(static_cast<char*>(a.y) + p * a.ldy * Bytes<T>::v, o, a.o, v);
+    if (!DX && a.codes) {
+        u32x2 codes; unsigned scale;
+        encode8<T>(v, a.is_signed != 0, codes, scale);
+        const int o32 = (a.o + 31) & ~31;
+        if (in) {
+            *reinterpret_cast<u32x2*>(a.codes + p * o32 + o) = codes;
+            if ((o & 31) == 0) a.scales[p * (o32 >> 5) + (o >> 5)] = (uint8_t)scale;
+        }
+    }
+}
+
 // The form for few rows, where one latency after the other is what a call costs: a workgroup makes 32 rows x 32 outputs, each of its 4 waves over a quarter of the reduction, straight
 // from global memory (operands in the order they lie there, 4 steps asked for at once), and the quarters meet in LDS once.
 constexpr int FEW_ROW = 36, FEW_LDS = 4 * 32 * FEW_ROW;      // floats
@@ -432,18 +451,7 @@ template <int T, bool DX> __device__ __forceinline__ void dense_few(const DenseR
         if (!DX && a.relu) v = __builtin_elementwise_maximum(v, 0.0f);
         f[e] = !DX && o0 + c + e >= a.o ? 0.0f : v;      // (columns beyond the layer's outputs are coded 0)
     }
-    const Raw8<T> v = from_floats<T>(f);
-    const bool in = p0 + row < a.n;
-    if (in && o0 + c < a.o) store8<T>(static_cast<char*>(a.y) + (p0 + row) * a.ldy * Bytes<T>::v, o0 + c, a.o, v);
-    if (!DX && a.codes) {
-        u32x2 codes; unsigned scale;
-        encode8<T>(v, a.is_signed != 0, codes, scale);
-        const int o32 = (a.o + 31) & ~31;
-        if (in) {
-            *reinterpret_cast<u32x2*>(a.codes + (p0 + row) * o32 + o0 + c) = codes;
-            if (c == 0) a.scales[(p0 + row) * (o32 >> 5) + (o0 >> 5)] = (uint8_t)scale;
-        }
-    }
+    finish8<T, DX>(a, p0 + row, o0 + c, f);
 }
 
 template <int T, bool DX> __global__ __launch_bounds__(256) void k_dense_few(DenseRows a) {
@@ -451,12 +459,8 @@ template <int T, bool DX> __global__ __launch_bounds__(256) void k_dense_few(Den
     dense_few<T, DX>(a, blockIdx.x, sums);
 }
 
-// The weights as matrix operands for k_dense_tall: [32-wide tile][16 reduction elements][lane][8], zeros beyond the layer
-template <int T, bool DX> __global__ __launch_bounds__(256) void k_dense_fragments(DenseRows a, u32x4* wf, int tiles, int steps) {
-    const int id = blockIdx.x * 256 + threadIdx.x;
-    const int lane = id & 63, ks = (id >> 6) % steps, tile = (id >> 6) / steps;
-    if (tile >= tiles) return;
-    const int i = 32 * tile + (lane & 31), r0 = 16 * ks + 8 * (lane >> 5);
+// One lane's 8 reduction elements of output i of the weights, zeros beyond the layer (16-bit types)
+template <int T, bool DX> __device__ __forceinline__ u32x4 weight_fragment(const DenseRows& a, int i, int r0) {
     u32x4 v = {0, 0, 0, 0};
     if (i < a.o) {
         if (!DX) {
@@ -468,7 +472,79 @@ template <int T, bool DX> __global__ __launch_bounds__(256) void k_dense_fragmen
                 if (r0 + e < a.r) v[e >> 1] |= (unsigned)w[(long)(r0 + e) * a.ldw] << (16 * (e & 1));
         }
     }
-    wf[id] = v;
+    return v;
+}
+
+// The form for many rows of at most 32 outputs (16-bit types): a wave takes 32 rows at a time, straight from memory in the order the matrix instruction wants them; the weights'
+// operands stay in LDS.  Chunks are read whole: what lies behind a row's end is cleared in registers, and only rows with 7 more behind them are read so.
+template <int T, bool DX> __global__ __launch_bounds__(256, 4) void k_dense_narrow(DenseRows a) {
+    constexpr int U = 4;
+    extern __shared__ __attribute__((aligned(16))) float narrow[];
+    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), i = lane & 31, h = lane >> 5;
+    const int steps = (a.r + 15) >> 4, r32 = (a.r + 31) & ~31, last = (a.r - 1) & ~7;
+    float* win = narrow + wave * 32 * FEW_ROW;
+    u32x4* wf = reinterpret_cast<u32x4*>(narrow + FEW_LDS);
+    for (int id = t; id < 64 * steps; id += 256) wf[id] = weight_fragment<T, DX>(a, id & 31, 16 * (id >> 6) + 8 * ((id >> 5) & 1));
+    f32x16 bias = {0};
+    if (!DX)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) bias[r] = bias_at<T>(a, (r & 3) + 8 * (r >> 2) + 4 * h);
+    __syncthreads();
+    for (long p0 = 32 * ((long)blockIdx.x * 4 + wave); p0 < a.n; p0 += 128L * gridDim.x) {
+        const long p = min(p0 + i, a.n - 1);
+        const char* x = static_cast<const char*>(a.a) + p * a.lda * 2;
+        const bool all = p0 + 32 + 7 <= a.n;
+        f32x16 acc = bias;
+        for (int s0 = 0; s0 < steps; s0 += U) {
+            Raw8<T> xv[U];
+            u32x2 q[U];
+            if (all) {
+#pragma unroll
+                for (int u = 0; u < U; ++u) xv[u].q[0] = load16(x + 2L * min(16 * (s0 + u) + 8 * h, last));
+            } else {
+#pragma unroll
+                for (int u = 0; u < U; ++u) xv[u] = load8<T>(x, 16 * (s0 + u) + 8 * h, a.r);
+            }
+            if (DX && a.open)
+#pragma unroll
+                for (int u = 0; u < U; ++u) q[u] = *reinterpret_cast<const u32x2*>(a.open + p * r32 + min(16 * (s0 + u) + 8 * h, last));
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (s0 + u >= steps) break;
+                if (DX && a.open) close8<T>(xv[u], q[u]);
+                if (16 * (s0 + u) + 16 > a.r) {
+                    const int left = a.r - 16 * (s0 + u) - 8 * h;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) xv[u].q[0][j] = left >= 2 * j + 2 ? xv[u].q[0][j] : left == 2 * j + 1 ? xv[u].q[0][j] & 0xffffu : 0u;
+                }
+                acc = mfma<T>(wf[64 * (s0 + u) + lane], xv[u].q[0], acc);
+            }
+        }
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+            *reinterpret_cast<u32x4*>(win + i * FEW_ROW + 8 * g + 4 * h) = u32x4{as_bits(acc[4 * g]), as_bits(acc[4 * g + 1]), as_bits(acc[4 * g + 2]), as_bits(acc[4 * g + 3])};
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int z = 0; z < 2; ++z) {
+            const int row = 16 * z + (lane >> 2), c = 8 * (lane & 3);
+            float f[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float v = win[row * FEW_ROW + c + e];
+                f[e] = !DX && c + e >= a.o ? 0.0f : !DX && a.relu ? __builtin_elementwise_maximum(v, 0.0f) : v;
+            }
+            finish8<T, DX>(a, p0 + row, c, f);
+        }
+        __builtin_amdgcn_wave_barrier();
+    }
+}
+
+// The weights as matrix operands for k_dense_tall: [32-wide tile][16 reduction elements][lane][8], zeros beyond the layer
+template <int T, bool DX> __global__ __launch_bounds__(256) void k_dense_fragments(DenseRows a, u32x4* wf, int tiles, int steps) {
+    const int id = blockIdx.x * 256 + threadIdx.x;
+    const int lane = id & 63, ks = (id >> 6) % steps, tile = (id >> 6) / steps;
+    if (tile >= tiles) return;
+    wf[id] = weight_fragment<T, DX>(a, 32 * tile + (lane & 31), 16 * ks + 8 * (lane >> 5));
 }
 
 constexpr int TALL_ROWS = 128;
@@ -725,68 +801,82 @@ __global__ __launch_bounds__(256, 2) void k_dense_tall(DenseRows a, const u32x4*
 // bits every time.
 //
 // W = 128: 4 waves, two workgroups on a compute unit; W = 256: 16 waves, half as many reads of either operand.  A wave takes 64 x 64.
-template <int T, int W> struct WeightsTile {
-    static constexpr int PARTS = T == LT_F32 ? 3 : 1, BR = T == LT_F32 ? 32 : 64, PLANE = BR * W, BUFFER = (PARTS + 1) * PLANE;
+template <int T, int WO, int WK> struct WeightsTile {
+    static constexpr int NT = WO == 256 ? 1024 : 256, PARTS = T == LT_F32 ? 3 : 1, BR = T == LT_F32 && WO != 32 ? 32 : 64;
+    static constexpr int ZPLANE = BR * WO, XPLANE = BR * WK, BUFFER = PARTS * ZPLANE + XPLANE;
+    static constexpr int TO = WO >= 128 && WK >= 128 ? 2 : 1, TK = TO;                       // 32-wide tiles of a wave
+    static constexpr int SHARE = NT / 64 / ((WO / 32 / TO) * (WK / 32 / TK));                // waves that share a tile, each with every SHARE-th 16 rows
 };
-template <int T, int W> __device__ __forceinline__ void dense_weights_tile(const DenseWeights& a, unsigned block, unsigned short* lds) {
-    constexpr int PARTS = WeightsTile<T, W>::PARTS, BR = WeightsTile<T, W>::BR, NT = W * W / 64, TO = 2, TK = 2;
-    constexpr int RT = W / 8, RP = NT / RT, NC = BR / RP;      // threads a row of a tile, rows at a time, 8-column chunks a thread stages
-    constexpr int PLANE = WeightsTile<T, W>::PLANE, BUFFER = WeightsTile<T, W>::BUFFER;
-    static_assert(NC >= 1 && NC <= BR / 16, "a chunk for each step of 16 rows at most");
+template <int T, int WO, int WK> __device__ __forceinline__ void dense_weights_tile(const DenseWeights& a, unsigned block, unsigned short* lds) {
+    using W = WeightsTile<T, WO, WK>;
+    constexpr int PARTS = W::PARTS, BR = W::BR, NT = W::NT, TO = W::TO, TK = W::TK, ZPLANE = W::ZPLANE, BUFFER = W::BUFFER, SHARE = W::SHARE;
+    // threads a row of either tile, rows at a time, 8-column chunks a thread stages (a thread without one stages another's again)
+    constexpr int RTZ = WO / 8, RTX = WK / 8, RPZ = NT / RTZ < BR ? NT / RTZ : BR, RPX = NT / RTX < BR ? NT / RTX : BR, NZ = BR / RPZ, NX = BR / RPX, NC = NZ > NX ? NZ : NX;
+    static_assert(NC <= BR / 16, "a chunk for each step of 16 rows at most");
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
-    const int kt = (a.k + W - 1) / W, ot = (a.o + W - 1) / W, tiles = kt * ot;
+    const int kt = (a.k + WK - 1) / WK, ot = (a.o + WO - 1) / WO, tiles = kt * ot;
     const long j = block >> 3;
     const int split = (int)(j / tiles) * 8 + (block & 7);
     if (split >= a.splits) return;
-    const int tile = (int)(j % tiles), k0 = (tile % kt) * W, o0 = (tile / kt) * W;
+    const int tile = (int)(j % tiles), k0 = (tile % kt) * WK, o0 = (tile / kt) * WO;
     const long steps = (a.n + BR - 1) / BR;
     const long s0 = steps * split / a.splits, s1 = steps * (split + 1) / a.splits;
     const int k32 = (a.k + 31) & ~31, o32 = (a.o + 31) & ~31;
-    // the thread's 8 columns of either tile are the same in every step; its rows: t / RT + RP * i.  Addresses are a scalar base that moves with the steps and 32-bit offsets
-    const int cc = 8 * (t % RT), row = t / RT;
+    // the thread's 8 columns of either tile are the same in every step; its rows: zrow + RPZ * i, xrow + RPX * i.  Addresses are a scalar base that moves with the steps and 32-bit
+    // offsets
+    const int zcc = 8 * (t % RTZ), zrow = (t / RTZ) % BR, xcc = 8 * (t % RTX), xrow = (t / RTX) % BR;
     // (columns beyond the outputs or inputs: any, their sums are not written)
-    const int zc = o0 + cc < a.o ? o0 + cc : 0, xc0 = k0 + cc < k32 ? k0 + cc : 0;
-    const unsigned zo = (unsigned)(row * (int)a.lddy + zc) * Bytes<T>::v, oo = row * o32 + zc, co = row * k32 + xc0, so = row * (k32 >> 5) + (xc0 >> 5);
+    const int zc = o0 + zcc < a.o ? o0 + zcc : 0, xc0 = k0 + xcc < k32 ? k0 + xcc : 0;
+    const unsigned zo = (unsigned)(zrow * (int)a.lddy + zc) * Bytes<T>::v, oo = zrow * o32 + zc, co = xrow * k32 + xc0, so = xrow * (k32 >> 5) + (xc0 >> 5);
     const char* zb = static_cast<const char*>(a.dy) + s0 * BR * a.lddy * Bytes<T>::v;
     const uint8_t *ob = a.open + s0 * BR * o32, *cb = a.x.codes + s0 * BR * k32, *sb = a.x.scales + s0 * BR * (k32 >> 5);
     const long rows = a.n - s0 * BR;
-    const bool whole = (a.o & 7) == 0;          // every 8-column chunk of dY is whole or absent
 
-    Raw8<T> zr[NC];
-    u32x2 cr[NC], xc[NC];
-    unsigned xs[NC];
-    auto load_whole = [&](long step, int i) {   // (step counts from s0) every row and chunk is there: straight code, the loads travel together
-        const long at = step * BR + RP * i;
-        const char* z = zb + at * a.lddy * Bytes<T>::v;
-        zr[i].q[0] = load16(z + zo);
-        if constexpr (T == LT_F32) zr[i].q[1] = load16(z + zo + 16);
-        if (a.open) cr[i] = *reinterpret_cast<const u32x2*>(ob + at * o32 + oo);
-        xc[i] = *reinterpret_cast<const u32x2*>(cb + at * k32 + co);
-        xs[i] = (sb + at * (k32 >> 5))[so];
-    };
-    auto load = [&](long step, int i) {
-        const long at = step * BR + RP * i;
-        const bool in = at + row < rows;
-        zr[i] = in ? load8<T>(zb + at * a.lddy * Bytes<T>::v + zo, 0, a.o - zc) : zero8<T>();
-        if (a.open && in) cr[i] = *reinterpret_cast<const u32x2*>(ob + at * o32 + oo);
-        xc[i] = in ? *reinterpret_cast<const u32x2*>(cb + at * k32 + co) : u32x2{0, 0};
-        xs[i] = in ? (sb + at * (k32 >> 5))[so] : 127u;
+    Raw8<T> zr[NZ];
+    u32x2 cr[NZ], xc[NX];
+    unsigned xs[NX];
+    // Chunk i of a step (counted from s0) into registers.  ALL: every row of the step is there and 7 more behind it, so that whole chunks may be read beyond a row's last column
+    // (their sums are not written): straight code, the loads travel together.  Otherwise what is there, and zeros.
+    auto load = [&](long step, int i, auto ALL) {
+        if (i < NZ) {
+            const long at = step * BR + RPZ * i;
+            const char* z = zb + at * a.lddy * Bytes<T>::v;
+            const uint8_t* open = ob + at * o32;
+            if constexpr (decltype(ALL)::value) {
+                zr[i].q[0] = load16(z + zo);
+                if constexpr (T == LT_F32) zr[i].q[1] = load16(z + zo + 16);
+                if (a.open) cr[i] = *reinterpret_cast<const u32x2*>(open + oo);
+            } else {
+                const bool in = at + zrow < rows;
+                zr[i] = in ? load8<T>(z + zo, 0, a.o - zc) : zero8<T>();
+                if (a.open && in) cr[i] = *reinterpret_cast<const u32x2*>(open + oo);
+            }
+        }
+        if (i < NX) {
+            const long at = step * BR + RPX * i;
+            const uint8_t *codes = cb + at * k32, *scales = sb + at * (k32 >> 5);
+            const bool in = decltype(ALL)::value || at + xrow < rows;
+            xc[i] = in ? *reinterpret_cast<const u32x2*>(codes + co) : u32x2{0, 0};
+            xs[i] = in ? scales[so] : 127u;
+        }
     };
     auto stage = [&](unsigned short* zt, int i) {
-        unsigned short* xt = zt + PARTS * PLANE;
-        const int at = across<W>(row + RP * i, (t % RT) >> 2) + 8 * (t & 3);
-        if (a.open) close8<T>(zr[i], cr[i]);
-        stage8<T>(zt + at, PLANE, zr[i]);
-        float f[8];
-        decode8(xc[i], xs[i], a.x.is_signed != 0, f);
-        u32x4 v;
+        if (i < NZ) {
+            if (a.open) close8<T>(zr[i], cr[i]);
+            stage8<T>(zt + across<WO>(zrow + RPZ * i, (t % RTZ) >> 2) + 8 * (t & 3), ZPLANE, zr[i]);
+        }
+        if (i < NX) {
+            float f[8];
+            decode8(xc[i], xs[i], a.x.is_signed != 0, f);
+            u32x4 v;
 #pragma unroll
-        for (int e = 0; e < 4; ++e)      // a value has at most 8 significant bits: its upper 16 bits are all of it
-            v[e] = T == LT_F16 ? pack2<LT_F16>(f[2 * e], f[2 * e + 1]) : __builtin_amdgcn_perm(as_bits(f[2 * e + 1]), as_bits(f[2 * e]), 0x07060302u);
-        *reinterpret_cast<u32x4*>(xt + at) = v;
+            for (int e = 0; e < 4; ++e)      // a value has at most 8 significant bits: its upper 16 bits are all of it
+                v[e] = T == LT_F16 ? pack2<LT_F16>(f[2 * e], f[2 * e + 1]) : __builtin_amdgcn_perm(as_bits(f[2 * e + 1]), as_bits(f[2 * e]), 0x07060302u);
+            *reinterpret_cast<u32x4*>(zt + PARTS * ZPLANE + across<WK>(xrow + RPX * i, (t % RTX) >> 2) + 8 * (t & 3)) = v;
+        }
     };
 
-    const int wo = (wave / (W / 64)) * TO, wk = (wave % (W / 64)) * TK;      // the wave's first 32-wide tile of either side
+    const int place = wave / SHARE, wo = (place / (WK / 32 / TK)) * TO, wk = (place % (WK / 32 / TK)) * TK;      // the wave's first 32-wide tile of either side
     f32x16 acc[TO][TK];
 #pragma unroll
     for (int i = 0; i < TO; ++i)
@@ -795,17 +885,18 @@ template <int T, int W> __device__ __forceinline__ void dense_weights_tile(const
     // The bias gradient falls off the fragments (a lane has 8 rows of one output), in the waves of the first column tile.  It is one sum over all rows with nothing to average an
     // error out: added up in 64 bits
     const bool sums = a.db != nullptr && k0 == 0 && wk == 0;
-    double bs[TO] = {0.0, 0.0};
+    double bs[TO] = {};
     auto multiply = [&](const unsigned short* zt, int ks) {
-        const unsigned short* xt = zt + PARTS * PLANE;
+        if (SHARE > 1 && ks % SHARE != wave % SHARE) return;
+        const unsigned short* xt = zt + PARTS * ZPLANE;
         u32x4 x[TK][1];
 #pragma unroll
-        for (int k = 0; k < TK; ++k) x[k][0] = frag_across<W>(xt, wk + k, ks, lane);
+        for (int k = 0; k < TK; ++k) x[k][0] = frag_across<WK>(xt, wk + k, ks, lane);
 #pragma unroll
         for (int i = 0; i < TO; ++i) {
             u32x4 z[PARTS];
 #pragma unroll
-            for (int q = 0; q < PARTS; ++q) z[q] = frag_across<W>(zt + q * PLANE, wo + i, ks, lane);
+            for (int q = 0; q < PARTS; ++q) z[q] = frag_across<WO>(zt + q * ZPLANE, wo + i, ks, lane);
 #pragma unroll
             for (int k = 0; k < TK; ++k) acc[i][k] = product<T, PARTS, 1>(z, x[k], acc[i][k]);
             if (sums)
@@ -822,34 +913,36 @@ template <int T, int W> __device__ __forceinline__ void dense_weights_tile(const
     // One barrier a step: while a step's products run, the next one's elements — already in registers — are masked, decoded and written to the other buffer, a chunk between
     // 16 rows of products and the next, and the chunk's registers are asked for the step after that: a load has a whole step to arrive
     const long count = s1 - s0;
+    constexpr std::true_type all{};
+    constexpr std::false_type some{};
     if (count > 0) {
-        if (whole && rows >= 2 * BR && count > 1) {
+        if (rows >= 2 * BR + 7 && count > 1) {
 #pragma unroll
-            for (int i = 0; i < NC; ++i) load_whole(0, i);
+            for (int i = 0; i < NC; ++i) load(0, i, all);
 #pragma unroll
             for (int i = 0; i < NC; ++i) {
                 stage(lds, i);
-                load_whole(1, i);
+                load(1, i, all);
             }
         } else {
 #pragma unroll
-            for (int i = 0; i < NC; ++i) load(0, i);
+            for (int i = 0; i < NC; ++i) load(0, i, some);
 #pragma unroll
             for (int i = 0; i < NC; ++i) {
                 stage(lds, i);
-                if (count > 1) load(1, i);
+                if (count > 1) load(1, i, some);
             }
         }
         __syncthreads();
         long s = 0;
-        const long full = whole ? rows / BR - 2 : -1;      // steps whose next but one is whole
+        const long full = (rows - 7) / BR - 2;      // steps whose next but one is whole
         for (; s + 2 < count && s < full; ++s) {
             const int b = (int)s & 1;
 #pragma unroll
             for (int i = 0; i < BR / 16; ++i) {
                 if (i < NC) {
                     stage(lds + (b ^ 1) * BUFFER, i);
-                    load_whole(s + 2, i);
+                    load(s + 2, i, all);
                 }
                 multiply(lds + b * BUFFER, i);
             }
@@ -861,12 +954,34 @@ template <int T, int W> __device__ __forceinline__ void dense_weights_tile(const
             for (int i = 0; i < BR / 16; ++i) {
                 if (i < NC && s + 1 < count) {
                     stage(lds + (b ^ 1) * BUFFER, i);
-                    if (s + 2 < count) load(s + 2, i);
+                    if (s + 2 < count) load(s + 2, i, some);
                 }
                 multiply(lds + b * BUFFER, i);
             }
             __syncthreads();
         }
+    }
+    if constexpr (SHARE > 1) {      // the waves' shares meet in LDS: a register of the tile is added up in the order of the waves (TO = TK = 1)
+        float* fs = reinterpret_cast<float*>(lds);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) fs[wave * 1024 + 64 * r + lane] = acc[0][0][r];
+        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            float v = fs[place * SHARE * 1024 + 64 * r + lane];
+#pragma unroll
+            for (int q = 1; q < SHARE; ++q) v += fs[(place * SHARE + q) * 1024 + 64 * r + lane];
+            acc[0][0][r] = v;
+        }
+        __syncthreads();
+        double* ds = reinterpret_cast<double*>(lds);
+        ds[t] = bs[0];
+        __syncthreads();
+        double v = ds[64 * place * SHARE + lane];
+#pragma unroll
+        for (int q = 1; q < SHARE; ++q) v += ds[64 * (place * SHARE + q) + lane];
+        bs[0] = v;
+        if (wave % SHARE != 0) return;
     }
     const bool last = a.splits == 1;
     auto put = [&](void* to, long at, float v) {
@@ -897,32 +1012,41 @@ template <int T, int W> __device__ __forceinline__ void dense_weights_tile(const
         }
 }
 
-template <int T, int W> __global__ __launch_bounds__(W * W / 64, W == 256 ? 4 : 2) void k_dense_weights(DenseWeights a) {
-    __shared__ __attribute__((aligned(16))) unsigned short lds[2 * WeightsTile<T, W>::BUFFER];
-    dense_weights_tile<T, W>(a, blockIdx.x, lds);
+template <int T, int WO, int WK> __global__ __launch_bounds__(WO == 256 ? 1024 : 256, (WO == 128 && WK == 128) || (T == LT_F32 && WO != WK) ? 2 : 4) void k_dense_weights(DenseWeights a) {
+    __shared__ __attribute__((aligned(16))) unsigned short lds[2 * WeightsTile<T, WO, WK>::BUFFER];
+    static_assert(WeightsTile<T, WO, WK>::SHARE == 1 || sizeof(lds) >= WeightsTile<T, WO, WK>::NT / 64 * 4096, "the shares of a tile");
+    dense_weights_tile<T, WO, WK>(a, blockIdx.x, lds);
 }
 
 // Both gradients of few rows in one launch: neither fills the chip, and they read the same dY.  The weight tiles, which take longer, come first.
 template <int T> __global__ __launch_bounds__(256, 2) void k_dense_backward_few(DenseRows x, DenseWeights w, unsigned weight_blocks) {
-    __shared__ __attribute__((aligned(16))) unsigned short lds[2 * WeightsTile<T, 128>::BUFFER];
+    __shared__ __attribute__((aligned(16))) unsigned short lds[2 * WeightsTile<T, 128, 128>::BUFFER];
     static_assert(sizeof(lds) >= FEW_LDS * sizeof(float), "one memory for both");
-    if (blockIdx.x < weight_blocks) dense_weights_tile<T, 128>(w, blockIdx.x, lds);
+    if (blockIdx.x < weight_blocks) dense_weights_tile<T, 128, 128>(w, blockIdx.x, lds);
     else dense_few<T, true>(x, blockIdx.x - weight_blocks, reinterpret_cast<float*>(lds));
 }
 
-template <int T> __global__ __launch_bounds__(256) void k_dense_weights_sum(DenseWeights a) {
-    const long nw = (long)a.o * a.k, i = (long)blockIdx.x * 256 + threadIdx.x;
-    if (i >= nw + (a.db ? a.o : 0)) return;
-    const bool bias = i >= nw;
-    const long at = bias ? i - nw : i;
+// The pieces' sums in order, in 64 bits: a workgroup takes 64 of the o k + o values, its 16 waves every 16th piece each (a narrow layer has hundreds of pieces and few values)
+template <int T> __global__ __launch_bounds__(1024) void k_dense_weights_sum(DenseWeights a) {
+    __shared__ double sums[1024];
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+    const long nw = (long)a.o * a.k, i = (long)blockIdx.x * 64 + lane;
+    const bool weight = i < nw, bias = !weight && a.db && i < nw + a.o;
     double s = 0.0;
-    if (bias) {
-        for (int q = 0; q < a.splits; ++q) s += a.bias_part[(long)q * a.o + at];
-    } else {
+    if (weight) {
 #pragma unroll 16
-        for (int q = 0; q < a.splits; ++q) s += (double)a.part[q * nw + at];
+        for (int q = wave; q < a.splits; q += 16) s += (double)a.part[q * nw + i];
+    } else if (bias) {
+#pragma unroll 16
+        for (int q = wave; q < a.splits; q += 16) s += a.bias_part[(long)q * a.o + (i - nw)];
     }
+    sums[t] = s;
+    __syncthreads();
+    if (wave != 0 || !(weight || bias)) return;
+#pragma unroll
+    for (int q = 1; q < 16; ++q) s += sums[64 * q + lane];
     void* to = bias ? a.db : a.dw;
+    const long at = bias ? i - nw : i;
     if (T == LT_F32 || a.grad32) static_cast<float*>(to)[at] = (float)s;
     else static_cast<unsigned short*>(to)[at] = (unsigned short)pack2<T == LT_F32 ? LT_F16 : T>((float)s, 0.0f);
 }
@@ -964,11 +1088,12 @@ unsigned few_blocks(const DenseRows& a) { return (unsigned)(((a.n + 31) / 32) * 
 
 // Which form Y = act(A B + bias) runs in, and the fragments' memory: the tall form for the 16-bit types once its tiles of 128 rows give every compute unit one (rows of 8
 // elements at least: it reads whole chunks; and as long as the biases of all passes fit LDS beside the two buffers).  A pass makes 256 outputs.
-struct RowsPlan { bool tall; int passes, steps; };
+struct RowsPlan { bool tall, narrow; int passes, steps; };
 RowsPlan rows_plan(int type, long n, int r, int o) {
     RowsPlan p{};
     p.passes = (o + 255) / 256;
-    p.tall = type != LT_F32 && n >= 256 * TALL_ROWS && r >= 8 && p.passes <= 8;
+    p.narrow = type != LT_F32 && o <= 32 && r <= 512 && n > 128 * FEW_TILES;
+    p.tall = !p.narrow && type != LT_F32 && n >= 256 * TALL_ROWS && r >= 8 && p.passes <= 8;
     p.steps = (r + 63) / 64 * 4;
     return p;
 }
@@ -997,6 +1122,11 @@ template <int T, int MODE> hipError_t dense_tall(const DenseRows& a, const RowsP
 template <int T, bool DX> hipError_t dense_rows(const DenseRows& a, void* ws, hipStream_t s) {
     const RowsPlan p = rows_plan(T, a.n, a.r, a.o);
     if constexpr (T != LT_F32) {
+        if (p.narrow) {
+            const long groups = (a.n + 127) / 128;
+            hipLaunchKernelGGL((k_dense_narrow<T, DX>), dim3((unsigned)(groups < 2048 ? groups : 2048)), dim3(256), (FEW_LDS + 256 * ((a.r + 15) / 16)) * sizeof(float), s, a);
+            return hipGetLastError();
+        }
         if (p.tall) {
             u32x4* wf = static_cast<u32x4*>(ws);
             if constexpr (DX) return dense_tall<T, TALL_DX>(a, p, wf, s);
@@ -1012,17 +1142,23 @@ template <int T, bool DX> hipError_t dense_rows(const DenseRows& a, void* ws, hi
     return hipGetLastError();
 }
 
+constexpr long NARROW_ROWS = 4096;
+
 // The weight gradient's tile and how many pieces the rows are cut into (functions of the sizes alone)
-struct WeightsPlan { int width, tiles, splits; };
+struct WeightsPlan { int wo, wk, tiles, splits; };
 WeightsPlan weights_plan(int type, long n, int k, int o) {
     WeightsPlan p;
     const long t4 = (long)((k + 127) / 128) * ((o + 127) / 128), t8 = (long)((k + 255) / 256) * ((o + 255) / 256);
-    // 256 x 256 where that computes at most half as much again beyond the layer's edges and each of the 256 compute units has some steps to do; pieces of two steps at least
-    // (1 003 x 539 -> 512: 18 us; 25 in 256-wide tiles, 24 in pieces of one step)
     const long steps = type == LT_F32 ? (n + 31) / 32 : (n + 63) / 64;
-    p.width = 2 * 4 * t8 <= 3 * t4 && steps * t8 >= 4 * 256 ? 256 : 128;
-    p.tiles = (int)(p.width == 256 ? t8 : t4);
-    long s = (p.width == 256 ? 256 : 512) / p.tiles;      // one workgroup a compute unit, or two
+    // 256 x 256 where that computes at most half as much again beyond the layer's edges and each of the 256 compute units has some steps to do; pieces of two steps at least
+    // (1 003 x 539 -> 512: 18 us; 25 in 256-wide tiles, 24 in pieces of one step).  A side of at most 32 columns takes 32-wide tiles, where its rows are many.
+    p.wo = p.wk = 2 * 4 * t8 <= 3 * t4 && steps * t8 >= 4 * 256 ? 256 : 128;
+    if (p.wo == 128 && n >= NARROW_ROWS) {
+        if (o <= 32) p.wo = 32;
+        if (k <= 32) p.wk = 32;
+    }
+    p.tiles = (int)(((long)(k + p.wk - 1) / p.wk) * ((o + p.wo - 1) / p.wo));
+    long s = (p.wo == 256 ? 256 : p.wo == 128 && p.wk == 128 ? 512 : 1024) / p.tiles;      // one workgroup a compute unit, two, four
     if (s > steps / 2) s = steps / 2;
     p.splits = (int)(s < 1 ? 1 : s);
     return p;
@@ -1032,16 +1168,19 @@ WeightsPlan weights_plan(int type, long n, int k, int o) {
 template <int T> hipError_t dense_weights(const DenseWeights& a, const DenseRows* x, hipStream_t s) {
     const WeightsPlan p = weights_plan(T, a.n, a.k, a.o);
     const dim3 grid((unsigned)((p.splits + 7) / 8 * 8 * p.tiles));
-    if (x && p.width == 128) {
+    if (x && p.wo == 128 && p.wk == 128) {
         hipLaunchKernelGGL((k_dense_backward_few<T>), dim3(grid.x + few_blocks(*x)), dim3(256), 0, s, *x, a, grid.x);
-    } else if (x) {
-        hipLaunchKernelGGL((k_dense_few<T, true>), dim3(few_blocks(*x)), dim3(256), 0, s, *x);
-        hipLaunchKernelGGL((k_dense_weights<T, 256>), grid, dim3(1024), 0, s, a);
-    } else if (p.width == 256) hipLaunchKernelGGL((k_dense_weights<T, 256>), grid, dim3(1024), 0, s, a);
-    else hipLaunchKernelGGL((k_dense_weights<T, 128>), grid, dim3(256), 0, s, a);
+    } else {
+        if (x) hipLaunchKernelGGL((k_dense_few<T, true>), dim3(few_blocks(*x)), dim3(256), 0, s, *x);
+        if (p.wo == 256) hipLaunchKernelGGL((k_dense_weights<T, 256, 256>), grid, dim3(1024), 0, s, a);
+        else if (p.wo == 32 && p.wk == 32) hipLaunchKernelGGL((k_dense_weights<T, 32, 32>), grid, dim3(256), 0, s, a);
+        else if (p.wo == 32) hipLaunchKernelGGL((k_dense_weights<T, 32, 128>), grid, dim3(256), 0, s, a);
+        else if (p.wk == 32) hipLaunchKernelGGL((k_dense_weights<T, 128, 32>), grid, dim3(256), 0, s, a);
+        else hipLaunchKernelGGL((k_dense_weights<T, 128, 128>), grid, dim3(256), 0, s, a);
+    }
     if (a.splits > 1) {
         const long m = (long)a.o * a.k + a.o;
-        hipLaunchKernelGGL((k_dense_weights_sum<T>), dim3((unsigned)((m + 255) / 256)), dim3(256), 0, s, a);
+        hipLaunchKernelGGL((k_dense_weights_sum<T>), dim3((unsigned)((m + 63) / 64)), dim3(1024), 0, s, a);
     }
     return hipGetLastError();
 }

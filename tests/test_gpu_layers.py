@@ -152,6 +152,29 @@ def test_dense_many_rows(n, k, o, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,k,o", [(4096, 32, 32), (4095, 32, 32), (5003, 5, 26), (4100, 33, 3), (9001, 280, 5), (6007, 31, 177), (4099, 1, 33), (33100, 26, 18), (33000, 8, 1), (33000, 160, 8), (8229, 26, 500), (8200, 511, 31), (8193, 4, 7)])
+def test_dense_narrow_layers(n, k, o, dtype):
+    """many rows of a layer with at most 32 inputs or outputs, and its borders"""
+    g = gen(n + 3 * k + 5 * o)
+    x, w, b = randn(g, n, k, dtype=dtype), randn(g, o, k, dtype=dtype, scale=k ** -0.5), randn(g, o, dtype=dtype)
+    for relu in (True, False):
+        y, kept = L.dense_forward(x, w, b, relu=relu)
+        want = x.double() @ w.double().t() + b.double()
+        R.close(y, want.clamp_min(0) if relu else want, x.double().abs() @ w.double().abs().t() + b.double().abs(), k, dtype)
+        again = L.checkpoint(y, signed=not relu)                   # (held to the definition above)
+        assert torch.equal(kept.codes, again.codes) and torch.equal(kept.scales, again.scales)
+        alone, none = L.dense_forward(x, w, b, relu=relu, keep=False)
+        assert none is None and torch.equal(alone, y)
+        dy = randn(g, n, o, dtype=dtype)
+        kx = L.checkpoint(x)
+        dx, dw, db = L.dense_backward(torch.where(y > 0, dy, torch.full_like(dy, float("nan"))) if relu else dy, kx, w, relu=kept if relu else None)
+        dz, xv = (torch.where(y > 0, dy, torch.zeros_like(dy)) if relu else dy).double(), kx.values().double()
+        R.close(dx, dz @ w.double(), dz.abs() @ w.double().abs(), o, dtype)
+        R.close(dw, dz.t() @ xv, dz.abs().t() @ xv.abs(), n // 4, dtype)
+        R.close(db, dz.sum(0), dz.abs().sum(0), n // 4, dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_dense_long_reduction(dtype):
     """many rows: the pieces of the weight gradient and their sum; 70 001 rows, more than one launch tile of each kind"""
     g = gen(11)
