@@ -141,18 +141,27 @@ __global__ __launch_bounds__(1024) void k_sort_small(LookupGrad a, int passes, i
     for (int i = t; i < n; i += 1024) { keys[i] = lk[i]; pos[i] = lp[i]; }
 }
 
+template <class Key> __device__ __forceinline__ void count_tile(Key key, long n, int shift, int bits, unsigned* hist) {
+    const long i0 = (long)blockIdx.x * TILE + threadIdx.x;
+    unsigned k[TILE / 256];
+#pragma unroll
+    for (int q = 0; q < TILE / 256; ++q) k[q] = key(min(i0 + 256 * q, n - 1));
+#pragma unroll
+    for (int q = 0; q < TILE / 256; ++q)
+        if (i0 + 256 * q < n) atomicAdd(&hist[(k[q] >> shift) & ((1u << bits) - 1)], 1u);
+}
+
 // Large sort, one pass = three launches: digit counts of each tile, their exclusive sums along the tiles (one workgroup a digit), the scatter.
 // The first pass reads the caller's index; its counting launch also clears the gradient table (tokens that no row has keep zero).
 __global__ __launch_bounds__(256) void k_sort_count(LookupGrad a, const unsigned* keys, int shift, int bits, unsigned* counts, size_t zero_bytes) {
     __shared__ unsigned hist[BINS];
-    clear(a.dtable, zero_bytes, (size_t)blockIdx.x * 256 + threadIdx.x, (size_t)gridDim.x * 256);
     for (int i = threadIdx.x; i < BINS; i += 256) hist[i] = 0;
     __syncthreads();
-    const long i0 = (long)blockIdx.x * TILE;
-    for (int q = threadIdx.x; q < TILE; q += 256)
-        if (i0 + q < a.n) atomicAdd(&hist[((keys ? keys[i0 + q] : key_at(a, i0 + q)) >> shift) & ((1u << bits) - 1)], 1u);
+    if (keys) count_tile([&](long i) { return keys[i]; }, a.n, shift, bits, hist);
+    else count_tile([&](long i) { return key_at(a, i); }, a.n, shift, bits, hist);
     __syncthreads();
     for (int i = threadIdx.x; i < (1 << bits); i += 256) counts[(size_t)i * gridDim.x + blockIdx.x] = hist[i];
+    clear(a.dtable, zero_bytes, (size_t)blockIdx.x * 256 + threadIdx.x, (size_t)gridDim.x * 256);
 }
 
 __global__ __launch_bounds__(256) void k_sort_scan(unsigned* counts, int tiles, unsigned* totals) {
@@ -181,9 +190,35 @@ __global__ __launch_bounds__(256) void k_sort_scatter(LookupGrad a, const unsign
                                                       unsigned* keys_out, unsigned* pos_out) {
     __shared__ unsigned hist[4 * BINS];
     __shared__ unsigned base[BINS];
+    constexpr int Q = TILE / 256, B = BINS / 256;
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6, bins = 1 << bits;
+    const long i0 = (long)blockIdx.x * TILE + (long)wave * (TILE / 4);
+    // everything the tile needs is asked for at once: its keys and positions, its counts, the digits' totals
+    unsigned k[Q], p[Q], r[Q], before[B], total[B];
+    if (keys) {
+#pragma unroll
+        for (int q = 0; q < Q; ++q) {
+            const long i = min(i0 + 64 * q + lane, a.n - 1);
+            k[q] = keys[i];
+            p[q] = pos[i];
+        }
+    } else {
+#pragma unroll
+        for (int q = 0; q < Q; ++q) {
+            const long i = min(i0 + 64 * q + lane, a.n - 1);
+            k[q] = key_at(a, i);
+            p[q] = (unsigned)i;
+        }
+    }
+#pragma unroll
+    for (int q = 0; q < B; ++q) {
+        const int d = min(t + 256 * q, bins - 1);
+        before[q] = counts[(size_t)d * gridDim.x + blockIdx.x];
+        total[q] = totals[d];
+    }
     for (int i = t; i < 4 * BINS; i += 256) hist[i] = 0;
-    for (int i = t; i < BINS; i += 256) base[i] = i < bins ? totals[i] : 0;
+#pragma unroll
+    for (int q = 0; q < B; ++q) base[t + 256 * q] = t + 256 * q < bins ? total[q] : 0;
     __syncthreads();
     if (t < 64) {
         unsigned v[BINS / 64], s = 0;
@@ -196,23 +231,17 @@ __global__ __launch_bounds__(256) void k_sort_scatter(LookupGrad a, const unsign
 #pragma unroll
         for (int q = 0; q < BINS / 64; ++q) { base[t * (BINS / 64) + q] = x; x += v[q]; }
     }
-    constexpr int Q = TILE / 256;
-    const long i0 = (long)blockIdx.x * TILE + (long)wave * (TILE / 4);
-    unsigned k[Q], p[Q], r[Q];
-#pragma unroll
-    for (int q = 0; q < Q; ++q) {
-        const long i = i0 + 64 * q + lane;
-        const bool in = i < a.n;
-        k[q] = in ? (keys ? keys[i] : key_at(a, i)) : 0;
-        p[q] = in ? (pos ? pos[i] : (unsigned)i) : 0;
-    }
 #pragma unroll
     for (int q = 0; q < Q; ++q) r[q] = rank_in_wave<4>((k[q] >> shift) & (bins - 1), i0 + 64 * q + lane < a.n, hist, wave, lane);
     __syncthreads();
-    for (int i = t; i < bins; i += 256) {
-        unsigned s = base[i] + counts[(size_t)i * gridDim.x + blockIdx.x];
 #pragma unroll
-        for (int w = 0; w < 4; ++w) { const unsigned h = hist[w * BINS + i]; hist[w * BINS + i] = s; s += h; }
+    for (int q = 0; q < B; ++q) {
+        const int i = t + 256 * q;
+        if (i < bins) {
+            unsigned s = base[i] + before[q];
+#pragma unroll
+            for (int w = 0; w < 4; ++w) { const unsigned h = hist[w * BINS + i]; hist[w * BINS + i] = s; s += h; }
+        }
     }
     __syncthreads();
 #pragma unroll
@@ -294,7 +323,7 @@ template <int T> __device__ __forceinline__ void put_one(const LookupGrad& a, un
 }
 template <int T> __global__ __launch_bounds__(256) void k_lookup_join(LookupGrad a, const unsigned* keys, long pieces, int len, const float* part) {
     constexpr long SHORT = 16;
-    __shared__ float sums[256];
+    __shared__ f32x4 sums[256];
     __shared__ unsigned token[4];
     __shared__ int goes_on[4];      // pieces that the run comes into, where it is a long one
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), w = 8 * ((a.d + 7) >> 3);
@@ -328,61 +357,176 @@ template <int T> __global__ __launch_bounds__(256) void k_lookup_join(LookupGrad
         const int n = goes_on[y];
         if (n == 0) continue;
         const float* from = part + (size_t)((long)blockIdx.x * 4 + y) * 2 * w;
-        for (int c0 = 0; c0 < a.d; c0 += 256) {
-            const int cols = a.d - c0 < 256 ? a.d - c0 : 256, g = 256 / cols, c = t % cols, z = t / cols;
-            float s = 0.0f;
+        const int quads = w >> 2;
+        for (int q0 = 0; q0 < quads; q0 += 256) {
+            const int cols = quads - q0 < 256 ? quads - q0 : 256, g = 256 / cols, c = t % cols, z = t / cols;
+            f32x4 s = {0.f, 0.f, 0.f, 0.f};
             if (z < g) {
-                if (z == 0) s = from[w + c0 + c];
-                const float* p = from + 2 * w + c0 + c;
-#pragma unroll 4
-                for (int q = z; q < n; q += g) s += p[(size_t)q * 2 * w];
+                if (z == 0) s = *reinterpret_cast<const f32x4*>(from + w + 4 * (q0 + c));
+                const float* p = from + 2 * w + 4 * (q0 + c);
+#pragma unroll 8
+                for (int q = z; q < n; q += g) s += *reinterpret_cast<const f32x4*>(p + (size_t)q * 2 * w);
             }
             sums[t] = s;
             __syncthreads();
             if (t < cols) {
-                float r = 0.0f;
-                for (int q = 0; q < g; ++q) r += sums[q * cols + t];
-                put_one<T>(a, token[y], c0 + t, r);
+                f32x4 r = sums[t];
+                for (int q = 1; q < g; ++q) r += sums[q * cols + t];
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (4 * (q0 + t) + e < a.d) put_one<T>(a, token[y], 4 * (q0 + t) + e, r[e]);
             }
             __syncthreads();
         }
     }
 }
 
-// Few positions (at most 4 096 sorted by one workgroup, at most 8 192 rows, a table of at most 4 096 tokens): one workgroup a token, which finds its rows by two 64-way searches of
-// the sorted keys and writes its gradient, zeros too — no pieces, no clearing, one launch behind the sort.
-__device__ __forceinline__ int below(const unsigned* keys, int n, unsigned token, int lane) {      // positions whose key is less than `token`
-    const int some = __popcll(__ballot(64 * lane < n && keys[min(64 * lane, n - 1)] < token));
-    if (some == 0) return 0;
-    const int i = 64 * (some - 1) + lane;
-    return 64 * (some - 1) + __popcll(__ballot(i < n && keys[min(i, n - 1)] < token));
+// Few positions, no sort: a workgroup takes a range of tokens, reads every key and keeps the positions of its tokens, in order; one launch writes the whole table, zeros too.  A range
+// of one token is summed by the whole workgroup, and so is a token with many rows in a longer range; the other tokens of that are a wave's work each (where positions
+// are fewer than tokens, found by their first position).
+constexpr int MANY = 256;      // rows
+constexpr long FEW_SHARE = 32768;      // elements of dOut a token
+struct FewLds {
+    unsigned short pos[SMALL], tok[SMALL];
+    unsigned short mine[16][64];
+    unsigned many[SMALL * 2 / MANY];
+    int wave[16], n_many;
+    float sums[1024 * 8];
+};
+__device__ __forceinline__ int few_collect(const LookupGrad& a, unsigned t0, unsigned tokens, FewLds& l) {
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, n = (int)a.n;
+    unsigned k[4];
+    int at[4], count = 0;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) k[q] = key_at(a, min(256 * wave + 64 * q + lane, n - 1));
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        const bool in = 256 * wave + 64 * q + lane < n && k[q] - t0 < tokens && k[q] < (unsigned)a.v;
+        const unsigned long long m = __ballot(in);
+        at[q] = in ? count + __popcll(m & ((1ull << lane) - 1)) : -1;
+        count += __popcll(m);
+    }
+    if (lane == 0) l.wave[wave] = count;
+    __syncthreads();
+    int before = 0, all = 0;
+#pragma unroll
+    for (int w = 0; w < 16; ++w) { if (w < wave) before += l.wave[w]; all += l.wave[w]; }
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+        if (at[q] >= 0) {
+            l.pos[before + at[q]] = (unsigned short)(256 * wave + 64 * q + lane);
+            l.tok[before + at[q]] = (unsigned short)(k[q] - t0);
+        }
+    __syncthreads();
+    return all;
 }
-template <int T> __global__ __launch_bounds__(256) void k_lookup_token(LookupGrad a, const unsigned* keys, const unsigned* pos) {
-    __shared__ float sums[256 * 8];
-    const int t = threadIdx.x, lane = t & 63, n = (int)a.n, per = (int)a.per, cpr = (a.d + 7) >> 3;
-    const unsigned token = blockIdx.x;
-    const int first = below(keys, n, token, lane) * per, last = below(keys, n, token + 1, lane) * per;
-    for (int c0 = 0; c0 < cpr; c0 += 256) {
-        const int chunks = cpr - c0 < 256 ? cpr - c0 : 256, g = 256 / chunks, y = t / chunks, c = 8 * (c0 + t % chunks);
-        float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        if (y < g)
-#pragma unroll 4
-            for (int i = first + y; i < last; i += g) {
-                const int e = i / per;
+// rows first, first + step, ... below `rows` of the positions in `pos`, 8 columns from c on
+template <int T> __device__ __forceinline__ void few_rows(const LookupGrad& a, const unsigned short* pos, int rows, int first, int step, int c, float (&s)[8]) {
+    constexpr int U = 8;
+    const int per = (int)a.per;
+    for (int i0 = first; i0 < rows; i0 += U * step) {
+        Raw8<T> v[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int i = min(i0 + u * step, rows - 1), e = i / per;
+            v[u] = load8<T>(static_cast<const char*>(a.dout) + ((long)pos[e] * per + (i - e * per)) * a.ld_dout * Bytes<T>::v, c, a.d);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (i0 + u * step < rows) {
                 float f[8];
-                to_floats<T>(load8<T>(static_cast<const char*>(a.dout) + ((long)pos[e] * per + (i - e * per)) * a.ld_dout * Bytes<T>::v, c, a.d), f);
+                to_floats<T>(v[u], f);
 #pragma unroll
                 for (int x = 0; x < 8; ++x) s[x] += f[x];
             }
+    }
+}
+// one token, all its `m` positions in the list: thread = 8 columns of every g-th row; the g sums meet in two steps
+template <int T> __device__ __forceinline__ void few_whole(const LookupGrad& a, unsigned token, int m, FewLds& l) {
+    const int t = threadIdx.x, cpr = (a.d + 7) >> 3, rows = m * (int)a.per;
+    for (int c0 = 0; c0 < cpr; c0 += 128) {
+        const int chunks = min(cpr - c0, 128), cols = 8 * chunks, g = min(1024 / chunks, max(rows, 1)), parts = min(min(1024 / cols, 32), g), y = t / chunks, c = 8 * (c0 + t % chunks);
+        float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        if (y < g) {
+            few_rows<T>(a, l.pos, rows, y, g, c, s);
 #pragma unroll
-        for (int x = 0; x < 8; ++x) sums[8 * t + x] = s[x];
-        __syncthreads();
-        for (int z = t; z < 8 * chunks; z += 256) {
-            float r = 0.0f;
-            for (int q = 0; q < g; ++q) r += sums[q * 8 * chunks + z];
-            if (8 * c0 + z < a.d) put_one<T>(a, token, 8 * c0 + z, r);
+            for (int x = 0; x < 8; ++x) l.sums[8 * t + x] = s[x];
         }
         __syncthreads();
+        const int part = t / cols, col = t % cols;
+        float r = 0.0f;
+        if (part < parts)
+            for (int q = part; q < g; q += parts) r += l.sums[q * cols + col];
+        __syncthreads();
+        l.sums[t] = r;
+        __syncthreads();
+        if (t < cols && 8 * c0 + t < a.d) {
+            for (int q = 1; q < parts; ++q) r += l.sums[q * cols + t];
+            put_one<T>(a, token, 8 * c0 + t, r);
+        }
+        __syncthreads();
+    }
+}
+template <int T> __global__ __launch_bounds__(1024) void k_lookup_few(LookupGrad a, unsigned range) {
+    __shared__ FewLds l;
+    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), cpr = (a.d + 7) >> 3, per = (int)a.per;
+    const unsigned t0 = blockIdx.x * range;
+    if (t == 0) l.n_many = 0;
+    const int m = few_collect(a, t0, range, l);
+    if (range == 1) {
+        few_whole<T>(a, t0, m, l);
+        return;
+    }
+    const size_t own = (size_t)min((unsigned)a.v - t0, range) * a.d * Bytes<T>::v;
+    clear(static_cast<char*>(a.dtable) + (size_t)t0 * a.d * Bytes<T>::v, own, t, 1024);
+    __syncthreads();
+    float* sums = l.sums + 512 * wave;
+    const bool by_token = m >= (int)range;      // (else by position, at a token's first)
+    for (int x = wave; x < (by_token ? (int)range : m); x += 16) {
+        const unsigned tl = by_token ? (unsigned)x : (unsigned)__builtin_amdgcn_readfirstlane((int)l.tok[x]);
+        const int first = by_token ? 0 : x;
+        int count = 0;
+        bool earlier = false;
+        for (int j = 0; j < m && !earlier; j += 64) {
+            const unsigned long long mask = __ballot(j + lane < m && l.tok[min(j + lane, m - 1)] == tl);
+            earlier = mask != 0 && count == 0 && j + (int)__builtin_ctzll(mask) < first;
+            count += __popcll(mask);
+        }
+        if (earlier || count == 0) continue;
+        if (count * per > MANY) {
+            if (lane == 0) l.many[atomicAdd(&l.n_many, 1)] = tl;      // (their order does not matter: each is a sum of its own)
+            continue;
+        }
+        for (int c0 = 0; c0 < cpr; c0 += 64) {
+            const int chunks = min(cpr - c0, 64), g = 64 / chunks, y = lane / chunks, c = 8 * (c0 + lane % chunks);
+            float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+            for (int j = first & ~63; j < m; j += 64) {
+                const bool in = j + lane < m && l.tok[min(j + lane, m - 1)] == tl;
+                const unsigned long long mask = __ballot(in);
+                if (mask == 0) continue;
+                __builtin_amdgcn_wave_barrier();
+                if (in) l.mine[wave][__popcll(mask & ((1ull << lane) - 1))] = l.pos[j + lane];
+                __builtin_amdgcn_wave_barrier();
+                if (y < g) few_rows<T>(a, l.mine[wave], (int)__popcll(mask) * per, y, g, c, s);
+            }
+            __builtin_amdgcn_wave_barrier();
+            if (y < g)
+#pragma unroll
+                for (int x = 0; x < 8; ++x) sums[8 * lane + x] = s[x];
+            __builtin_amdgcn_wave_barrier();
+            for (int z = lane; z < 8 * chunks; z += 64) {
+                float r = sums[z];
+                for (int q = 1; q < g; ++q) r += sums[q * 8 * chunks + z];
+                if (8 * c0 + z < a.d) put_one<T>(a, t0 + tl, 8 * c0 + z, r);
+            }
+        }
+    }
+    __syncthreads();
+    const int many = l.n_many;
+    for (int i = 0; i < many; ++i) {
+        const unsigned token = t0 + l.many[i];
+        __syncthreads();
+        few_whole<T>(a, token, few_collect(a, token, 1, l), l);
     }
 }
 
@@ -426,9 +570,12 @@ template <int T> hipError_t lookup_backward(const LookupGrad& a, hipStream_t s) 
     char* ws = static_cast<char*>(a.ws);
     auto u = [&](size_t at) { return reinterpret_cast<unsigned*>(ws + at); };
     const size_t zero = (size_t)a.v * a.d * Bytes<T>::v;
-    if (a.n > 0 && p.tiles == 0 && p.rows <= 8192 && a.v <= 4096) {
-        hipLaunchKernelGGL(k_sort_small, dim3(1), dim3(1024), 0, s, a, p.passes, p.bits, u(p.keys), u(p.pos), (size_t)0);
-        hipLaunchKernelGGL((k_lookup_token<T>), dim3((unsigned)a.v), dim3(256), 0, s, a, u(p.keys), u(p.pos));
+    // (a token's rows are one workgroup's work: not where few tokens share much)
+    if (a.n > 0 && p.tiles == 0 && p.rows <= 2 * SMALL && a.v <= 131072 && p.rows * a.d <= FEW_SHARE * a.v) {
+        // one workgroup a compute unit where positions are few, shorter ranges where one could gather many
+        const long groups = a.n < 1024 ? 256 : 1024;
+        const unsigned range = (unsigned)((a.v + groups - 1) / groups);
+        hipLaunchKernelGGL((k_lookup_few<T>), dim3((unsigned)((a.v + range - 1) / range)), dim3(1024), 0, s, a, range);
         return hipGetLastError();
     }
     if (a.n == 0 || p.tiles == 0) {

@@ -342,6 +342,25 @@ def test_lookup_gradient_of_one_token(n, per):
     assert torch.equal(got.double(), want)                  # whole numbers below 2^24
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,per,v,d", [(4096, 1, 1024, 24), (4096, 2, 1025, 24), (4095, 1, 5003, 3), (64, 128, 131072, 9), (64, 128, 131073, 9), (7, 1, 100000, 300), (1, 1, 2049, 1030),
+                                       (2000, 4, 1500, 70), (4096, 1, 3, 2), (4096, 2, 1, 256), (90, 91, 2, 33), (5000, 1, 40, 2056)])
+def test_lookup_gradient_of_clustered_tokens(n, per, v, d, dtype):
+    """most positions on few tokens that lie side by side (one workgroup's range), one of them with half of all: whole numbers, so that every sum is exact"""
+    g = gen(n + per + v + d)
+    index = torch.randint(0, min(v, 40), (n,), generator=g)
+    index[torch.rand(n, generator=g) < 0.5] = min(v - 1, 17)
+    index[torch.rand(n, generator=g) < 0.05] = v - 1
+    index[torch.rand(n, generator=g) < 0.05] = -1
+    index = index.to(DEV)
+    dout = torch.randint(-2, 3, (n * per, d), generator=g).to(DEV)
+    rows = index.repeat_interleave(per)
+    want = torch.zeros((v, d), dtype=torch.float64, device=DEV).index_add_(0, rows.clamp_min(0), torch.where(rows[:, None] >= 0, dout, torch.zeros_like(dout)).double())
+    assert float(want.abs().max()) < 2 ** 24
+    got = L.lookup_backward(dout.to(dtype), index, v, rows_per_index=per)
+    assert torch.equal(got, want.to(dtype))                  # (float64 holds the sums, and one rounding is what the operator does)
+
+
 def test_lookup_indices_outside_the_table():
     table = randn(gen(32), 6, 10)
     index = torch.tensor([0, -1, 6, 5, -(1 << 40), 1 << 40, 2], device=DEV)
