@@ -535,11 +535,12 @@ __global__ __launch_bounds__(256) void k_clear(void* table, size_t bytes) { clea
 struct Plan {
     long rows, pieces;
     int len, passes, bits, tiles;
+    bool few;
     size_t keys, pos, keys2, pos2, counts, totals, part, bytes;      // offsets into the workspace
 };
 
 Plan plan(long n, long per, long v, int d) {
-    Plan p;
+    Plan p{};
     p.rows = n * per;
     // pieces: enough threads (a thread = 8 columns of a piece) to fill the chip's 256 x 4 SIMDs a few waves deep; 16 rows at least, so that partial sums stay few
     const long cpr = (d + 7) / 8;
@@ -552,6 +553,12 @@ Plan plan(long n, long per, long v, int d) {
     p.passes = (all + 8) / 9;
     p.bits = (all + p.passes - 1) / p.passes;
     p.tiles = n > SMALL ? (int)((n + TILE - 1) / TILE) : 0;
+    // (a token's rows are one workgroup's work there: not where few tokens share much)
+    p.few = n > 0 && p.tiles == 0 && p.rows <= 2 * SMALL && v <= 131072 && p.rows * d <= FEW_SHARE * v;
+    if (p.few || n == 0) {
+        p.bytes = 0;
+        return p;
+    }
     size_t at = 0;
     auto take = [&](size_t bytes) { const size_t was = at; at += (bytes + 255) & ~(size_t)255; return was; };
     p.keys = take((size_t)n * 4);
@@ -570,8 +577,7 @@ template <int T> hipError_t lookup_backward(const LookupGrad& a, hipStream_t s) 
     char* ws = static_cast<char*>(a.ws);
     auto u = [&](size_t at) { return reinterpret_cast<unsigned*>(ws + at); };
     const size_t zero = (size_t)a.v * a.d * Bytes<T>::v;
-    // (a token's rows are one workgroup's work: not where few tokens share much)
-    if (a.n > 0 && p.tiles == 0 && p.rows <= 2 * SMALL && a.v <= 131072 && p.rows * a.d <= FEW_SHARE * a.v) {
+    if (p.few) {
         // one workgroup a compute unit where positions are few, shorter ranges where one could gather many
         const long groups = a.n < 1024 ? 256 : 1024;
         const unsigned range = (unsigned)((a.v + groups - 1) / groups);

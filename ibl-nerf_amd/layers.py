@@ -63,9 +63,9 @@ def _rows(t, what):
     return t, (t.stride(0) if t.shape[0] > 1 else k)
 
 
-def _workspace(size, device):
+def _workspace(size, like):
     """Scratch memory of one call from torch's allocator: reused in stream order, a captured graph's from the graph's own pool."""
-    return (torch.empty((size,), dtype=torch.uint8, device=device), size) if size else (None, 0)
+    return (like.new_empty((size,), dtype=torch.uint8), size) if size else (None, 0)
 
 
 def _address(t):
@@ -93,7 +93,7 @@ class Checkpoint:
 
     def values(self, dtype=torch.float32):
         """The values the checkpoint stands for, [n, columns]: exact in float32 and bfloat16 (at most 8 significant bits)."""
-        out = torch.empty((self.rows, self.columns), dtype=dtype, device=self.codes.device)
+        out = self.codes.new_empty((self.codes.shape[0], self.columns), dtype=dtype)
         t = _type(out, "the values")
         lib, stream, guard = _on(out)
         with guard:
@@ -110,7 +110,7 @@ def _made(codes, scales, columns, signed):
 
 def _codes_like(x, n, columns):
     blocks = (columns + 31) // 32
-    return torch.empty((n, 32 * blocks), dtype=torch.uint8, device=x.device), torch.empty((n, blocks), dtype=torch.uint8, device=x.device)
+    return x.new_empty((n, 32 * blocks), dtype=torch.uint8), x.new_empty((n, blocks), dtype=torch.uint8)
 
 
 def checkpoint(x, signed=True):
@@ -149,9 +149,9 @@ def dense_forward(x, weight, bias=None, relu=False, keep=True):
             raise ValueError("the bias of a layer of %d outputs is [%d], got %s" % (o, o, tuple(bias.shape)))
         _same(bias, x, "bias", x.dtype)
         bias = bias.contiguous()
-    y = torch.empty((n, o), dtype=x.dtype, device=x.device)
+    y = x.new_empty((n, o))
     codes, scales = _codes_like(x, n, o) if keep else (None, None)
-    ws, ws_bytes = _workspace(lib.iblnerf_dense_forward_workspace(t, n, k, o), x.device)
+    ws, ws_bytes = _workspace(lib.iblnerf_dense_forward_workspace(t, n, k, o), x)
     with guard:
         B.check_layers(lib.iblnerf_dense_forward(stream, t, x.data_ptr(), ld, n, k, w.data_ptr(), ldw, o, _address(bias), int(bool(relu)), y.data_ptr(), o, _address(codes), _address(scales),
                                                  _address(ws), ws_bytes))
@@ -180,11 +180,10 @@ def dense_backward(dy, x, weight, relu=None, need_dx=True, need_dw=True, need_db
     grad_dtype = grad_dtype or dy.dtype
     if grad_dtype not in (dy.dtype, torch.float32):
         raise TypeError("the parameters' gradients are %s or float32, not %s" % (dy.dtype, grad_dtype))
-    dev = dy.device
-    dx = torch.empty((n, k), dtype=dy.dtype, device=dev) if need_dx else None
-    dw = torch.empty((o, k), dtype=grad_dtype, device=dev) if need_dw or need_db else None
-    db = torch.empty((o,), dtype=grad_dtype, device=dev) if need_db else None
-    ws, ws_bytes = _workspace(lib.iblnerf_dense_backward_workspace(t, n, k, o), dev)
+    dx = dy.new_empty((n, k)) if need_dx else None
+    dw = dy.new_empty((o, k), dtype=grad_dtype) if need_dw or need_db else None
+    db = dy.new_empty((o,), dtype=grad_dtype) if need_db else None
+    ws, ws_bytes = _workspace(lib.iblnerf_dense_backward_workspace(t, n, k, o), dy)
     with guard:
         B.check_layers(lib.iblnerf_dense_backward(stream, t, dy.data_ptr(), ld, n, k, o, x.codes.data_ptr(), x.scales.data_ptr(), int(x.signed),
                                                   None if relu is None else relu.codes.data_ptr(), w.data_ptr(), ldw, _address(dx), k, _TYPES[grad_dtype], _address(dw), _address(db),
@@ -268,7 +267,7 @@ def _lookup(table, index, scale, rows_per_index, out):
         raise ValueError("rows_per_index must be at least 1, got %d" % per)
     shape = tuple(index.shape[:-1]) + (index.shape[-1] * per, d) if index.dim() else (per, d)
     if out is None:
-        out = torch.empty(shape, dtype=table.dtype, device=table.device)
+        out = table.new_empty(shape)
     else:
         _same(out, table, "out", table.dtype)
         if out.dim() != 2 or tuple(out.shape) != (n * per, d) or (d > 1 and out.stride(1) != 1) or (out.shape[0] > 1 and not d <= out.stride(0) <= MAX_STRIDE):
@@ -289,10 +288,10 @@ def lookup_backward(dout, index, v, scale=1.0, rows_per_index=1):
     n, per, d = idx.numel(), int(rows_per_index), dout.shape[1]
     if per < 1 or int(v) < 1 or n * per != dout.shape[0]:
         raise ValueError("%d indices with %d rows each over a table of %d rows do not fit %d gradient rows" % (n, per, int(v), dout.shape[0]))
-    grad = torch.empty((int(v), d), dtype=dout.dtype, device=dout.device)
-    ws = torch.empty((lib.iblnerf_lookup_backward_workspace(n, per, int(v), d),), dtype=torch.uint8, device=dout.device)
+    grad = dout.new_empty((int(v), d))
+    ws, ws_bytes = _workspace(lib.iblnerf_lookup_backward_workspace(n, per, int(v), d), dout)
     with guard:
-        B.check_layers(lib.iblnerf_lookup_backward(stream, t, dout.data_ptr(), ld, idx.data_ptr(), bits, n, per, int(v), d, float(scale), grad.data_ptr(), ws.data_ptr(), ws.numel()))
+        B.check_layers(lib.iblnerf_lookup_backward(stream, t, dout.data_ptr(), ld, idx.data_ptr(), bits, n, per, int(v), d, float(scale), grad.data_ptr(), _address(ws), ws_bytes))
     return grad
 
 
