@@ -344,7 +344,7 @@ def test_lookup_gradient_of_one_token(n, per):
 
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("n,per,v,d", [(4096, 1, 1024, 24), (4096, 2, 1025, 24), (4095, 1, 5003, 3), (64, 128, 131072, 9), (64, 128, 131073, 9), (7, 1, 100000, 300), (1, 1, 2049, 1030),
-                                       (2000, 4, 1500, 70), (4096, 1, 3, 2), (4096, 2, 1, 256), (90, 91, 2, 33), (5000, 1, 40, 2056)])
+                                       (2000, 4, 1500, 70), (4096, 1, 3, 2), (4096, 2, 1, 256), (90, 91, 2, 33), (5000, 1, 40, 2056), (16384, 1, 257, 5), (16384, 4, 70000, 31), (16385, 1, 300, 5), (341, 192, 3000, 20)])
 def test_lookup_gradient_of_clustered_tokens(n, per, v, d, dtype):
     """most positions on few tokens that lie side by side (one workgroup's range), one of them with half of all: whole numbers, so that every sum is exact"""
     g = gen(n + per + v + d)

@@ -86,6 +86,6 @@ def test_c_lookup_refuses(lib):
         refused(lib, lib.iblnerf_lookup(None, a["dtype"], a["tab"], a["ld"], a["v"], a["d"], a["idx"], a["bits"], a["n"], a["per"], 1.0, a["out"], a["ldo"]), "lookup")
         if not set(bad) & {"ld"}:
             refused(lib, lib.iblnerf_lookup_backward(None, a["dtype"], a["out"], a["ldo"], a["idx"], a["bits"], a["n"], a["per"], a["v"], a["d"], 1.0, a["tab"], P, 1 << 40), "lookup_backward")
-    need = lib.iblnerf_lookup_backward_workspace(5000, 2, 10, 8)          # (few positions need none)
-    assert need > 0 and lib.iblnerf_lookup_backward_workspace(5000, 0, 10, 8) == 0 and lib.iblnerf_lookup_backward_workspace(4, 2, 10, 8) == 0
-    refused(lib, lib.iblnerf_lookup_backward(None, 0, P, 8, P, 64, 5000, 2, 10, 8, 1.0, P, P, need - 1), "workspace")
+    need = lib.iblnerf_lookup_backward_workspace(20000, 2, 10, 8)          # (few positions need none)
+    assert need > 0 and lib.iblnerf_lookup_backward_workspace(20000, 0, 10, 8) == 0 and lib.iblnerf_lookup_backward_workspace(4, 2, 10, 8) == 0
+    refused(lib, lib.iblnerf_lookup_backward(None, 0, P, 8, P, 64, 20000, 2, 10, 8, 1.0, P, P, need - 1), "workspace")
