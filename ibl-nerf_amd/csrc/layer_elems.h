@@ -66,6 +66,14 @@ template <int T> __device__ __forceinline__ Raw8<T> load8(const char* row, int c
     return v;
 }
 
+// eight columns from c on, all of them there (straight code)
+template <int T> __device__ __forceinline__ Raw8<T> load8_whole(const char* row, int c) {
+    Raw8<T> v;
+    v.q[0] = load16(row + (size_t)c * Bytes<T>::v);
+    if constexpr (T == LT_F32) v.q[1] = load16(row + (size_t)c * 4 + 16);
+    return v;
+}
+
 // the elements whose code byte is zero become zero (a select: what stands in a closed place, a NaN too, is gone)
 template <int T> __device__ __forceinline__ void close8(Raw8<T>& v, u32x2 codes) {
 #pragma unroll

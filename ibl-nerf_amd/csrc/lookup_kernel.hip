@@ -261,15 +261,23 @@ template <int T> __device__ __forceinline__ void put_sum(const LookupGrad& a, un
     store8<T>(static_cast<char*>(a.dtable) + (size_t)token * a.d * Bytes<T>::v, c, a.d, from_floats<T>(f));
 }
 
+// Where a thread's 8 columns begin: in rows of 8 and more the last chunk moves back to end with the row, so that every chunk is whole — two neighbours then hold some columns'
+// sums twice, the same bits — and loads need no branch.  WIDE: such rows.
+template <bool WIDE> __device__ __forceinline__ int chunk_at(int chunk, int d) { return WIDE ? min(8 * chunk, d - 8) : 8 * chunk; }
+template <int T, bool WIDE> __device__ __forceinline__ Raw8<T> load_chunk(const char* row, int c, int d) {
+    if constexpr (WIDE) return load8_whole<T>(row, c);
+    else return load8<T>(row, c, d);
+}
+
 // A thread = 8 columns of one piece: sorted rows [piece * len, piece * len + len), sorted row i = row i % per of the entry i / per.  part [pieces][2][8 cpr]: the sum of the
 // run that comes in from the piece before (0) and of the run that goes on into the next (1).
-template <int T> __global__ __launch_bounds__(256) void k_lookup_sum(LookupGrad a, const unsigned* keys, const unsigned* pos, long pieces, int len, float* part) {
+template <int T, bool WIDE> __global__ __launch_bounds__(256) void k_lookup_sum(LookupGrad a, const unsigned* keys, const unsigned* pos, long pieces, int len, float* part) {
     constexpr int U = 8;      // rows in flight
     const int cpr = (a.d + 7) >> 3;
     const long id = (long)blockIdx.x * 256 + threadIdx.x;
     const long piece = id / cpr;
     if (piece >= pieces) return;
-    const int c = 8 * (int)(id - piece * cpr);
+    const int c = chunk_at<WIDE>((int)(id - piece * cpr), a.d);
     const long rows = a.n * a.per, i0 = piece * len, i1 = i0 + len < rows ? i0 + len : rows;
     const unsigned none = (unsigned)a.v;
     float* out = part + (size_t)piece * 2 * 8 * cpr + c;
@@ -282,18 +290,21 @@ template <int T> __global__ __launch_bounds__(256) void k_lookup_sum(LookupGrad 
     float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     for (long i = i0; i < i1; i += U) {
         unsigned k[U];
+        long at[U];
         Raw8<T> v[U];
         long e = i / a.per, q = i - e * a.per;
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const bool in = i + u < i1;
-            k[u] = in ? keys[e] : none;
-            v[u] = in && k[u] != none ? load8<T>(static_cast<const char*>(a.dout) + ((long)pos[e] * a.per + q) * a.ld_dout * Bytes<T>::v, c, a.d) : zero8<T>();
-            if (++q == a.per) { q = 0; ++e; }
+        for (int u = 0; u < U; ++u) {      // (rows beyond the piece: its last again)
+            k[u] = keys[e];
+            at[u] = (long)pos[e] * a.per + q;
+            if (i + u + 1 < i1 && ++q == a.per) { q = 0; ++e; }
         }
 #pragma unroll
+        for (int u = 0; u < U; ++u) v[u] = load_chunk<T, WIDE>(static_cast<const char*>(a.dout) + at[u] * a.ld_dout * Bytes<T>::v, c, a.d);
+#pragma unroll
         for (int u = 0; u < U; ++u) {
-            if (i + u < i1 && k[u] != cur) {
+            if (i + u >= i1) break;
+            if (k[u] != cur) {
                 if (coming) keep(0, s);
                 else if (cur != none) put_sum<T>(a, cur, c, s);
                 coming = false;
@@ -433,7 +444,7 @@ __device__ __forceinline__ int few_collect(const LookupGrad& a, unsigned t0, int
     return total;
 }
 // rows first, first + step, ... below `rows` of the positions in `pos`, 8 columns from c on
-template <int T> __device__ __forceinline__ void few_rows(const LookupGrad& a, const unsigned short* pos, int rows, int first, int step, int c, float (&s)[8]) {
+template <int T, bool WIDE> __device__ __forceinline__ void few_rows(const LookupGrad& a, const unsigned short* pos, int rows, int first, int step, int c, float (&s)[8]) {
     constexpr int U = 8;
     const int per = (int)a.per;
     for (int i0 = first; i0 < rows; i0 += U * step) {
@@ -441,7 +452,7 @@ template <int T> __device__ __forceinline__ void few_rows(const LookupGrad& a, c
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int i = min(i0 + u * step, rows - 1), e = i / per;
-            v[u] = load8<T>(static_cast<const char*>(a.dout) + ((long)pos[e] * per + (i - e * per)) * a.ld_dout * Bytes<T>::v, c, a.d);
+            v[u] = load_chunk<T, WIDE>(static_cast<const char*>(a.dout) + ((long)pos[e] * per + (i - e * per)) * a.ld_dout * Bytes<T>::v, c, a.d);
         }
 #pragma unroll
         for (int u = 0; u < U; ++u)
@@ -454,15 +465,16 @@ template <int T> __device__ __forceinline__ void few_rows(const LookupGrad& a, c
     }
 }
 // one token, all its `m` positions in the list: thread = 8 columns of every g-th row; the g sums meet in two steps
-template <int T> __device__ __forceinline__ void few_whole(const LookupGrad& a, unsigned token, int m, FewLds& l) {
+template <int T, bool WIDE> __device__ __forceinline__ void few_whole(const LookupGrad& a, unsigned token, int m, FewLds& l) {
     const int t = threadIdx.x, cpr = (a.d + 7) >> 3, rows = m * (int)a.per;
     for (int c0 = 0; c0 < cpr; c0 += 128) {
-        const int chunks = min(cpr - c0, 128), cols = 8 * chunks, g = min(1024 / chunks, max(rows, 1)), parts = min(min(1024 / cols, 32), g), y = t / chunks, c = 8 * (c0 + t % chunks);
+        const int chunks = min(cpr - c0, 128), cols = 8 * chunks, g = min(1024 / chunks, max(rows, 1)), parts = min(min(1024 / cols, 32), g), y = t / chunks, c = chunk_at<WIDE>(c0 + t % chunks, a.d);
         float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
         if (y < g) {
-            few_rows<T>(a, l.pos, rows, y, g, c, s);
+            few_rows<T, WIDE>(a, l.pos, rows, y, g, c, s);
 #pragma unroll
-            for (int x = 0; x < 8; ++x) l.sums[8 * t + x] = s[x];
+            for (int x = 0; x < 8; ++x)
+                if (c + x >= 8 * c0) l.sums[y * cols + c - 8 * c0 + x] = s[x];
         }
         __syncthreads();
         const int part = t / cols, col = t % cols;
@@ -479,14 +491,14 @@ template <int T> __device__ __forceinline__ void few_whole(const LookupGrad& a, 
         __syncthreads();
     }
 }
-template <int T> __global__ __launch_bounds__(1024) void k_lookup_few(LookupGrad a, int bits) {
+template <int T, bool WIDE> __global__ __launch_bounds__(1024) void k_lookup_few(LookupGrad a, int bits) {
     __shared__ FewLds l;
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), cpr = (a.d + 7) >> 3, per = (int)a.per;
     const unsigned t0 = blockIdx.x;
     if (t == 0) l.n_many = 0;
     const int m = few_collect(a, t0, bits, l);
     if (bits == 32) {
-        few_whole<T>(a, t0, m, l);
+        few_whole<T, WIDE>(a, t0, m, l);
         return;
     }
     const int tokens = (int)(((unsigned)a.v - t0 + (1u << bits) - 1) >> bits);
@@ -513,7 +525,7 @@ template <int T> __global__ __launch_bounds__(1024) void k_lookup_few(LookupGrad
             continue;
         }
         for (int c0 = 0; c0 < cpr; c0 += 64) {
-            const int chunks = min(cpr - c0, 64), g = 64 / chunks, y = lane / chunks, c = 8 * (c0 + lane % chunks);
+            const int chunks = min(cpr - c0, 64), g = 64 / chunks, y = lane / chunks, c = chunk_at<WIDE>(c0 + lane % chunks, a.d);
             float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
             for (int j = first & ~63; j < m; j += 64) {
                 const bool in = j + lane < m && l.tok[min(j + lane, m - 1)] == tl;
@@ -522,12 +534,13 @@ template <int T> __global__ __launch_bounds__(1024) void k_lookup_few(LookupGrad
                 __builtin_amdgcn_wave_barrier();
                 if (in) l.mine[wave][__popcll(mask & ((1ull << lane) - 1))] = l.pos[j + lane];
                 __builtin_amdgcn_wave_barrier();
-                if (y < g) few_rows<T>(a, l.mine[wave], (int)__popcll(mask) * per, y, g, c, s);
+                if (y < g) few_rows<T, WIDE>(a, l.mine[wave], (int)__popcll(mask) * per, y, g, c, s);
             }
             __builtin_amdgcn_wave_barrier();
             if (y < g)
 #pragma unroll
-                for (int x = 0; x < 8; ++x) sums[8 * lane + x] = s[x];
+                for (int x = 0; x < 8; ++x)
+                    if (c + x >= 8 * c0) sums[y * 8 * chunks + c - 8 * c0 + x] = s[x];
             __builtin_amdgcn_wave_barrier();
             for (int z = lane; z < 8 * chunks; z += 64) {
                 float r = sums[z];
@@ -541,7 +554,7 @@ template <int T> __global__ __launch_bounds__(1024) void k_lookup_few(LookupGrad
     for (int i = 0; i < many; ++i) {
         const unsigned token = t0 + (l.many[i] << bits);
         __syncthreads();
-        few_whole<T>(a, token, few_collect(a, token, 32, l), l);
+        few_whole<T, WIDE>(a, token, few_collect(a, token, 32, l), l);
     }
 }
 
@@ -595,7 +608,9 @@ template <int T> hipError_t lookup_backward(const LookupGrad& a, hipStream_t s) 
     if (p.few) {
         // one workgroup a compute unit: 512 (1 024) of them took 16 (26) us instead of 10.5 for 4 096 of 4 096 x 48, 43 (60) instead of 38 for 10 762 of 56 940 x 69
         const bool alone = a.v <= 256;
-        hipLaunchKernelGGL((k_lookup_few<T>), dim3(alone ? (unsigned)a.v : 256), dim3(1024), 0, s, a, alone ? 32 : 8);
+        const dim3 grid(alone ? (unsigned)a.v : 256);
+        if (a.d >= 8) hipLaunchKernelGGL((k_lookup_few<T, true>), grid, dim3(1024), 0, s, a, alone ? 32 : 8);
+        else hipLaunchKernelGGL((k_lookup_few<T, false>), grid, dim3(1024), 0, s, a, alone ? 32 : 8);
         return hipGetLastError();
     }
     if (a.n == 0 || p.tiles == 0) {
@@ -618,7 +633,9 @@ template <int T> hipError_t lookup_backward(const LookupGrad& a, hipStream_t s) 
     }
     const long threads = p.pieces * ((a.d + 7) / 8);
     float* part = reinterpret_cast<float*>(ws + p.part);
-    hipLaunchKernelGGL((k_lookup_sum<T>), dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, s, a, u(p.keys), u(p.pos), p.pieces, p.len, part);
+    const dim3 grid((unsigned)((threads + 255) / 256));
+    if (a.d >= 8) hipLaunchKernelGGL((k_lookup_sum<T, true>), grid, dim3(256), 0, s, a, u(p.keys), u(p.pos), p.pieces, p.len, part);
+    else hipLaunchKernelGGL((k_lookup_sum<T, false>), grid, dim3(256), 0, s, a, u(p.keys), u(p.pos), p.pieces, p.len, part);
     if (p.pieces > 1) hipLaunchKernelGGL((k_lookup_join<T>), dim3((unsigned)((p.pieces + 3) / 4)), dim3(256), 0, s, a, u(p.keys), p.pieces, p.len, part);
     return hipGetLastError();
 }
