@@ -18,6 +18,7 @@ namespace {
 constexpr int SMALL = 4096;          // positions that one workgroup sorts in LDS
 constexpr int TILE = 2048;           // positions a workgroup of the large sort takes
 constexpr int BINS = 512;            // at most 9 bits a pass
+typedef u32x2 Entry;                 // a sorted position: its key, itself (one store where the sort scatters)
 
 __device__ __forceinline__ long index_at(const void* index, int index64, long i) {
     return index64 ? static_cast<const long long*>(index)[i] : (long)static_cast<const int*>(index)[i];
@@ -84,7 +85,7 @@ template <int WAVES> __device__ __forceinline__ unsigned rank_in_wave(unsigned d
 }
 
 // up to SMALL positions, all passes in one workgroup of 16 waves; wave w holds positions 256 w .. 256 w + 255
-__global__ __launch_bounds__(1024) void k_sort_small(LookupGrad a, int passes, int bits, unsigned* keys, unsigned* pos, size_t zero_bytes) {
+__global__ __launch_bounds__(1024) void k_sort_small(LookupGrad a, int passes, int bits, Entry* sorted, size_t zero_bytes) {
     __shared__ unsigned lk[SMALL], lp[SMALL];
     __shared__ unsigned hist[16 * BINS];
     __shared__ unsigned base[BINS];
@@ -138,7 +139,7 @@ __global__ __launch_bounds__(1024) void k_sort_small(LookupGrad a, int passes, i
         }
         __syncthreads();
     }
-    for (int i = t; i < n; i += 1024) { keys[i] = lk[i]; pos[i] = lp[i]; }
+    for (int i = t; i < n; i += 1024) sorted[i] = Entry{lk[i], lp[i]};
 }
 
 template <class Key> __device__ __forceinline__ void count_tile(Key key, long n, int shift, int bits, unsigned* hist) {
@@ -153,11 +154,11 @@ template <class Key> __device__ __forceinline__ void count_tile(Key key, long n,
 
 // Large sort, one pass = three launches: digit counts of each tile, their exclusive sums along the tiles (one workgroup a digit), the scatter.
 // The first pass reads the caller's index; its counting launch also clears the gradient table (tokens that no row has keep zero).
-__global__ __launch_bounds__(256) void k_sort_count(LookupGrad a, const unsigned* keys, int shift, int bits, unsigned* counts, size_t zero_bytes) {
+__global__ __launch_bounds__(256) void k_sort_count(LookupGrad a, const Entry* from, int shift, int bits, unsigned* counts, size_t zero_bytes) {
     __shared__ unsigned hist[BINS];
     for (int i = threadIdx.x; i < BINS; i += 256) hist[i] = 0;
     __syncthreads();
-    if (keys) count_tile([&](long i) { return keys[i]; }, a.n, shift, bits, hist);
+    if (from) count_tile([&](long i) { return from[i][0]; }, a.n, shift, bits, hist);
     else count_tile([&](long i) { return key_at(a, i); }, a.n, shift, bits, hist);
     __syncthreads();
     for (int i = threadIdx.x; i < (1 << bits); i += 256) counts[(size_t)i * gridDim.x + blockIdx.x] = hist[i];
@@ -186,8 +187,7 @@ __global__ __launch_bounds__(256) void k_sort_scan(unsigned* counts, int tiles, 
     if (t == 0) totals[blockIdx.x] = carry;
 }
 
-__global__ __launch_bounds__(256) void k_sort_scatter(LookupGrad a, const unsigned* keys, const unsigned* pos, int shift, int bits, const unsigned* counts, const unsigned* totals,
-                                                      unsigned* keys_out, unsigned* pos_out) {
+__global__ __launch_bounds__(256) void k_sort_scatter(LookupGrad a, const Entry* from, int shift, int bits, const unsigned* counts, const unsigned* totals, Entry* to) {
     __shared__ unsigned hist[4 * BINS];
     __shared__ unsigned base[BINS];
     constexpr int Q = TILE / 256, B = BINS / 256;
@@ -195,12 +195,12 @@ __global__ __launch_bounds__(256) void k_sort_scatter(LookupGrad a, const unsign
     const long i0 = (long)blockIdx.x * TILE + (long)wave * (TILE / 4);
     // everything the tile needs is asked for at once: its keys and positions, its counts, the digits' totals
     unsigned k[Q], p[Q], r[Q], before[B], total[B];
-    if (keys) {
+    if (from) {
 #pragma unroll
         for (int q = 0; q < Q; ++q) {
-            const long i = min(i0 + 64 * q + lane, a.n - 1);
-            k[q] = keys[i];
-            p[q] = pos[i];
+            const Entry e = from[min(i0 + 64 * q + lane, a.n - 1)];
+            k[q] = e[0];
+            p[q] = e[1];
         }
     } else {
 #pragma unroll
@@ -248,8 +248,7 @@ __global__ __launch_bounds__(256) void k_sort_scatter(LookupGrad a, const unsign
     for (int q = 0; q < Q; ++q)
         if (i0 + 64 * q + lane < a.n) {
             const unsigned at = hist[wave * BINS + ((k[q] >> shift) & (bins - 1))] + r[q];
-            keys_out[at] = k[q];
-            pos_out[at] = p[q];
+            to[at] = Entry{k[q], p[q]};
         }
 }
 
@@ -271,7 +270,7 @@ template <int T, bool WIDE> __device__ __forceinline__ Raw8<T> load_chunk(const 
 
 // A thread = 8 columns of one piece: sorted rows [piece * len, piece * len + len), sorted row i = row i % per of the entry i / per.  part [pieces][2][8 cpr]: the sum of the
 // run that comes in from the piece before (0) and of the run that goes on into the next (1).
-template <int T, bool WIDE> __global__ __launch_bounds__(256) void k_lookup_sum(LookupGrad a, const unsigned* keys, const unsigned* pos, long pieces, int len, float* part) {
+template <int T, bool WIDE> __global__ __launch_bounds__(256) void k_lookup_sum(LookupGrad a, const Entry* sorted, long pieces, int len, float* part) {
     constexpr int U = 8;      // rows in flight
     const int cpr = (a.d + 7) >> 3;
     const long id = (long)blockIdx.x * 256 + threadIdx.x;
@@ -285,8 +284,8 @@ template <int T, bool WIDE> __global__ __launch_bounds__(256) void k_lookup_sum(
 #pragma unroll
         for (int e = 0; e < 8; ++e) out[which * 8 * cpr + e] = s[e];
     };
-    unsigned cur = keys[i0 / a.per];
-    bool coming = i0 > 0 && keys[(i0 - 1) / a.per] == cur;
+    unsigned cur = sorted[i0 / a.per][0];
+    bool coming = i0 > 0 && sorted[(i0 - 1) / a.per][0] == cur;
     float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     for (long i = i0; i < i1; i += U) {
         unsigned k[U];
@@ -295,8 +294,9 @@ template <int T, bool WIDE> __global__ __launch_bounds__(256) void k_lookup_sum(
         long e = i / a.per, q = i - e * a.per;
 #pragma unroll
         for (int u = 0; u < U; ++u) {      // (rows beyond the piece: its last again)
-            k[u] = keys[e];
-            at[u] = (long)pos[e] * a.per + q;
+            const Entry x = sorted[e];
+            k[u] = x[0];
+            at[u] = (long)x[1] * a.per + q;
             if (i + u + 1 < i1 && ++q == a.per) { q = 0; ++e; }
         }
 #pragma unroll
@@ -320,7 +320,7 @@ template <int T, bool WIDE> __global__ __launch_bounds__(256) void k_lookup_sum(
     }
     if (cur == none) return;
     if (coming) keep(0, s);
-    else if (i1 < rows && keys[i1 / a.per] == cur) keep(1, s);
+    else if (i1 < rows && sorted[i1 / a.per][0] == cur) keep(1, s);
     else put_sum<T>(a, cur, c, s);
 }
 
@@ -332,7 +332,7 @@ template <int T> __device__ __forceinline__ void put_one(const LookupGrad& a, un
     if constexpr (T == LT_F32) static_cast<float*>(a.dtable)[at] = s;
     else static_cast<unsigned short*>(a.dtable)[at] = (unsigned short)pack2<T>(s, 0.0f);
 }
-template <int T> __global__ __launch_bounds__(256) void k_lookup_join(LookupGrad a, const unsigned* keys, long pieces, int len, const float* part) {
+template <int T> __global__ __launch_bounds__(256) void k_lookup_join(LookupGrad a, const Entry* sorted, long pieces, int len, const float* part) {
     constexpr long SHORT = 16;
     __shared__ f32x4 sums[256];
     __shared__ unsigned token[4];
@@ -342,14 +342,14 @@ template <int T> __global__ __launch_bounds__(256) void k_lookup_join(LookupGrad
     long more = 0;
     unsigned tok = 0;
     if (i1 < rows) {
-        tok = keys[(i1 - 1) / a.per];
-        if (tok != (unsigned)a.v && keys[i1 / a.per] == tok && !(i0 > 0 && keys[(i0 - 1) / a.per] == tok)) {      // (else: no run goes on, or it began in an earlier piece)
+        tok = sorted[(i1 - 1) / a.per][0];
+        if (tok != (unsigned)a.v && sorted[i1 / a.per][0] == tok && !(i0 > 0 && sorted[(i0 - 1) / a.per][0] == tok)) {      // (else: no run goes on, or it began in an earlier piece)
             more = 1;
-            if (i1 + len < rows && keys[(i1 + len) / a.per] == tok) {      // further than the next piece: where the run ends
+            if (i1 + len < rows && sorted[(i1 + len) / a.per][0] == tok) {      // further than the next piece: where the run ends
                 long lo = (i1 + len) / a.per, hi = a.n;
                 while (lo < hi) {
                     const long m = (lo + hi) >> 1;
-                    if (keys[m] <= tok) lo = m + 1; else hi = m;
+                    if (sorted[m][0] <= tok) lo = m + 1; else hi = m;
                 }
                 more = (lo * a.per - 1) / len - piece;
             }
@@ -564,7 +564,7 @@ struct Plan {
     long rows, pieces;
     int len, passes, bits, tiles;
     bool few;
-    size_t keys, pos, keys2, pos2, counts, totals, part, bytes;      // offsets into the workspace
+    size_t sorted, other, counts, totals, part, bytes;      // offsets into the workspace
 };
 
 Plan plan(long n, long per, long v, int d) {
@@ -589,10 +589,8 @@ Plan plan(long n, long per, long v, int d) {
     }
     size_t at = 0;
     auto take = [&](size_t bytes) { const size_t was = at; at += (bytes + 255) & ~(size_t)255; return was; };
-    p.keys = take((size_t)n * 4);
-    p.pos = take((size_t)n * 4);
-    p.keys2 = take(p.tiles ? (size_t)n * 4 : 0);
-    p.pos2 = take(p.tiles ? (size_t)n * 4 : 0);
+    p.sorted = take((size_t)n * sizeof(Entry));
+    p.other = take(p.tiles ? (size_t)n * sizeof(Entry) : 0);
     p.counts = take((size_t)p.tiles << (p.bits + 2));
     p.totals = take(BINS * 4);
     p.part = take((size_t)p.pieces * 2 * 8 * cpr * 4);
@@ -604,6 +602,7 @@ template <int T> hipError_t lookup_backward(const LookupGrad& a, hipStream_t s) 
     const Plan p = plan(a.n, a.per, a.v, a.d);
     char* ws = static_cast<char*>(a.ws);
     auto u = [&](size_t at) { return reinterpret_cast<unsigned*>(ws + at); };
+    Entry *sorted = reinterpret_cast<Entry*>(ws + p.sorted), *other = reinterpret_cast<Entry*>(ws + p.other);
     const size_t zero = (size_t)a.v * a.d * Bytes<T>::v;
     if (p.few) {
         // one workgroup a compute unit: 512 (1 024) of them took 16 (26) us instead of 10.5 for 4 096 of 4 096 x 48, 43 (60) instead of 38 for 10 762 of 56 940 x 69
@@ -618,25 +617,23 @@ template <int T> hipError_t lookup_backward(const LookupGrad& a, hipStream_t s) 
         const bool own = a.n > 0 && zero <= 65536;
         if (!own) hipLaunchKernelGGL(k_clear, dim3((unsigned)(zero / 4096 < 4095 ? zero / 4096 + 1 : 4096)), dim3(256), 0, s, a.dtable, zero);
         if (a.n == 0) return hipGetLastError();
-        hipLaunchKernelGGL(k_sort_small, dim3(1), dim3(1024), 0, s, a, p.passes, p.bits, u(p.keys), u(p.pos), own ? zero : 0);
+        hipLaunchKernelGGL(k_sort_small, dim3(1), dim3(1024), 0, s, a, p.passes, p.bits, sorted, own ? zero : 0);
     } else {
-        const unsigned *kin = nullptr, *pin = nullptr;
+        const Entry* from = nullptr;
         for (int pass = 0; pass < p.passes; ++pass) {
-            const bool to2 = ((p.passes - 1 - pass) & 1) != 0;      // the last pass ends in keys / pos
-            unsigned *ko = u(to2 ? p.keys2 : p.keys), *po = u(to2 ? p.pos2 : p.pos);
-            hipLaunchKernelGGL(k_sort_count, dim3(p.tiles), dim3(256), 0, s, a, kin, pass * p.bits, p.bits, u(p.counts), pass == 0 ? zero : 0);
+            Entry* to = ((p.passes - 1 - pass) & 1) != 0 ? other : sorted;      // the last pass ends in `sorted`
+            hipLaunchKernelGGL(k_sort_count, dim3(p.tiles), dim3(256), 0, s, a, from, pass * p.bits, p.bits, u(p.counts), pass == 0 ? zero : 0);
             hipLaunchKernelGGL(k_sort_scan, dim3(1u << p.bits), dim3(256), 0, s, u(p.counts), p.tiles, u(p.totals));
-            hipLaunchKernelGGL(k_sort_scatter, dim3(p.tiles), dim3(256), 0, s, a, kin, pin, pass * p.bits, p.bits, u(p.counts), u(p.totals), ko, po);
-            kin = ko;
-            pin = po;
+            hipLaunchKernelGGL(k_sort_scatter, dim3(p.tiles), dim3(256), 0, s, a, from, pass * p.bits, p.bits, u(p.counts), u(p.totals), to);
+            from = to;
         }
     }
     const long threads = p.pieces * ((a.d + 7) / 8);
     float* part = reinterpret_cast<float*>(ws + p.part);
     const dim3 grid((unsigned)((threads + 255) / 256));
-    if (a.d >= 8) hipLaunchKernelGGL((k_lookup_sum<T, true>), grid, dim3(256), 0, s, a, u(p.keys), u(p.pos), p.pieces, p.len, part);
-    else hipLaunchKernelGGL((k_lookup_sum<T, false>), grid, dim3(256), 0, s, a, u(p.keys), u(p.pos), p.pieces, p.len, part);
-    if (p.pieces > 1) hipLaunchKernelGGL((k_lookup_join<T>), dim3((unsigned)((p.pieces + 3) / 4)), dim3(256), 0, s, a, u(p.keys), p.pieces, p.len, part);
+    if (a.d >= 8) hipLaunchKernelGGL((k_lookup_sum<T, true>), grid, dim3(256), 0, s, a, sorted, p.pieces, p.len, part);
+    else hipLaunchKernelGGL((k_lookup_sum<T, false>), grid, dim3(256), 0, s, a, sorted, p.pieces, p.len, part);
+    if (p.pieces > 1) hipLaunchKernelGGL((k_lookup_join<T>), dim3((unsigned)((p.pieces + 3) / 4)), dim3(256), 0, s, a, sorted, p.pieces, p.len, part);
     return hipGetLastError();
 }
 
