@@ -1026,25 +1026,32 @@ template <int T> __global__ __launch_bounds__(256, 2) void k_dense_backward_few(
     else dense_few<T, true>(x, blockIdx.x - weight_blocks, reinterpret_cast<float*>(lds));
 }
 
-// The pieces' sums in order, in 64 bits: a workgroup takes 64 of the o k + o values, its 16 waves every 16th piece each (a narrow layer has hundreds of pieces and few values)
-template <int T> __global__ __launch_bounds__(1024) void k_dense_weights_sum(DenseWeights a) {
-    __shared__ double sums[1024];
-    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-    const long nw = (long)a.o * a.k, i = (long)blockIdx.x * 64 + lane;
+// The pieces' sums in order, in 64 bits: a workgroup takes N of the o k + o values, G groups of threads every G-th piece each
+template <int T, int G, int N> __global__ __launch_bounds__(G * N) void k_dense_weights_sum(DenseWeights a) {
+    __shared__ double sums[G > 1 ? G * N : 1];
+    const int t = threadIdx.x, group = t / N;
+    const long nw = (long)a.o * a.k, i = (long)blockIdx.x * N + t % N;
     const bool weight = i < nw, bias = !weight && a.db && i < nw + a.o;
     double s = 0.0;
-    if (weight) {
-#pragma unroll 16
-        for (int q = wave; q < a.splits; q += 16) s += (double)a.part[q * nw + i];
-    } else if (bias) {
-#pragma unroll 16
-        for (int q = wave; q < a.splits; q += 16) s += a.bias_part[(long)q * a.o + (i - nw)];
-    }
-    sums[t] = s;
-    __syncthreads();
-    if (wave != 0 || !(weight || bias)) return;
+    auto add = [&](auto* from, long stride) {      // 16 loads at a time, the last piece again beyond the end
+        for (int q0 = group; q0 < a.splits; q0 += 16 * G) {
+            double v[16];
 #pragma unroll
-    for (int q = 1; q < 16; ++q) s += sums[64 * q + lane];
+            for (int u = 0; u < 16; ++u) v[u] = (double)from[min(q0 + u * G, a.splits - 1) * stride];
+#pragma unroll
+            for (int u = 0; u < 16; ++u) s += q0 + u * G < a.splits ? v[u] : 0.0;
+        }
+    };
+    if (weight) add(a.part + i, nw);
+    else if (bias) add(a.bias_part + (i - nw), (long)a.o);
+    if constexpr (G > 1) {
+        sums[t] = s;
+        __syncthreads();
+        if (group == 0)
+#pragma unroll
+            for (int q = 1; q < G; ++q) s += sums[N * q + t];
+    }
+    if (group != 0 || !(weight || bias)) return;
     void* to = bias ? a.db : a.dw;
     const long at = bias ? i - nw : i;
     if (T == LT_F32 || a.grad32) static_cast<float*>(to)[at] = (float)s;
@@ -1180,7 +1187,10 @@ template <int T> hipError_t dense_weights(const DenseWeights& a, const DenseRows
     }
     if (a.splits > 1) {
         const long m = (long)a.o * a.k + a.o;
-        hipLaunchKernelGGL((k_dense_weights_sum<T>), dim3((unsigned)((m + 63) / 64)), dim3(1024), 0, s, a);
+        if (a.splits <= 16) hipLaunchKernelGGL((k_dense_weights_sum<T, 1, 256>), dim3((unsigned)((m + 255) / 256)), dim3(256), 0, s, a);
+        else if (m >= 16384) hipLaunchKernelGGL((k_dense_weights_sum<T, 4, 64>), dim3((unsigned)((m + 63) / 64)), dim3(256), 0, s, a);
+        else if (a.splits <= 256) hipLaunchKernelGGL((k_dense_weights_sum<T, 16, 64>), dim3((unsigned)((m + 63) / 64)), dim3(1024), 0, s, a);
+        else hipLaunchKernelGGL((k_dense_weights_sum<T, 64, 16>), dim3((unsigned)((m + 15) / 16)), dim3(1024), 0, s, a);
     }
     return hipGetLastError();
 }
