@@ -192,19 +192,22 @@ def dense_backward(dy, x, weight, relu=None, need_dx=True, need_dw=True, need_db
 
 
 def _leaves(*tensors, capturing=None):
-    """A leaf's gradient is accumulated on the stream of the first live graph that reads the leaf.  Under stream capture an EAGER graph that still lives would pull its stream into
-    the captured backward pass, where nothing can be reported and the process ends; so eager graphs sign the accumulation node (it lives as long as they do: called behind the
-    operator that holds it), and a capture that meets the sign is refused."""
-    for t in tensors:
-        if t is not None and t.requires_grad and t.is_leaf:
-            if capturing is None:
-                with _on(t)[2] if t.is_cuda else _SAME_DEVICE:
-                    capturing = t.is_cuda and torch.cuda.is_current_stream_capturing()
-            sign = t.view_as(t).grad_fn.next_functions[0][0].metadata
-            if not capturing:
-                sign["eager"] = True
-            elif "eager" in sign:
-                raise RuntimeError("a graph is being captured while an eager result of the same leaf (%s) is alive: delete that result (or its loss) first" % (tuple(t.shape),))
+    """A leaf's gradient is accumulated on the stream of the first live graph that reads the leaf.  Under stream capture an EAGER graph of the default stream that still lives would
+    pull that stream into the captured backward pass, where nothing can be reported and the process ends; so such graphs sign the accumulation node (it lives as long as
+    they do: called behind the operator that holds it), and a capture that meets the sign is refused."""
+    leaves = [t for t in tensors if t is not None and t.requires_grad and t.is_leaf]
+    default = True
+    if capturing is None and leaves and leaves[0].is_cuda:
+        with _on(leaves[0])[2]:
+            capturing, default = torch.cuda.is_current_stream_capturing(), _raw_stream(leaves[0].get_device()) == 0
+    if not (capturing or default):
+        return
+    for t in leaves:
+        sign = t.view_as(t).grad_fn.next_functions[0][0].metadata
+        if not capturing:
+            sign["eager"] = True
+        elif "eager" in sign:
+            raise RuntimeError("a graph is being captured while an eager result of the same leaf (%s) is alive: delete that result (or its loss) first" % (tuple(t.shape),))
 
 
 class _Dense(torch.autograd.Function):
