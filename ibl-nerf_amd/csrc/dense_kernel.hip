@@ -882,9 +882,12 @@ template <int T, int WO, int WK> __device__ __forceinline__ void dense_weights_t
     for (int i = 0; i < TO; ++i)
 #pragma unroll
         for (int k = 0; k < TK; ++k) acc[i][k] = f32x16{0};
-    // The bias gradient falls off the fragments (a lane has 8 rows of one output), in the waves of the first column tile.  It is one sum over all rows with nothing to average an
-    // error out: added up in 64 bits
-    const bool sums = a.db != nullptr && k0 == 0 && wk == 0;
+    // The bias gradient falls off the fragments (a lane has 8 rows of one output).  It is one sum over all rows with nothing to average an error out: added up in 64 bits, which is as
+    // much work as products are, so it is dealt out — a wave's first 32 outputs to the workgroups of the first column tile, the next to those of the second, and 16 rows in
+    // turn to the waves of one row of tiles (one wave of one workgroup for all of it: 786 432 x 512 took 650 us instead of 590)
+    constexpr int TURNS = WK / 32 / TK;
+    const int turn = place % TURNS;
+    auto sums = [&](int i) { return a.db != nullptr && (kt > 1 ? i : 0) * WK == k0; };
     double bs[TO] = {};
     auto multiply = [&](const unsigned short* zt, int ks) {
         if (SHARE > 1 && ks % SHARE != wave % SHARE) return;
@@ -899,7 +902,7 @@ template <int T, int WO, int WK> __device__ __forceinline__ void dense_weights_t
             for (int q = 0; q < PARTS; ++q) z[q] = frag_across<WO>(zt + q * ZPLANE, wo + i, ks, lane);
 #pragma unroll
             for (int k = 0; k < TK; ++k) acc[i][k] = product<T, PARTS, 1>(z, x[k], acc[i][k]);
-            if (sums)
+            if (sums(i) && ks % TURNS == turn)
 #pragma unroll
                 for (int q = 0; q < PARTS; ++q) {
                     Raw8<T == LT_F16 ? LT_F16 : LT_BF16> v;
@@ -983,6 +986,17 @@ template <int T, int WO, int WK> __device__ __forceinline__ void dense_weights_t
         bs[0] = v;
         if (wave % SHARE != 0) return;
     }
+    if (TURNS > 1 && a.db && k0 < TO * WK) {
+        double* ds = reinterpret_cast<double*>(lds);
+#pragma unroll
+        for (int i = 0; i < TO; ++i) ds[64 * (TO * wave + i) + lane] = bs[i];
+        __syncthreads();
+        if (turn == 0)
+#pragma unroll
+            for (int i = 0; i < TO; ++i)
+#pragma unroll
+                for (int q = 1; q < TURNS; ++q) bs[i] += ds[64 * (TO * (wave + q * SHARE) + i) + lane];
+    }
     const bool last = a.splits == 1;
     auto put = [&](void* to, long at, float v) {
         if (T == LT_F32 || a.grad32) static_cast<float*>(to)[at] = v;
@@ -1000,9 +1014,10 @@ template <int T, int WO, int WK> __device__ __forceinline__ void dense_weights_t
                     else a.part[((long)split * a.o + o) * a.k + c] = acc[i][k][r];
                 }
             }
-    if (sums)
+    if (turn == 0)
 #pragma unroll
         for (int i = 0; i < TO; ++i) {
+            if (!sums(i)) continue;
             const double s = bs[i] + __shfl_xor(bs[i], 32);
             const int o = o0 + 32 * (wo + i) + lane;
             if (lane < 32 && o < a.o) {
