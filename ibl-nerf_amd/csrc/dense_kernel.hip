@@ -1034,10 +1034,10 @@ template <int T, int WO, int WK> __global__ __launch_bounds__(WO == 256 ? 1024 :
 }
 
 // Both gradients of few rows in one launch: neither fills the chip, and they read the same dY.  The weight tiles, which take longer, come first.
-template <int T> __global__ __launch_bounds__(256, 2) void k_dense_backward_few(DenseRows x, DenseWeights w, unsigned weight_blocks) {
-    __shared__ __attribute__((aligned(16))) unsigned short lds[2 * WeightsTile<T, 128, 128>::BUFFER];
-    static_assert(sizeof(lds) >= FEW_LDS * sizeof(float), "one memory for both");
-    if (blockIdx.x < weight_blocks) dense_weights_tile<T, 128, 128>(w, blockIdx.x, lds);
+template <int T, int WO, int WK> __global__ __launch_bounds__(256, 2) void k_dense_backward_few(DenseRows x, DenseWeights w, unsigned weight_blocks) {
+    constexpr int WEIGHTS = 2 * WeightsTile<T, WO, WK>::BUFFER, ROWS = FEW_LDS * 2;
+    __shared__ __attribute__((aligned(16))) unsigned short lds[WEIGHTS > ROWS ? WEIGHTS : ROWS];
+    if (blockIdx.x < weight_blocks) dense_weights_tile<T, WO, WK>(w, blockIdx.x, lds);
     else dense_few<T, true>(x, blockIdx.x - weight_blocks, reinterpret_cast<float*>(lds));
 }
 
@@ -1103,19 +1103,21 @@ template <int T> __global__ __launch_bounds__(256) void k_checkpoint_values(Chec
     }
 }
 
-// few tiles of 128 x 128: small ones instead
-constexpr long FEW_TILES = 64;
-bool few_rows(const DenseRows& a) { return ((a.n + 127) / 128) * ((a.o + 127) / 128) <= FEW_TILES; }
-unsigned few_blocks(const DenseRows& a) { return (unsigned)(((a.n + 31) / 32) * ((a.o + 31) / 32)); }
+// Few rows: 1 024 workgroups of k_dense_few or less, four a compute unit.  (us, k_dense_few / the others, at 1 024 rows of 512 -> 512: float32 14 / 35, bfloat16 8 / 16; 2 048: 22 / 36 and
+// 13 / 16; 4 096: 39 / 37 and 21 / 17; 20 000 of 512 -> 4 bfloat16: 8 / 13)
+long few_blocks(long n, int o) { return ((n + 31) / 32) * ((o + 31) / 32); }
+constexpr long FEW_BLOCKS = 1024;
 
-// Which form Y = act(A B + bias) runs in, and the fragments' memory: the tall form for the 16-bit types once its tiles of 128 rows give every compute unit one (rows of 8
-// elements at least: it reads whole chunks; and as long as the biases of all passes fit LDS beside the two buffers).  A pass makes 256 outputs.
-struct RowsPlan { bool tall, narrow; int passes, steps; };
+// Which form Y = act(A B + bias) runs in, and the fragments' memory.  For the 16-bit types, beyond few rows: the narrow form for at most 32 outputs (100 000 rows of 26 -> 18: 8 us, 30
+// in the tall form; of 500 -> 32: 34, 55; longer rows would take more LDS than leaves room for four workgroups), else the tall form once its tiles of 128 rows give every
+// compute unit one (rows of 8 elements at least: it reads whole chunks; and as long as the biases of all passes fit LDS beside the two buffers).  A pass makes 256 outputs.
+struct RowsPlan { bool few, narrow, tall; int passes, steps; };
 RowsPlan rows_plan(int type, long n, int r, int o) {
     RowsPlan p{};
     p.passes = (o + 255) / 256;
-    p.narrow = type != LT_F32 && o <= 32 && r <= 512 && n > 128 * FEW_TILES;
-    p.tall = !p.narrow && type != LT_F32 && n >= 256 * TALL_ROWS && r >= 8 && p.passes <= 8;
+    p.few = few_blocks(n, o) <= FEW_BLOCKS;
+    p.narrow = !p.few && type != LT_F32 && o <= 32 && r <= 512;
+    p.tall = !p.few && !p.narrow && type != LT_F32 && n >= 256 * TALL_ROWS && r >= 8 && p.passes <= 8;
     p.steps = (r + 63) / 64 * 4;
     return p;
 }
@@ -1155,16 +1157,14 @@ template <int T, bool DX> hipError_t dense_rows(const DenseRows& a, void* ws, hi
             else return !a.codes ? dense_tall<T, TALL_Y>(a, p, wf, s) : a.relu ? dense_tall<T, TALL_RELU_KEEP>(a, p, wf, s) : dense_tall<T, TALL_KEEP>(a, p, wf, s);
         }
     }
-    if (few_rows(a)) {
-        hipLaunchKernelGGL((k_dense_few<T, DX>), dim3(few_blocks(a)), dim3(256), 0, s, a);
+    if (p.few) {
+        hipLaunchKernelGGL((k_dense_few<T, DX>), dim3((unsigned)few_blocks(a.n, a.o)), dim3(256), 0, s, a);
         return hipGetLastError();
     }
     const long pt = ((a.n + 127) / 128 + 7) / 8 * 8;
     hipLaunchKernelGGL((k_dense_rows<T, DX, 128, 128>), dim3((unsigned)(pt * ((a.o + 127) / 128))), dim3(256), 0, s, a);
     return hipGetLastError();
 }
-
-constexpr long NARROW_ROWS = 4096;
 
 // The weight gradient's tile and how many pieces the rows are cut into (functions of the sizes alone)
 struct WeightsPlan { int wo, wk, tiles, splits; };
@@ -1173,9 +1173,10 @@ WeightsPlan weights_plan(int type, long n, int k, int o) {
     const long t4 = (long)((k + 127) / 128) * ((o + 127) / 128), t8 = (long)((k + 255) / 256) * ((o + 255) / 256);
     const long steps = type == LT_F32 ? (n + 31) / 32 : (n + 63) / 64;
     // 256 x 256 where that computes at most half as much again beyond the layer's edges and each of the 256 compute units has some steps to do; pieces of two steps at least
-    // (1 003 x 539 -> 512: 18 us; 25 in 256-wide tiles, 24 in pieces of one step).  A side of at most 32 columns takes 32-wide tiles, where its rows are many.
+    // (1 003 x 539 -> 512: 18 us; 25 in 256-wide tiles, 24 in pieces of one step).  A side of at most 32 columns takes 32-wide tiles (512 -> 4 float32: 9 us instead of 12 for 2 048
+    // rows, 15 instead of 18 for 16 384; 26 <- 5 bfloat16: 15 instead of 100 for 730 935)
     p.wo = p.wk = 2 * 4 * t8 <= 3 * t4 && steps * t8 >= 4 * 256 ? 256 : 128;
-    if (p.wo == 128 && n >= NARROW_ROWS) {
+    if (p.wo == 128) {
         if (o <= 32) p.wo = 32;
         if (k <= 32) p.wk = 32;
     }
@@ -1187,19 +1188,20 @@ WeightsPlan weights_plan(int type, long n, int k, int o) {
 }
 
 // (x: the input gradient where that is asked for too and runs in the few-rows form, or null)
+template <int T, int WO, int WK> void dense_weights(const DenseWeights& a, unsigned blocks, const DenseRows* x, hipStream_t s) {
+    if (x) hipLaunchKernelGGL((k_dense_backward_few<T, WO, WK>), dim3(blocks + (unsigned)few_blocks(x->n, x->o)), dim3(256), 0, s, *x, a, blocks);
+    else hipLaunchKernelGGL((k_dense_weights<T, WO, WK>), dim3(blocks), dim3(256), 0, s, a);
+}
 template <int T> hipError_t dense_weights(const DenseWeights& a, const DenseRows* x, hipStream_t s) {
     const WeightsPlan p = weights_plan(T, a.n, a.k, a.o);
-    const dim3 grid((unsigned)((p.splits + 7) / 8 * 8 * p.tiles));
-    if (x && p.wo == 128 && p.wk == 128) {
-        hipLaunchKernelGGL((k_dense_backward_few<T>), dim3(grid.x + few_blocks(*x)), dim3(256), 0, s, *x, a, grid.x);
-    } else {
-        if (x) hipLaunchKernelGGL((k_dense_few<T, true>), dim3(few_blocks(*x)), dim3(256), 0, s, *x);
-        if (p.wo == 256) hipLaunchKernelGGL((k_dense_weights<T, 256, 256>), grid, dim3(1024), 0, s, a);
-        else if (p.wo == 32 && p.wk == 32) hipLaunchKernelGGL((k_dense_weights<T, 32, 32>), grid, dim3(256), 0, s, a);
-        else if (p.wo == 32) hipLaunchKernelGGL((k_dense_weights<T, 32, 128>), grid, dim3(256), 0, s, a);
-        else if (p.wk == 32) hipLaunchKernelGGL((k_dense_weights<T, 128, 32>), grid, dim3(256), 0, s, a);
-        else hipLaunchKernelGGL((k_dense_weights<T, 128, 128>), grid, dim3(256), 0, s, a);
-    }
+    const unsigned blocks = (unsigned)((p.splits + 7) / 8 * 8 * p.tiles);
+    if (p.wo == 256) {
+        if (x) hipLaunchKernelGGL((k_dense_few<T, true>), dim3((unsigned)few_blocks(x->n, x->o)), dim3(256), 0, s, *x);
+        hipLaunchKernelGGL((k_dense_weights<T, 256, 256>), dim3(blocks), dim3(1024), 0, s, a);
+    } else if (p.wo == 32 && p.wk == 32) dense_weights<T, 32, 32>(a, blocks, x, s);
+    else if (p.wo == 32) dense_weights<T, 32, 128>(a, blocks, x, s);
+    else if (p.wk == 32) dense_weights<T, 128, 32>(a, blocks, x, s);
+    else dense_weights<T, 128, 128>(a, blocks, x, s);
     if (a.splits > 1) {
         const long m = (long)a.o * a.k + a.o;
         if (a.splits <= 16) hipLaunchKernelGGL((k_dense_weights_sum<T, 1, 256>), dim3((unsigned)((m + 255) / 256)), dim3(256), 0, s, a);
@@ -1230,7 +1232,7 @@ hipError_t launch_dense_rows(int type, bool input_gradient, const DenseRows& a, 
 }
 
 hipError_t launch_dense_backward(int type, const DenseRows* x, const DenseWeights* w, void* ws, hipStream_t s) {
-    const bool together = x && w && x->n > 0 && few_rows(*x);
+    const bool together = x && w && x->n > 0 && rows_plan(type, x->n, x->r, x->o).few;
     if (x && x->n > 0 && !together) {
         const hipError_t e = launch_dense_rows(type, true, *x, ws, s);
         if (e != hipSuccess) return e;

@@ -152,7 +152,7 @@ def test_dense_many_rows(n, k, o, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("n,k,o", [(4096, 32, 32), (4095, 32, 32), (5003, 5, 26), (4100, 33, 3), (9001, 280, 5), (6007, 31, 177), (4099, 1, 33), (33100, 26, 18), (33000, 8, 1), (33000, 160, 8), (8229, 26, 500), (8200, 511, 31), (8193, 4, 7)])
+@pytest.mark.parametrize("n,k,o", [(4096, 32, 32), (4095, 32, 32), (5003, 5, 26), (4100, 33, 3), (9001, 280, 5), (6007, 31, 177), (4099, 1, 33), (33100, 26, 18), (33000, 8, 1), (33000, 160, 8), (8229, 26, 500), (8200, 511, 31), (8193, 4, 7), (33001, 511, 31), (32769, 32, 33), (700, 30, 7), (1500, 200, 20), (1025, 9, 140)])
 def test_dense_narrow_layers(n, k, o, dtype):
     """many rows of a layer with at most 32 inputs or outputs, and its borders"""
     g = gen(n + 3 * k + 5 * o)
