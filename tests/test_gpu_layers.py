@@ -416,6 +416,89 @@ def test_lookup_refuses():
         L.lookup(t, i, out=torch.zeros(3, 8, device=DEV).half())
 
 
+# ------------------------------------------------------------------------------------------------------------------------------ the C boundary: strided rows, what lies around them
+class Guarded:
+    """rows x cols elements with a row stride, 64 KB of sentinel bytes before and behind, sentinels between the rows"""
+
+    def __init__(self, rows, cols, dtype, ld=None, values=None, fill=0xA5):
+        self.rows, self.cols, self.ld = rows, cols, ld or cols
+        size = torch.empty((), dtype=dtype).element_size()
+        n = ((rows - 1) * self.ld + cols if rows else 0) * size
+        self.raw = torch.full((65536 + n + 65536,), fill, dtype=torch.uint8, device=DEV)
+        self.view = self.raw[65536:65536 + n].view(dtype).as_strided((rows, cols), (self.ld, 1)) if n else torch.empty((0, cols), dtype=dtype, device=DEV)
+        self.ptr = self.raw.data_ptr() + 65536
+        self.fill = fill
+        if values is not None:
+            self.view.copy_(values)
+
+    def intact(self):
+        """are all bytes but the rows' own still the sentinel?"""
+        mine = torch.zeros(self.raw.numel(), dtype=torch.bool, device=DEV)
+        if self.rows:
+            size = self.view.element_size()
+            mine[65536:mine.numel() - 65536].as_strided((self.rows, self.cols * size), (self.ld * size, 1)).fill_(True)
+        return bool((self.raw[~mine] == self.fill).all())
+
+
+def call(name, *args):
+    import _pkg
+    B = _pkg.load().binding
+    B.check_layers(getattr(B.load_library(), name)(torch.cuda.current_stream().cuda_stream, *args))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,k,o", [(3, 5, 7), (200, 70, 33), (1003, 539, 512), (8300, 65, 130), (8300, 65, 260), (33000, 70, 130), (33000, 26, 18), (40000, 130, 5), (33000, 64, 300)])
+def test_nothing_else_is_read_or_written(n, k, o, dtype):
+    """through the C boundary: rows with a stride, NaN between and behind the inputs' rows, sentinels around the outputs — the same bits as for contiguous rows, the sentinels untouched"""
+    lib = _pkg.load().binding.load_library()
+    code = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}[dtype]
+    g = gen(n + k + o)
+    x, w, b, dy = randn(g, n, k, dtype=dtype).clamp_min(0), randn(g, o, k, dtype=dtype, scale=k ** -0.5), randn(g, o, dtype=dtype), randn(g, n, o, dtype=dtype)
+    gx, gw, gdy = (Guarded(*t.shape, dtype, t.shape[1] + pad, t, fill=0xFF) for t, pad in ((x, 3), (w, 5), (dy, 1)))       # (bytes 0xff: NaN in every type)
+    ko, kk = (o + 31) // 32, (k + 31) // 32
+    y, kept = L.dense_forward(x, w, b, relu=True)
+    gy, gc, gs = Guarded(n, o, dtype, o + 9), Guarded(n, 32 * ko, torch.uint8), Guarded(n, ko, torch.uint8)
+    need = lib.iblnerf_dense_forward_workspace(code, n, k, o)
+    ws = Guarded(1, max(need, 1), torch.uint8)
+    call("iblnerf_dense_forward", code, gx.ptr, k + 3, n, k, gw.ptr, k + 5, o, b.data_ptr(), 1, gy.ptr, o + 9, gc.ptr, gs.ptr, ws.ptr, need)
+    assert torch.equal(gy.view, y) and torch.equal(gc.view, kept.codes) and torch.equal(gs.view, kept.scales)
+    kx = L.checkpoint(x, signed=False)
+    gxc, gxs, gyc = Guarded(n, 32 * kk, torch.uint8, values=kx.codes), Guarded(n, kk, torch.uint8, values=kx.scales), Guarded(n, 32 * ko, torch.uint8, values=kept.codes)
+    cc, cs = Guarded(n, 32 * kk, torch.uint8), Guarded(n, kk, torch.uint8)
+    call("iblnerf_checkpoint", code, gx.ptr, k + 3, n, k, 0, cc.ptr, cs.ptr)
+    assert torch.equal(cc.view, kx.codes) and torch.equal(cs.view, kx.scales)
+    dx, dw, db = L.dense_backward(dy, kx, w, relu=kept)
+    gdx, gdw, gdb = Guarded(n, k, dtype, k + 2), Guarded(o, k, dtype), Guarded(1, o, dtype)
+    need = lib.iblnerf_dense_backward_workspace(code, n, k, o)
+    ws2 = Guarded(1, max(need, 1), torch.uint8)
+    call("iblnerf_dense_backward", code, gdy.ptr, o + 1, n, k, o, gxc.ptr, gxs.ptr, 0, gyc.ptr, gw.ptr, k + 5, gdx.ptr, k + 2, code, gdw.ptr, gdb.ptr, ws2.ptr, need)
+    assert torch.equal(gdx.view, dx) and torch.equal(gdw.view, dw) and torch.equal(gdb.view[0], db)
+    vals = Guarded(n, k, dtype, k + 6)
+    call("iblnerf_checkpoint_values", gxc.ptr, gxs.ptr, n, k, 0, code, vals.ptr, k + 6)
+    assert torch.equal(vals.view, kx.values(dtype))
+    for t in (gx, gw, gdy, gy, gc, gs, ws, cc, cs, gdx, gdw, gdb, ws2, gxc, gxs, gyc, vals):
+        assert t.intact()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,per,v,d", [(5, 3, 7, 9), (4096, 1, 200, 48), (300, 7, 900, 13), (17000, 1, 5000, 21), (2000, 64, 300, 33), (20000, 2, 9, 3)])
+def test_lookups_read_and_write_nothing_else(n, per, v, d, dtype):
+    lib = _pkg.load().binding.load_library()
+    code = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}[dtype]
+    g = gen(n + per + v + d)
+    table, dout, index = randn(g, v, d, dtype=dtype), randn(g, n * per, d, dtype=dtype), torch.randint(-1, v, (n,), generator=g).to(DEV)
+    gt, gd = Guarded(v, d, dtype, d + 3, table, fill=0xFF), Guarded(n * per, d, dtype, d + 5, dout, fill=0xFF)
+    out = Guarded(n * per, d, dtype, d + 7)
+    call("iblnerf_lookup", code, gt.ptr, d + 3, v, d, index.data_ptr(), 64, n, per, 0.5, out.ptr, d + 7)
+    assert torch.equal(out.view, L.lookup(table, index, 0.5, per))
+    need = lib.iblnerf_lookup_backward_workspace(n, per, v, d)
+    ws, grad = Guarded(1, max(need, 1), torch.uint8), Guarded(v, d, dtype)
+    call("iblnerf_lookup_backward", code, gd.ptr, d + 5, index.data_ptr(), 64, n, per, v, d, 0.5, grad.ptr, ws.ptr, need)
+    assert torch.equal(grad.view, L.lookup_backward(dout, index, v, 0.5, per))
+    for t in (gt, gd, out, ws, grad):
+        assert t.intact()
+
+
 # ------------------------------------------------------------------------------------------------------------------------------ streams, graphs, together
 def _step(table, index, x, w1, w2):
     """codes beside the input, two layers, their gradients: what a training step does with the operators together"""
