@@ -89,7 +89,7 @@ struct iblnerf_ctx {
     char* d_stream_mx[N_SLOTS] = {};             // f16 + MX-fp6 form (mlp_precision F16_MXFP6, F16_MIXED, F16X3_MXFP6)
     char* d_stream_f16[N_SLOTS] = {};            // f16 (hi, lo) form of d_stream's layout (mlp_precision F16X3, F16X3_MXFP6)
     GenericNet generic[2];                        // networks 0 / 1 of an architecture OUTSIDE the built one (iblnerf_upload_weights_arch): blob != null = this slot runs
-                                                  // on generic_mlp.hip — every sample of every query, layer by layer in exact fp32; no lists, no estimates, no backward
+                                                  // on generic_mlp.hip — every sample of every query, layer by layer in exact fp32; no lists, no estimates, no backward here (layers_api.cpp)
     float* generic_ws = nullptr;                  // ... its activation workspace (grown on demand)
     size_t generic_ws_floats = 0;
     float* d_blob32[2] = {};                      // networks 0 / 1 as they are: the fp32 state dict (trunk_fp32_kernel.hip reads the reference's own [out][in] rows)

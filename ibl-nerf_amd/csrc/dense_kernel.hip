@@ -255,7 +255,8 @@ template <bool DX, int TO, int TP> __device__ __forceinline__ void begin(f32x16 
 // ------------------------------------------------------------------------------------------------------------------------------ Y = act(A B + bias)
 // One workgroup = BP rows x BO outputs, 4 waves of (BP / 2) x (BO / 2); D[output][row] so that a lane's accumulators are runs of 4 outputs of ONE row.  The reduction runs
 // in steps of BK staged through LDS: the next step's elements travel into registers while this step's products run.
-// Neighbouring workgroups of one XCD take the output tiles of the same rows (the rows are read from HBM once and then from that XCD's L2).
+// Neighbouring workgroups of one XCD take the output tiles of the same rows (the rows are read from HBM once and then from that XCD's L2).  float32 is bound by the six products:
+// 64 064 x 384 -> 384 121 us (156 TFLOP/s of float32, 936 of products; a library's float32 product of 786 432 rows reaches 132), its input gradient 125 for 65 536 rows.
 template <int T, bool DX, int BP, int BO>
 __global__ __launch_bounds__(256, 2) void k_dense_rows(DenseRows a) {
     constexpr int PARTS = T == LT_F32 ? 3 : 1, BK = T == LT_F32 ? 32 : 64;
@@ -368,7 +369,7 @@ template <int T, bool DX> __device__ __forceinline__ void finish8(const DenseRow
 }
 
 // The form for few rows, where one latency after the other is what a call costs: a workgroup makes 32 rows x 32 outputs, each of its 4 waves over a quarter of the reduction, straight
-// from global memory (operands in the order they lie there, 4 steps asked for at once), and the quarters meet in LDS once.
+// from global memory (operands in the order they lie there, 4 steps asked for at once), and the quarters meet in LDS once.  1 x 512 -> 512 bfloat16: 5.0 us of kernel.
 constexpr int FEW_ROW = 36, FEW_LDS = 4 * 32 * FEW_ROW;      // floats
 template <int T, bool DX> __device__ __forceinline__ void dense_few(const DenseRows& a, unsigned block, float* sums) {
     constexpr int U = 4, RS = FEW_ROW;
@@ -476,7 +477,8 @@ template <int T, bool DX> __device__ __forceinline__ u32x4 weight_fragment(const
 }
 
 // The form for many rows of at most 32 outputs (16-bit types): a wave takes 32 rows at a time, straight from memory in the order the matrix instruction wants them; the weights'
-// operands stay in LDS.  Chunks are read whole: what lies behind a row's end is cleared in registers, and only rows with 7 more behind them are read so.
+// operands stay in LDS.  Chunks are read whole: what lies behind a row's end is cleared in registers, and only rows with 7 more behind them are read so.  Bound by HBM once rows
+// are long (100 000 x 500 -> 32 bfloat16: 34 us, 3.1 TB/s), by the many small stores where they are short (730 935 x 26 -> 5: 15 us, 3 TB/s).
 template <int T, bool DX> __global__ __launch_bounds__(256, 4) void k_dense_narrow(DenseRows a) {
     constexpr int U = 4;
     extern __shared__ __attribute__((aligned(16))) float narrow[];
@@ -796,11 +798,13 @@ __global__ __launch_bounds__(256, 2) void k_dense_tall(DenseRows a, const u32x4*
 }
 
 // --------------------------------------------------------------------------------------------------------------------------------- dW = dZ^T X, db
-// One workgroup = a square tile of outputs x input columns over its piece of the rows, BR rows a step.  Both operands lie with the REDUCTION index as the row, as
+// One workgroup = a tile of WO outputs x WK input columns over its piece of the rows, BR rows a step.  Both operands lie with the REDUCTION index as the row, as
 // they do in memory, and are turned by the transposing LDS read.  The pieces' sums go to `part` and are added in order by k_dense_weights_sum: no atomics, the same
 // bits every time.
 //
-// W = 128: 4 waves, two workgroups on a compute unit; W = 256: 16 waves, half as many reads of either operand.  A wave takes 64 x 64.
+// 128 x 128: 4 waves of 64 x 64, two workgroups on a compute unit; 256 x 256: 16 waves, half as many reads of either operand; 32 on the side of a narrow layer: a wave has one
+// 32 x 32 tile, or a share of the rows of the only one.  786 432 x 512 -> 512 float16: 550 us (1.6 GB: 2.9 TB/s; 750 TFLOP/s), bound by the way through registers and LDS that
+// turns and decodes the operands; 65 536 x 384 float32 85 us; 196 608 x 512 -> 4 float32 52.
 template <int T, int WO, int WK> struct WeightsTile {
     static constexpr int NT = WO == 256 ? 1024 : 256, PARTS = T == LT_F32 ? 3 : 1, BR = T == LT_F32 && WO != 32 ? 32 : 64;
     static constexpr int ZPLANE = BR * WO, XPLANE = BR * WK, BUFFER = PARTS * ZPLANE + XPLANE;
@@ -1041,7 +1045,9 @@ template <int T, int WO, int WK> __global__ __launch_bounds__(256, 2) void k_den
     else dense_few<T, true>(x, blockIdx.x - weight_blocks, reinterpret_cast<float*>(lds));
 }
 
-// The pieces' sums in order, in 64 bits: a workgroup takes N of the o k + o values, G groups of threads every G-th piece each
+// The pieces' sums in order, in 64 bits: a workgroup takes N of the o k + o values, G groups of threads every G-th piece each.  Many values fill the chip by themselves, few values
+// of many pieces take groups (26 x 5 values of 1 024 pieces: 130 us with one thread a value, 13 with 16 groups, 6 with 64; 512 x 539 of 8: 4 us with one, 12.5 with 16;
+// 384 x 384 of 56: 7 with four, 17 with one)
 template <int T, int G, int N> __global__ __launch_bounds__(G * N) void k_dense_weights_sum(DenseWeights a) {
     __shared__ double sums[G > 1 ? G * N : 1];
     const int t = threadIdx.x, group = t / N;
@@ -1074,6 +1080,7 @@ template <int T, int G, int N> __global__ __launch_bounds__(G * N) void k_dense_
 }
 
 // ------------------------------------------------------------------------------------------------------------------------- checkpoints on their own
+// One pass, a thread = 8 columns, HBM-bound: 786 432 x 512 bfloat16 in 250 us (1.2 GB: 4.9 TB/s, what a copy reaches), back in 225.
 template <int T> __global__ __launch_bounds__(256) void k_checkpoint(const char* x, long ld, long n, int k, int is_signed, uint8_t* codes, uint8_t* scales) {
     const int cpr = ((k + 31) >> 5) * 4;      // 8-column chunks a row; a block's four lie in four neighbouring lanes
     const long total = n * cpr;

@@ -4,10 +4,13 @@
 //
 // A negative index is a row without a code: zeros, no gradient.  An index beyond the table reads NaN (a wrong index shows) and has no gradient.
 //
-// The gradient is bound by reading dOut once, in an order that the tokens set.  The positions are sorted by token (stable, so a token's rows keep their order), the sorted
-// rows are cut into pieces of equal length — a token that most rows share (a batch drawn from few views) costs no more than any other — and each piece adds up its
-// runs of equal tokens in 32 bits.  A run inside one piece is finished there; the pieces of a longer run are joined in order by k_lookup_join.  No atomics on
-// values: the same inputs give the same bits.
+// The gradient is bound by reading dOut once, in an order that the tokens set.  Up to 16 384 positions one launch does it all (k_lookup_few).  Otherwise the positions are sorted
+// by token (stable, so a token's rows keep their order), the sorted rows are cut into pieces of equal length — a token that most rows share (a batch drawn from few views)
+// costs no more than any other — and each piece adds up its runs of equal tokens in 32 bits.  A run inside one piece is finished there; the pieces of a longer run are
+// joined in order by k_lookup_join.  No atomics on values: the same inputs give the same bits.
+//
+// Measured: lookup 786 432 x 32 bfloat16 12.5 us (50 MB: 4.0 TB/s).  Gradient of 4 096 positions, 200 x 48: 6.4 us.  Of 640 000, 65 536 x 64 float32: 81 to 94 us — each of two
+// sorting passes 6.7 (counts) + 3.7 (their sums) + 11 (scatter), rows 31 (164 MB: 5.3 TB/s), joins 11.
 #include "layer_elems.h"
 #include "layers.h"
 
@@ -397,7 +400,9 @@ template <int T> __global__ __launch_bounds__(256) void k_lookup_join(LookupGrad
 // tokens are a wave's work each (where positions are fewer than tokens, found by their first position).
 constexpr int MANY = 256;      // rows
 constexpr int FEW = 16384;     // positions
-constexpr long FEW_ROWS = 65536, FEW_ELEMENTS = 1 << 21, FEW_SHARE = 32768;      // rows, elements of dOut, elements a token on the average
+// rows, elements of dOut, elements a token on the average: beyond these one workgroup may have too much to read alone (8 192 rows of one token x 256 float32: 87 us, 27 in pieces;
+// 13 030 positions of 2 495 x 1: 19, 43 in pieces)
+constexpr long FEW_ROWS = 65536, FEW_ELEMENTS = 1 << 21, FEW_SHARE = 32768;
 struct FewLds {
     unsigned short pos[FEW], tok[FEW];
     unsigned short mine[16][64];

@@ -248,7 +248,8 @@ int iblnerf_upload_weights(iblnerf_ctx* ctx, int which, const float* h_blob, siz
  * src/nerf_models/ibl_nerf.py:14-60 and config_parser.py's --netdepth / --netwidth / --multires / --multires_views accept any.  h_blob = the state dict's tensors in
  * registration order, [out, in] row-major weight then bias per layer (ibl-nerf_amd/checkpoint.py arch_schema / arch_blob).  Such a network is evaluated by
  * csrc/generic_mlp.hip: layer by layer in exact fp32 on the matrix cores (v_mfma_f32_32x32x2_f32), activations in HBM, every sample of every query — no lists, no
- * estimates (the context holds no route), no backward (the gradient entry points return IBLNERF_ERR_STATE for this slot), not for colour-independent contexts;
+ * estimates (the context holds no route), no backward in this header (the gradient entry points return IBLNERF_ERR_STATE for this slot; iblnerf_layers.h trains such
+ * networks layer by layer), not for colour-independent contexts;
  * ~1/20 of the fused kernels' rate at the built width.  Networks INSIDE the built architecture (smaller ones) are embedded exactly by the caller and uploaded with
  * iblnerf_upload_weights.  A later iblnerf_upload_weights for the same slot takes the slot back to the fused kernels. */
 int iblnerf_upload_weights_arch(iblnerf_ctx* ctx, int which, const float* h_blob, size_t n_floats, int netdepth, int netwidth, int multires, int multires_views);
