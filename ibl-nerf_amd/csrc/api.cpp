@@ -570,6 +570,11 @@ int iblnerf_upload_weights_device(iblnerf_ctx* c, void* stream, int which, const
                                    (hipStream_t)stream));
     c->mx_ok[which] = true;
     c->have_net[which] = true;
+    if (c->generic[which].blob) {                 // the slot held a network of another architecture, which a render may still be reading
+        HIP_TRY(c, hipDeviceSynchronize());
+        (void)hipFree(const_cast<float*>(c->generic[which].blob));
+        c->generic[which] = GenericNet();
+    }
     reset_route(c, which);
     return arm_range_snapshot(c, (hipStream_t)stream);
 }

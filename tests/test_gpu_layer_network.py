@@ -236,6 +236,51 @@ def test_steps_of_a_larger_network_learn(lut):
     assert all(torch.isfinite(p).all() and not torch.equal(p, q) for p, q in zip((p for net in nets for p in net.parameters()), before))
 
 
+@pytest.mark.parametrize("approx", [False, True])
+def test_a_batch_and_its_halves(lut, approx):
+    """2 304 rays (the backward on the live samples, where a route would be held for the built shape): the gradients of a summed loss are those of its two halves.  The same rows, the
+    same codes: what differs is the order of float32 sums over up to 2 304 x 64 rows (their rounding averages out: 2^-24 sqrt(10^5) = 2e-5 of the magnitudes summed) and the
+    rows below 1e-7 of a pass's largest."""
+    from ibl_nerf_amd import renderer as R
+    arch = (8, 288, 10, 4)
+    nets = [RefShaped(ck.synthetic_arch_state_dict(s, arch, 1.5, sigma_bias=1.0), arch).cuda() for s in (1, 2)]
+    for net in nets:
+        net.coarse_radiance_number = 3
+    params = [p for net in nets for p in net.parameters()]
+    kw = dict(network_fn=nets[0], network_fine=nets[1], N_samples=32, N_importance=32, perturb=0.0, brdf_lut=torch.from_numpy(lut).cuda(), lut_coefficient="F", gamma_correct=True,
+              use_radiance_linear=False, near=0.5, far=4.0, epsilon=0.01, correct_depth_for_prefiltered_radiance_infer=True,
+              target_normal_map_for_radiance_calculation="normal_map_from_depth_gradient_epsilon")
+    g = torch.Generator().manual_seed(1)
+    rays = torch.stack([torch.zeros(2304, 3), torch.nn.functional.normalize(torch.randn(2304, 3, generator=g), dim=-1)]).cuda()
+
+    def grads(part):
+        res = R.render_decomp(8, 12, np.eye(3, dtype=np.float32), rays=rays[:, part].contiguous(), gt_values={}, approximate_radiance=approx, **kw)
+        loss = sum((res[k + s] - 0.3).square().sum() for k in ("radiance_map", "albedo_map", "irradiance_map", "radiance_map_1") for s in ("", "0"))
+        return torch.autograd.grad(loss, params, allow_unused=True)
+    whole, a, b = grads(slice(0, 2304)), grads(slice(0, 1152)), grads(slice(1152, 2304))
+    names = [n for net in nets for n, _ in net.named_parameters()]
+    assert sum(w is not None and bool(w.any()) for w in whole) >= 60
+    for n, w, x, y in zip(names, whole, a, b):
+        if w is not None:
+            assert (w - (x + y)).abs().max() <= 1e-3 * max(float(x.abs().max() + y.abs().max()), 1e-6), n
+
+
+def test_a_context_takes_a_built_network_behind_a_larger_one():
+    """weights that live on the GPU (a training step's) leave a slot that held a larger network as a fresh context has it"""
+    from ibl_nerf_amd import renderer as R
+    built, larger = (8, 256, 10, 4), (8, 264, 10, 4)
+    sds = [{k: torch.from_numpy(v).cuda() for k, v in ck.synthetic_arch_state_dict(s, a, 1.5).items()} for s, a in ((4, built), (5, larger), (6, built))]
+    g = torch.Generator().manual_seed(2)
+    pts, dirs = (torch.rand(50, 7, 3, generator=g) - 0.5).cuda(), torch.randn(50, 3, generator=g).cuda()
+    used, fresh = R.Renderer(64, 128), R.Renderer(64, 128)
+    used.load_weights(0, sds[0])
+    used.load_weights(0, sds[1])
+    big = used.network_query(pts, dirs, 0)
+    used.load_weights(0, sds[2])
+    fresh.load_weights(0, sds[2])
+    assert torch.equal(used.network_query(pts, dirs, 0), fresh.network_query(pts, dirs, 0)) and not torch.equal(used.network_query(pts, dirs, 0), big)
+
+
 def test_points_and_density_alone_against_differences():
     """The density's gradient in the points (the trunk-only query of the normal modes) against central differences of the float64 module, on points whose ReLU arguments keep 2e-5 of
     their layer's rms from zero: no step of 1e-8 and no float32 error crosses one.  The differences are right to 1e-16 / 1e-8; the float32 products to 22 * 270 * 2^-23 = 7e-4 of the
