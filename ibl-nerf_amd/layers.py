@@ -23,7 +23,7 @@ _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 MAX_COLUMNS, MAX_STRIDE = 65536, 1 << 24
 # the current stream's handle without a Stream object around it (these calls cost microseconds, and so do a small layer's kernels)
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda device: torch.cuda.current_stream(device).cuda_stream)
-_SAME_DEVICE = contextlib.nullcontext()
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
 def _type(t, what):
@@ -34,11 +34,21 @@ def _type(t, what):
 
 
 def _on(t):
-    """(library, stream, guard): the tensor's device made current for the call where it is not."""
+    """(library, stream, what makes the tensor's device current for the call, or None where it is)."""
     if not t.is_cuda:
         raise B.IblNerfError("the layer operators have no CPU path: got a tensor on %s" % t.device)
     dev = t.get_device()
-    return B.load_library(), _raw_stream(dev), _SAME_DEVICE if dev == torch.cuda.current_device() else torch.cuda.device(dev)
+    return B.load_library(), _raw_stream(dev), None if dev == _current_device() else torch.cuda.device(dev)
+
+
+def _call(guard, f, *args):
+    if guard is None:
+        rc = f(*args)
+    else:
+        with guard:
+            rc = f(*args)
+    if rc:
+        B.check_layers(rc)
 
 
 def _same(t, like, what, dtype=None):
@@ -96,8 +106,7 @@ class Checkpoint:
         out = self.codes.new_empty((self.codes.shape[0], self.columns), dtype=dtype)
         t = _type(out, "the values")
         lib, stream, guard = _on(out)
-        with guard:
-            B.check_layers(lib.iblnerf_checkpoint_values(stream, self.codes.data_ptr(), self.scales.data_ptr(), self.rows, self.columns, int(self.signed), t, out.data_ptr(), self.columns))
+        _call(guard, lib.iblnerf_checkpoint_values, stream, self.codes.data_ptr(), self.scales.data_ptr(), self.rows, self.columns, int(self.signed), t, out.data_ptr(), self.columns)
         return out
 
 
@@ -120,8 +129,7 @@ def checkpoint(x, signed=True):
     x, ld = _rows(x, "x")
     n, k = x.shape
     codes, scales = _codes_like(x, n, k)
-    with guard:
-        B.check_layers(lib.iblnerf_checkpoint(stream, t, x.data_ptr(), ld, n, k, int(bool(signed)), codes.data_ptr(), scales.data_ptr()))
+    _call(guard, lib.iblnerf_checkpoint, stream, t, x.data_ptr(), ld, n, k, int(bool(signed)), codes.data_ptr(), scales.data_ptr())
     return _made(codes, scales, k, signed)
 
 
@@ -152,9 +160,8 @@ def dense_forward(x, weight, bias=None, relu=False, keep=True):
     y = x.new_empty((n, o))
     codes, scales = _codes_like(x, n, o) if keep else (None, None)
     ws, ws_bytes = _workspace(lib.iblnerf_dense_forward_workspace(t, n, k, o), x)
-    with guard:
-        B.check_layers(lib.iblnerf_dense_forward(stream, t, x.data_ptr(), ld, n, k, w.data_ptr(), ldw, o, _address(bias), int(bool(relu)), y.data_ptr(), o, _address(codes), _address(scales),
-                                                 _address(ws), ws_bytes))
+    _call(guard, lib.iblnerf_dense_forward, stream, t, x.data_ptr(), ld, n, k, w.data_ptr(), ldw, o, _address(bias), int(bool(relu)), y.data_ptr(), o, _address(codes), _address(scales),
+          _address(ws), ws_bytes)
     return (y if len(lead) == 1 else y.reshape(lead + (o,))), (_made(codes, scales, o, not relu) if keep else None)
 
 
@@ -184,10 +191,9 @@ def dense_backward(dy, x, weight, relu=None, need_dx=True, need_dw=True, need_db
     dw = dy.new_empty((o, k), dtype=grad_dtype) if need_dw or need_db else None
     db = dy.new_empty((o,), dtype=grad_dtype) if need_db else None
     ws, ws_bytes = _workspace(lib.iblnerf_dense_backward_workspace(t, n, k, o), dy)
-    with guard:
-        B.check_layers(lib.iblnerf_dense_backward(stream, t, dy.data_ptr(), ld, n, k, o, x.codes.data_ptr(), x.scales.data_ptr(), int(x.signed),
-                                                  None if relu is None else relu.codes.data_ptr(), w.data_ptr(), ldw, _address(dx), k, _TYPES[grad_dtype], _address(dw), _address(db),
-                                                  _address(ws), ws_bytes))
+    _call(guard, lib.iblnerf_dense_backward, stream, t, dy.data_ptr(), ld, n, k, o, x.codes.data_ptr(), x.scales.data_ptr(), int(x.signed),
+          None if relu is None else relu.codes.data_ptr(), w.data_ptr(), ldw, _address(dx), k, _TYPES[grad_dtype], _address(dw), _address(db),
+          _address(ws), ws_bytes)
     return (dx if dx is None or len(lead) == 1 else dx.reshape(lead + (k,))), (dw if need_dw else None), db
 
 
@@ -198,7 +204,7 @@ def _leaves(*tensors, capturing=None):
     leaves = [t for t in tensors if t is not None and t.requires_grad and t.is_leaf]
     default = True
     if capturing is None and leaves and leaves[0].is_cuda:
-        with _on(leaves[0])[2]:
+        with _on(leaves[0])[2] or contextlib.nullcontext():
             capturing, default = torch.cuda.is_current_stream_capturing(), _raw_stream(leaves[0].get_device()) == 0
     if not (capturing or default):
         return
@@ -276,8 +282,7 @@ def _lookup(table, index, scale, rows_per_index, out):
         if out.dim() != 2 or tuple(out.shape) != (n * per, d) or (d > 1 and out.stride(1) != 1) or (out.shape[0] > 1 and not d <= out.stride(0) <= MAX_STRIDE):
             raise ValueError("out must be [%d, %d] with unit stride along a row, got %s strides %s" % (n * per, d, tuple(out.shape), tuple(out.stride())))
     ld_out = out.stride(0) if out.dim() == 2 and out.shape[0] > 1 else d
-    with guard:
-        B.check_layers(lib.iblnerf_lookup(stream, t, tab.data_ptr(), ld, v, d, idx.data_ptr(), bits, n, per, float(scale), out.data_ptr(), ld_out))
+    _call(guard, lib.iblnerf_lookup, stream, t, tab.data_ptr(), ld, v, d, idx.data_ptr(), bits, n, per, float(scale), out.data_ptr(), ld_out)
     return out
 
 
@@ -293,8 +298,7 @@ def lookup_backward(dout, index, v, scale=1.0, rows_per_index=1):
         raise ValueError("%d indices with %d rows each over a table of %d rows do not fit %d gradient rows" % (n, per, int(v), dout.shape[0]))
     grad = dout.new_empty((int(v), d))
     ws, ws_bytes = _workspace(lib.iblnerf_lookup_backward_workspace(n, per, int(v), d), dout)
-    with guard:
-        B.check_layers(lib.iblnerf_lookup_backward(stream, t, dout.data_ptr(), ld, idx.data_ptr(), bits, n, per, int(v), d, float(scale), grad.data_ptr(), _address(ws), ws_bytes))
+    _call(guard, lib.iblnerf_lookup_backward, stream, t, dout.data_ptr(), ld, idx.data_ptr(), bits, n, per, int(v), d, float(scale), grad.data_ptr(), _address(ws), ws_bytes)
     return grad
 
 
