@@ -416,6 +416,50 @@ def test_lookup_refuses():
         L.lookup(t, i, out=torch.zeros(3, 8, device=DEV).half())
 
 
+# ------------------------------------------------------------------------------------------------------------------------------ offsets beyond 32 bits
+@pytest.mark.parametrize("dtype,n,k,o", [(torch.bfloat16, 8400000, 520, 520), (torch.float32, 2200000, 500, 500), (torch.bfloat16, 150000000, 30, 20)])
+def test_offsets_beyond_32_bits(dtype, n, k, o):
+    """the last rows of tensors of more than 4 GB (more than 2^32 elements in 16 bits) are what a call on those rows alone gives, bit for bit (40 000: the same form of the kernels)"""
+    g = torch.Generator(device=DEV)
+    g.manual_seed(n)
+    tail = 40000
+    w, b = torch.randn(o, k, generator=g, device=DEV).to(dtype), torch.randn(o, generator=g, device=DEV).to(dtype)
+    x = torch.zeros(n, k, dtype=dtype, device=DEV)
+    x[-tail:] = torch.randn(tail, k, generator=g, device=DEV).to(dtype)
+    y, kept = L.dense_forward(x, w, b, relu=True)
+    y2, kept2 = L.dense_forward(x[-tail:].clone(), w, b, relu=True)
+    assert torch.equal(y[-tail:], y2) and torch.equal(kept.codes[-tail:], kept2.codes) and torch.equal(kept.scales[-tail:], kept2.scales)
+    assert torch.equal(y[0], b.clamp_min(0)) and torch.equal(y[n // 2], y[0])
+    kx, kx2 = L.checkpoint(x), L.checkpoint(x[-tail:].clone())
+    assert torch.equal(kx.codes[-tail:], kx2.codes) and torch.equal(kx.scales[-tail:], kx2.scales)
+    del x, y2
+    vals = kx.values(dtype)
+    assert torch.equal(vals[-tail:], kx2.values(dtype)) and not vals[0].any()
+    del vals
+    dy = torch.zeros_like(y)
+    del y
+    dy[-tail:] = torch.randn(tail, o, generator=g, device=DEV).to(dtype)
+    dx, dw, db = L.dense_backward(dy, kx, w, relu=kept, grad_dtype=torch.float32)
+    dx2, dw2, db2 = L.dense_backward(dy[-tail:].clone(), kx2, w, relu=kept2, grad_dtype=torch.float32)
+    assert torch.equal(dx[-tail:], dx2) and not dx[0].any()
+    for p, q in ((dw, dw2), (db, db2)):          # (other pieces: float32 sums of 40 000 terms in another order, 200 of them in one chain at random)
+        assert (p - q).abs().max() <= 2e-4 * q.abs().max()
+
+
+def test_lookup_offsets_beyond_32_bits():
+    n, per, d = 400000, 192, 64
+    g = torch.Generator(device=DEV)
+    g.manual_seed(1)
+    table, index = torch.randn(50, d, generator=g, device=DEV).half(), torch.randint(0, 50, (n,), generator=g, device=DEV)
+    out = L.lookup(table, index, 1.0, per)
+    assert torch.equal(out[-per * 1000:], table[index[-1000:].repeat_interleave(per)]) and torch.equal(out[0], table[index[0]])
+    out.zero_()
+    out[-per * 1000:] = torch.randint(-1, 2, (per * 1000, d), generator=g, device=DEV).half()
+    got = L.lookup_backward(out, index, 50, 1.0, per)
+    want = torch.zeros(50, d, dtype=torch.float64, device=DEV).index_add_(0, index[-1000:].repeat_interleave(per), out[-per * 1000:].double())
+    assert torch.equal(got, want.half())          # (whole numbers)
+
+
 # ------------------------------------------------------------------------------------------------------------------------------ the C boundary: strided rows, what lies around them
 class Guarded:
     """rows x cols elements with a row stride, 64 KB of sentinel bytes before and behind, sentinels between the rows"""
