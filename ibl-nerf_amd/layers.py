@@ -342,7 +342,7 @@ def _linear(params, name):
     return params[name + ".weight"], params[name + ".bias"]
 
 
-def network_query(inputs, viewdirs, network_fn, codes=None, views=None, code_scale=1.0, dtype=torch.float32):
+def network_query(inputs, viewdirs, network_fn, codes=None, views=None, code_scale=1.0, dtype=None):
     """IBLNeRF.forward (ibl_nerf.py:154-208) of a network of ANY depth and width, with autograd, on `dense`: inputs [..., 3] points, viewdirs [n, 3] one direction for each row
     of points (or None: the density alone, :175-176), `network_fn` a torch module with the reference's parameter names -> raw [..., 18] float32 (or [..., 1]).  What is held for
     the backward pass is one 8-bit checkpoint of each activation.
@@ -350,7 +350,9 @@ def network_query(inputs, viewdirs, network_fn, codes=None, views=None, code_sca
     encoding of every sample of the ray: views_linears.0 then takes c more columns (checkpoint.bake_view_code makes the network of one view for rendering); the codes
     receive their gradient by sorted views.  (Such a network queried without its codes is refused by its width, unless c is a multiple of 6: then its shapes are those of a
     network with more frequencies.)
-    dtype: the type of the layers between the encodings and the heads (float32, bfloat16, float16); parameters stay what they are, heads are float32."""
+    dtype: the type of the layers between the encodings and the heads (float32, bfloat16, float16: the last for a scaled loss); parameters stay what they are, heads are float32.
+    None: what the module's attribute `layer_dtype` says, or float32."""
+    dtype = dtype or getattr(network_fn, "layer_dtype", None) or torch.float32
     params = dict(network_fn.named_parameters())
     if getattr(network_fn, "is_color_independent_to_direction", False):
         raise NotImplementedError("colour-independent networks run on the fused kernels only")
@@ -404,8 +406,9 @@ def network_query(inputs, viewdirs, network_fn, codes=None, views=None, code_sca
     return torch.cat(out, -1).reshape(lead + (18,))
 
 
-def network_gradients(inputs, viewdirs, draw, network_fn, dtype=torch.float32, points=1 << 20):
+def network_gradients(inputs, viewdirs, draw, network_fn, dtype=None, points=1 << 20):
     """{parameter name: dL/d parameter} of network_query from dL/d raw (draw [n, S, 18]), `points` samples at a time (14 checkpoints of a 512-wide network: 7 KB a sample)."""
+    dtype = dtype or getattr(network_fn, "layer_dtype", None)
     named = dict(network_fn.named_parameters())
     names, params = list(named), list(named.values())
     total = None

@@ -267,11 +267,11 @@ def fused_network_query(inputs, viewdirs, network_fn, codes=None, views=None, co
     """`network_query_fn(inputs, viewdirs, network_fn)` WITH autograd, the whole network on the fused kernels in both directions: forward =
     the precise network query, backward = iblnerf_network_backward (dL/d raw rows in; dL/dinputs and all 46 parameter gradients out).
     A network outside the built shape, and any network with a code for each view (codes, views, code_scale: layers.network_query), runs layer by layer from 8-bit
-    checkpoints, its layers in layer_dtype (float32 by default)."""
+    checkpoints, its layers in layer_dtype (None: the module's attribute of that name, or float32; a training render takes the attribute)."""
     import torch
     if codes is not None or layer_dtype is not None or layered(network_fn):
         from . import layers
-        return layers.network_query(inputs, viewdirs, network_fn, codes=codes, views=views, code_scale=code_scale, dtype=layer_dtype or torch.float32)
+        return layers.network_query(inputs, viewdirs, network_fn, codes=codes, views=views, code_scale=code_scale, dtype=layer_dtype)
     named = dict(network_fn.named_parameters())
     params = [named[k] for k in ALL_PARAMS]
 

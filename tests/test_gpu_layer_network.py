@@ -321,6 +321,31 @@ def test_pieces_of_a_batch_and_its_whole():
     assert empty.shape == (0, 8, 18)
 
 
+def test_the_type_of_the_layers_is_the_modules_attribute(lut):
+    from ibl_nerf_amd import renderer as R
+    arch = (2, 264, 4, 1)
+    nets = [RefShaped(ck.synthetic_arch_state_dict(s, arch, 1.5, sigma_bias=1.0), arch).cuda() for s in (1, 2)]
+    g = torch.Generator().manual_seed(2)
+    pts, dirs, draw = torch.rand(40, 8, 3, generator=g).cuda(), torch.randn(40, 3, generator=g).cuda(), torch.randn(40, 8, 18, generator=g).cuda()
+    rays = torch.stack([torch.zeros(40, 3), torch.nn.functional.normalize(torch.randn(40, 3, generator=g), dim=-1)]).cuda()
+    kw = dict(network_fn=nets[0], network_fine=nets[1], N_samples=32, N_importance=32, perturb=0.0, brdf_lut=torch.from_numpy(lut).cuda(), lut_coefficient="F", gamma_correct=True,
+              use_radiance_linear=False, near=0.5, far=4.0)
+
+    def step():
+        res = R.render_decomp(8, 12, np.eye(3, dtype=np.float32), rays=rays, gt_values={}, approximate_radiance=False, **kw)
+        w = nets[1].positions_linears[1].weight
+        return torch.autograd.grad((res["radiance_map"] - 0.3).square().sum(), w)[0]
+    single = layers.network_gradients(pts, dirs, draw, nets[0]), M.fused_network_query(pts, dirs, nets[0]).detach(), step()
+    low = layers.network_gradients(pts, dirs, draw, nets[0], dtype=torch.bfloat16), M.fused_network_query(pts, dirs, nets[0], layer_dtype=torch.bfloat16).detach()
+    for net in nets:
+        net.coarse_radiance_number, net.layer_dtype = 3, torch.bfloat16
+    got = layers.network_gradients(pts, dirs, draw, nets[0]), M.fused_network_query(pts, dirs, nets[0]).detach(), step()
+    assert all(torch.equal(got[0][k], low[0][k]) and got[0][k].dtype == torch.float32 for k in low[0]) and torch.equal(got[1], low[1])
+    assert not torch.equal(got[1], single[1]) and not torch.equal(got[2], single[2])
+    # (the step's gradient in 16 bits: 2 + 3 layers forward and backward, 10 roundings of 2^-8 and half a code step: 0.08 of the magnitudes summed, which here cancel little)
+    assert float((got[2] - single[2]).norm()) <= 0.08 * float(single[2].norm())
+
+
 def test_captured_training_of_a_network():
     """forward and backward in a graph, replayed with new points between eager work; an eager result of the same leaves that is alive is refused."""
     arch = (2, 264, 4, 1)
