@@ -3,7 +3,8 @@
 // CHECKPOINT of an activation [n][k]: per row and block of 32 columns one scale byte s and 32 codes; value = code * 2^(s - 127).  Signed: code in [-127, 127] (two's
 // complement), unsigned (what a ReLU leaves): [0, 255].  e = s - 127 is the smallest exponent >= -126 with max|x| <= 127 * 2^e (255 * 2^e), so the codes use 6.98 to
 // 7.98 bits of the block's largest entry and an entry is off by at most half a step of 2^e.  A power of two, not max / 255, so that a value has at most 8 significant bits:
-// it IS a bfloat16 (and, for an activation that was one, a float16), and the weight gradient's matrix products read it without another rounding.  A positive entry of an
+// it IS a bfloat16 (and, for an activation that was one, a float16: but for the upper ends of their ranges, see decode8_large), and the weight gradient's matrix products read it without
+// another rounding.  A positive entry of an
 // unsigned checkpoint keeps at least code 1 (off by less than one step instead of half): "code is not zero" is then exactly "the ReLU was open", and no mask is stored.
 // A block with a non-finite entry has scale byte 255 and codes 1: all its values are NaN, and its ReLUs count as open.  Rows are padded to 32 columns with zeros.
 //
@@ -164,8 +165,8 @@ template <int T> __device__ __forceinline__ void encode8(const Raw8<T>& v, bool 
     scale = s.scale;
 }
 
-// the eight values behind codes: (u - off) * step in one exact fused multiply-add (u the code byte, its top bit flipped where signed); scale byte 255 makes step infinite
-// and every value NaN
+// the eight values behind codes: (u - off) * step in one exact fused multiply-add (u the code byte, its top bit flipped where signed); scale byte 255 makes step infinite and every
+// value NaN.  Not for the blocks of large_block
 __device__ __forceinline__ void decode8(u32x2 codes, unsigned scale, bool is_signed, float (&f)[8]) {
     const float step = as_float(scale << 23);
     const unsigned flip = is_signed ? 0x80808080u : 0u;
@@ -174,6 +175,23 @@ __device__ __forceinline__ void decode8(u32x2 codes, unsigned scale, bool is_sig
     for (int i = 0; i < 8; ++i) {
         const unsigned u = ((codes[i >> 2] ^ flip) >> (8 * (i & 3))) & 255u;
         f[i] = __builtin_fmaf((float)u, step, off);
+    }
+}
+// The upper end of T's range.  An entry may be coded as one step beyond it: 2^128 (float32, bfloat16: read as 255 * 2^120, bfloat16's largest) or 65536 (float16: read as
+// 65504), so that a finite activation stays finite; and from step 2^121 on decode8's offset, 128 * step, is beyond float32: here the difference comes first.  Blocks whose values
+// stay below 2^16 or 2^128 are none of these.
+template <int T> __device__ __forceinline__ bool large_block(unsigned scale) {
+    constexpr unsigned FIRST = T == LT_F16 ? 127 + 9 : 127 + 121;      // 128 steps of 2^9 are 65536, of 2^121 are 2^128
+    return scale - FIRST < 255 - FIRST;
+}
+template <int T> __device__ __forceinline__ void decode8_large(u32x2 codes, unsigned scale, bool is_signed, float (&f)[8]) {
+    asm volatile("" : "+v"(codes));      // (shared with decode8, the converted codes stay in registers across the branch: the widest weight tiles spill)
+    const float step = as_float(scale << 23), most = T == LT_F16 ? 65504.0f : 0x1.fep+127f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const unsigned u = (codes[i >> 2] >> (8 * (i & 3))) & 255u;
+        const float v = (float)(is_signed ? (int)(signed char)u : (int)u) * step;
+        f[i] = T == LT_F16 && __builtin_fabsf(v) != 65536.0f ? v : __builtin_amdgcn_fmed3f(v, -most, most);
     }
 }
 
@@ -870,13 +888,21 @@ template <int T, int WO, int WK> __device__ __forceinline__ void dense_weights_t
             stage8<T>(zt + across<WO>(zrow + RPZ * i, (t % RTZ) >> 2) + 8 * (t & 3), ZPLANE, zr[i]);
         }
         if (i < NX) {
+            unsigned short* to = zt + PARTS * ZPLANE + across<WK>(xrow + RPX * i, (t % RTX) >> 2) + 8 * (t & 3);
+            auto put = [&](const float (&f)[8]) {
+                u32x4 v;
+#pragma unroll
+                for (int e = 0; e < 4; ++e)      // a value has at most 8 significant bits: its upper 16 bits are all of it
+                    v[e] = T == LT_F16 ? pack2<LT_F16>(f[2 * e], f[2 * e + 1]) : __builtin_amdgcn_perm(as_bits(f[2 * e + 1]), as_bits(f[2 * e]), 0x07060302u);
+                *reinterpret_cast<u32x4*>(to) = v;
+            };
             float f[8];
             decode8(xc[i], xs[i], a.x.is_signed != 0, f);
-            u32x4 v;
-#pragma unroll
-            for (int e = 0; e < 4; ++e)      // a value has at most 8 significant bits: its upper 16 bits are all of it
-                v[e] = T == LT_F16 ? pack2<LT_F16>(f[2 * e], f[2 * e + 1]) : __builtin_amdgcn_perm(as_bits(f[2 * e + 1]), as_bits(f[2 * e]), 0x07060302u);
-            *reinterpret_cast<u32x4*>(zt + PARTS * ZPLANE + across<WK>(xrow + RPX * i, (t % RTX) >> 2) + 8 * (t & 3)) = v;
+            put(f);
+            if (__builtin_expect(large_block<T>(xs[i]), 0)) {      // written again, out of the way: 786 432 x 512 float16 takes 5 % longer where the compiler weighs both alike
+                decode8_large<T>(xc[i], xs[i], a.x.is_signed != 0, f);
+                put(f);
+            }
         }
     };
 
@@ -1105,7 +1131,10 @@ template <int T> __global__ __launch_bounds__(256) void k_checkpoint_values(Chec
         const int c = 8 * (int)(i - p * cpr);
         if (c >= k) continue;
         float f[8];
-        decode8(*reinterpret_cast<const u32x2*>(a.codes + 8 * i), a.scales[i >> 2], a.is_signed != 0, f);
+        const u32x2 codes = *reinterpret_cast<const u32x2*>(a.codes + 8 * i);
+        const unsigned scale = a.scales[i >> 2];
+        if (large_block<T>(scale)) decode8_large<T>(codes, scale, a.is_signed != 0, f);
+        else decode8(codes, scale, a.is_signed != 0, f);
         store8<T>(out + p * ld * Bytes<T>::v, c, k, from_floats<T>(f));
     }
 }

@@ -102,7 +102,8 @@ class Checkpoint:
         return self.codes.shape[0]
 
     def values(self, dtype=torch.float32):
-        """The values the checkpoint stands for, [n, columns]: exact in float32 and bfloat16 (at most 8 significant bits)."""
+        """The values the checkpoint stands for, [n, columns]: exact in float32 and bfloat16 (at most 8 significant bits; 2^128, which an entry beyond 3.37e38 may round up
+        to, as 3.39e38, and 65536 in float16 as 65504)."""
         out = self.codes.new_empty((self.codes.shape[0], self.columns), dtype=dtype)
         t = _type(out, "the values")
         lib, stream, guard = _on(out)

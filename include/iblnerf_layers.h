@@ -28,7 +28,8 @@ const char* iblnerf_layers_last_error(void);
 /* Checkpoint of an activation x [n, k]: d_codes [n, 32 kb] bytes, d_scales [n, kb] bytes, kb = ceil(k / 32).  Per row and block of 32 columns value = code * 2^(scale - 127):
  * signed codes (two's complement) in [-127, 127], unsigned ones (is_signed = 0; negative entries become 0) in [0, 255]; the exponent is the smallest >= -126 that holds the
  * block's largest entry, codes are rounded to nearest (ties to even), a positive entry of an unsigned checkpoint keeps at least code 1.  Columns beyond k are coded 0.  A block
- * with an infinity or NaN has scale 255 and codes 1: its values are NaN. */
+ * with an infinity or NaN has scale 255 and codes 1: its values are NaN.  A finite entry stays finite: what rounds up to one step beyond its type (2^128, or 65536 from float16) is
+ * read as 255 * 2^120, or as 65504 where float16 is read. */
 int iblnerf_checkpoint(void* stream, int dtype, const void* d_x, int64_t ld_x, int64_t n, int k, int is_signed, uint8_t* d_codes, uint8_t* d_scales);
 int iblnerf_checkpoint_values(void* stream, const uint8_t* d_codes, const uint8_t* d_scales, int64_t n, int k, int is_signed, int dtype, void* d_out, int64_t ld_out);
 
@@ -43,7 +44,7 @@ int iblnerf_dense_forward(void* stream, int dtype, const void* d_x, int64_t ld_x
  *   dZ = dY where the output's code is not 0 (elsewhere 0, whatever dY holds there);  dX [n, k] = dZ w;  dW [o, k] = dZ^T X;  db [o] = sum over the rows of dZ
  * d_dx may be NULL, d_dw and d_db may be NULL together, d_db alone may be.  d_dw and d_db are contiguous and written, not accumulated, in grad_dtype: dtype itself, or
  * IBLNERF_FLOAT32 for parameters that are kept in float32 beside 16-bit activations.  For float16 a checkpoint of float16
- * activations is read exactly; values of another origin are rounded to float16. */
+ * activations is read exactly (65536 as 65504); values of another origin are rounded to float16. */
 size_t iblnerf_dense_backward_workspace(int dtype, int64_t n, int k, int o);
 int iblnerf_dense_backward(void* stream, int dtype, const void* d_dy, int64_t ld_dy, int64_t n, int k, int o, const uint8_t* d_x_codes, const uint8_t* d_x_scales, int x_is_signed,
                            const uint8_t* d_y_codes, const void* d_w, int64_t ld_w, void* d_dx, int64_t ld_dx, int grad_dtype, void* d_dw, void* d_db, void* d_workspace,

@@ -1,0 +1,80 @@
+"""Checkpoints at the upper end of their types' ranges: what a finite activation's codes stand for is finite, and the weight gradient reads just that."""
+import pytest
+import torch
+
+import _pkg
+import layers_ref as R
+
+pytestmark = pytest.mark.gpu
+L = _pkg.load().layers
+DEV = "cuda"
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+MOST = {torch.float32: 255 * 2.0 ** 120, torch.bfloat16: 255 * 2.0 ** 120, torch.float16: 65504.0}
+
+
+def read_as(kept, dtype):
+    """The definition's values in `dtype`: one step beyond the type's range is the type's largest (bfloat16's for float32, whose products take a checkpoint's value as one)."""
+    v = R.stored(kept)
+    beyond = 65536.0 if dtype == torch.float16 else 2.0 ** 128
+    return torch.where(v.abs() == beyond, v.sign() * MOST[dtype], v).to(dtype)
+
+
+def large_rows(dtype, signed):
+    """a block of small and large entries of both signs for each of these maxima"""
+    top = torch.finfo(dtype).max
+    tops = [top, top * (1 - 2.0 ** -7), 65280.0, 65296.0, 65504.0, 65024.0, 65056.0, 32512.0, 32768.0, 512.0]
+    if dtype != torch.float16:
+        tops += [1.8e38, 1.6e38, 127 * 2.0 ** 120, 128 * 2.0 ** 120, 127 * 2.0 ** 121, 254.5 * 2.0 ** 120, 255 * 2.0 ** 120, 2.0 ** 126, 1e38, 70000.0]
+    g = torch.Generator().manual_seed(6)
+    x = torch.empty((len(tops), 40), dtype=torch.float64)
+    for i, m in enumerate(tops):
+        x[i] = m * (torch.rand(40, generator=g, dtype=torch.float64) * 2 - 1)
+        x[i, 3], x[i, 5], x[i, 7], x[i, 35] = m, -m, 0.0, m
+    x = x.clamp(-top, top).to(dtype)
+    return x if signed else x.clamp_min(0)
+
+
+@pytest.mark.parametrize("signed", [True, False])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_values_of_large_blocks(dtype, signed):
+    x = large_rows(dtype, signed)
+    kept = L.checkpoint(x.to(DEV), signed=signed)
+    c, e = R.pack(x, signed)
+    got_c, got_e = R.raw(kept)
+    assert (got_c == c).all() and (got_e == e).all()
+    for t in TYPES:
+        got, want = kept.values(t).cpu(), read_as(kept, t)
+        assert torch.equal(got, want)
+        if t != torch.float16 or dtype == torch.float16:
+            assert torch.isfinite(got).all()
+    # half a step; a positive entry of an unsigned checkpoint that keeps code 1: a step
+    step, one = torch.from_numpy(2.0 ** e).repeat_interleave(32, 1)[:, :40], torch.from_numpy(c == 1)[:, :40]
+    assert ((kept.values(dtype).double().cpu() - x.double()).abs() <= torch.where(one & (not signed), step, step / 2)).all()
+
+
+@pytest.mark.parametrize("signed", [True, False])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,o", [(1, 1), (1, 40), (3, 200), (66000, 3), (66000, 200)])
+def test_weight_gradient_of_large_blocks(n, o, dtype, signed):
+    """one row of dY is 1, the others 0: dW is that row's values, with no rounding (a tile of every width; 66 000 rows of 216 or more columns: the widest)"""
+    rows = large_rows(dtype, signed)
+    wide = torch.cat([rows, torch.zeros(rows.shape[0], 24, dtype=dtype)], 1)                  # [., 64]
+    for r0 in range(0, rows.shape[0], 4):
+        x = wide[r0:r0 + 4].reshape(1, -1)                                                    # up to 256 columns
+        k = x.shape[1]
+        kept = L.checkpoint(x.to(DEV), signed=signed)
+        codes, scales = torch.zeros(n, kept.codes.shape[1], dtype=torch.uint8, device=DEV), torch.full((n, kept.scales.shape[1]), 127, dtype=torch.uint8, device=DEV)
+        codes[-1], scales[-1] = kept.codes[0], kept.scales[0]
+        dy = torch.zeros(n, o, dtype=dtype, device=DEV)
+        dy[-1] = 1
+        _, dw, db = L.dense_backward(dy, L.Checkpoint(codes, scales, k, signed), torch.zeros(o, k, dtype=dtype, device=DEV), need_dx=False, grad_dtype=torch.float32)
+        want = read_as(kept, dtype).float()
+        assert torch.equal(dw.cpu(), want.expand(o, k)) and (db == 1).all()
+
+
+def test_a_bad_block_is_nan_beside_large_ones():
+    x = torch.full((2, 64), 3e38, device=DEV)
+    x[1, 40] = float("inf")
+    for signed in (True, False):
+        v = L.checkpoint(x, signed=signed).values()
+        assert torch.isfinite(v[0]).all() and torch.isfinite(v[1, :32]).all() and torch.isnan(v[1, 32:]).all()
