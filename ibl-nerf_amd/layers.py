@@ -407,11 +407,25 @@ def network_query(inputs, viewdirs, network_fn, codes=None, views=None, code_sca
     return torch.cat(out, -1).reshape(lead + (18,))
 
 
-def network_gradients(inputs, viewdirs, draw, network_fn, dtype=None, points=1 << 20):
-    """{parameter name: dL/d parameter} of network_query from dL/d raw (draw [n, S, 18]), `points` samples at a time (14 checkpoints of a 512-wide network: 7 KB a sample)."""
+GRADIENT_BYTES = 24 << 30      # what a piece of network_gradients may take beside the batch (of the card's 288 GB)
+
+
+def gradient_points(params):
+    """Samples that network_gradients takes at a time, at most 2^20: a sample holds a checkpoint of each layer's output and of the three inputs that no layer wrote (33 / 32 bytes a
+    column), and beside them at most six float32 rows of the widest layer are alive (an activation and its gradient, the sum of the branches' gradients and the term being
+    added, a concatenation and its parts)."""
+    sides = {k[:-len(".weight")]: tuple(w.shape) for k, w in params.items() if k.endswith(".weight")}
+    made = [o for o, _ in sides.values()] + [sides[k][1] for k in ("positions_linears.0", "positions_linears.5", "views_linears.0") if k in sides]
+    a_sample = sum((c + 31) // 32 * 33 for c in made) + 6 * 4 * max(max(s) for s in sides.values())
+    return max(1, min(1 << 20, GRADIENT_BYTES // a_sample))
+
+
+def network_gradients(inputs, viewdirs, draw, network_fn, dtype=None, points=None):
+    """{parameter name: dL/d parameter} of network_query from dL/d raw (draw [n, S, 18]), `points` samples at a time (None: gradient_points, by the network's widths), whole rays."""
     dtype = dtype or getattr(network_fn, "layer_dtype", None)
     named = dict(network_fn.named_parameters())
     names, params = list(named), list(named.values())
+    points = points or gradient_points(named)
     total = None
     step = max(1, points // max(1, inputs.shape[1]))
     for i in range(0, inputs.shape[0], step):

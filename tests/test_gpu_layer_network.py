@@ -375,3 +375,21 @@ def test_captured_training_of_a_network():
         with torch.cuda.graph(torch.cuda.CUDAGraph()):
             M.fused_network_query(pts, dirs, net)
     del alive
+
+
+def test_memory_of_a_wide_networks_gradients(monkeypatch):
+    """a batch of several pieces takes a piece's memory (a sample's bytes: layers.gradient_points) and the parameters' gradients: two pieces' and the running total, and the weights in the products' type"""
+    arch = (6, 1024, 10, 4)
+    net = RefShaped(ck.synthetic_arch_state_dict(9, arch), arch).cuda()
+    monkeypatch.setattr(layers, "GRADIENT_BYTES", 1 << 30)
+    piece = layers.gradient_points(dict(net.named_parameters()))
+    n = 4 * piece // 64
+    g = torch.Generator(device="cuda").manual_seed(2)
+    pts, dirs, draw = torch.rand(n, 64, 3, generator=g, device="cuda"), torch.randn(n, 3, generator=g, device="cuda"), torch.randn(n, 64, 18, generator=g, device="cuda")
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    layers.network_gradients(pts, dirs, draw, net)
+    parameters = sum(4 * p.numel() for p in net.parameters())
+    workspaces = 64 << 20          # (the weight gradient's pieces: up to 512 / tiles of a layer's float32 weights, a few MB each)
+    assert torch.cuda.max_memory_allocated() - before <= (1 << 30) + 4 * parameters + workspaces

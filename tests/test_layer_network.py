@@ -125,3 +125,15 @@ def test_an_eager_graph_signs_its_leaves():
     z = w * 2
     layers._leaves(w, capturing=True)                           # a graph made within the capture is no eager one
     del z
+
+
+def test_pieces_of_the_gradients_go_by_the_widths():
+    """the 512-wide network keeps its 2^20 samples a piece; the widest one that trains takes what fits the same memory"""
+    def shapes(arch):
+        return {n + ".weight": torch.empty(o, i, device="meta") for n, o, i in ck.arch_schema(*arch)}
+    assert layers.gradient_points(shapes((8, 512, 10, 4))) == 1 << 20 and layers.gradient_points(shapes((9, 256, 10, 4))) == 1 << 20
+    for arch in ((8, 1024, 10, 4), (32, 512, 10, 4), (32, 4096, 24, 24)):
+        held = sum(33 / 32 * o for _, o, _ in ck.arch_schema(*arch))
+        n = layers.gradient_points(shapes(arch))
+        assert 1000 < n < 1 << 20 and n * (held + 4 * 4 * arch[1]) < layers.GRADIENT_BYTES
+    assert layers.gradient_points(shapes((32, 4096, 24, 24))) > 80000
