@@ -18,6 +18,7 @@ import contextlib
 import torch
 
 from . import binding as B
+from . import checkpoint as ck
 
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 MAX_COLUMNS, MAX_STRIDE = 65536, 1 << 24
@@ -343,10 +344,36 @@ def _linear(params, name):
     return params[name + ".weight"], params[name + ".bias"]
 
 
+def _network(params, n_code, whole):
+    """(depth, width, frequencies of the points, of the directions) behind a network's parameters, n_code columns of views_linears.0 being a view's code; whole=False: the trunk and the
+    density alone.  What no other path of the framework takes is refused here too: the module's own forward fails for 5 layers (the skip's concatenation is consumed by none),
+    and layers beyond the reference's would not be run."""
+    shapes = {k[:-len(".weight")]: tuple(w.shape) for k, w in params.items() if k.endswith(".weight")}
+    width, ch = shapes["positions_linears.0"]
+    depth = 1 + max(int(k.split(".")[1]) for k in shapes if k.startswith("positions_linears."))
+    chv = 3
+    if whole:
+        columns = shapes["views_linears.0"][1]
+        chv = columns - width - n_code
+        if chv < 3 or (chv - 3) % 6:
+            raise ValueError("views_linears.0 takes %d columns: %d features, %d code columns and no positional encoding's width beside them" % (columns, width, n_code))
+    if ch < 3 or (ch - 3) % 6:
+        raise ValueError("positions_linears.0 takes %d columns, no positional encoding's width" % ch)
+    arch = (depth, width, (ch - 3) // 6, (chv - 3) // 6)
+    if not (ck.is_member_of_built(arch) or ck.is_generic_arch(arch)):
+        raise NotImplementedError("IBLNeRF%s is outside what is built (netdepth <= 32 and != 5, netwidth <= 256 or even and <= 4096, multires, multires_views <= 24)" % (arch,))
+    want = {n: (o, i + (n_code if n == "views_linears.0" else 0)) for n, o, i in ck.arch_schema(*arch) if whole or n.startswith(("positions_linears.", "sigma_linear"))}
+    lists = ("positions_linears.",) + (("views_linears.", "additional_radiance_feature_linear.", "additional_radiance_linear.") if whole else ())
+    odd = sorted({n for n, s in want.items() if shapes.get(n) != s} | {n for n in shapes if n.startswith(lists) and n not in want})
+    if odd:
+        raise NotImplementedError("not the layers of IBLNeRF%s (skips = [4], coarse_radiance_number = 3): %s" % (arch, ", ".join("%s %s" % (n, shapes.get(n, "is missing")) for n in odd[:4])))
+    return arch
+
+
 def network_query(inputs, viewdirs, network_fn, codes=None, views=None, code_scale=1.0, dtype=None):
-    """IBLNeRF.forward (ibl_nerf.py:154-208) of a network of ANY depth and width, with autograd, on `dense`: inputs [..., 3] points, viewdirs [n, 3] one direction for each row
-    of points (or None: the density alone, :175-176), `network_fn` a torch module with the reference's parameter names -> raw [..., 18] float32 (or [..., 1]).  What is held for
-    the backward pass is one 8-bit checkpoint of each activation.
+    """IBLNeRF.forward (ibl_nerf.py:154-208) of any network that the framework renders (netdepth <= 32 and != 5, netwidth <= 4096), with autograd, on `dense`: inputs [..., 3] points,
+    viewdirs [n, 3] one direction for each row of points (or None: the density alone, :175-176), `network_fn` a torch module with the reference's parameter names -> raw
+    [..., 18] float32 (or [..., 1]).  What is held for the backward pass is one 8-bit checkpoint of each activation.
     codes [v, c] and views [n] (int): a code for each training view (photographs differ in exposure and white balance), code_scale * codes[view], beside the direction's
     encoding of every sample of the ray: views_linears.0 then takes c more columns (checkpoint.bake_view_code makes the network of one view for rendering); the codes
     receive their gradient by sorted views.  (Such a network queried without its codes is refused by its width, unless c is a multiple of 6: then its shapes are those of a
@@ -360,9 +387,9 @@ def network_query(inputs, viewdirs, network_fn, codes=None, views=None, code_sca
     if (codes is None) != (views is None):
         raise ValueError("codes and views come together")
     lead, flat = inputs.shape[:-1], inputs.reshape(-1, 3)
-    W, ch = params["positions_linears.0.weight"].shape
-    depth = 1 + max(int(k.split(".")[1]) for k in params if k.startswith("positions_linears."))
-    e = encode(flat, (ch - 3) // 6).to(dtype)
+    n_code = 0 if codes is None else codes.shape[1]
+    depth, _, freqs, freqs_views = _network(params, n_code, viewdirs is not None)
+    e = encode(flat, freqs).to(dtype)
     h, kept = dense(e, *_linear(params, "positions_linears.0"), relu=True)
     for i in range(1, depth):
         if i == 5:                                                              # cat([x, h]) behind layer 4 (:168)
@@ -391,12 +418,8 @@ def network_query(inputs, viewdirs, network_fn, codes=None, views=None, code_sca
     rays, samples = viewdirs.shape[0], flat.shape[0] // max(viewdirs.shape[0], 1)
     if rays * samples != flat.shape[0]:
         raise ValueError("%d points do not divide among %d directions" % (flat.shape[0], rays))
-    n_code = 0 if codes is None else codes.shape[1]
-    chv = params["views_linears.0.weight"].shape[1] - W - n_code
-    if chv < 3 or (chv - 3) % 6:
-        raise ValueError("views_linears.0 takes %d columns: %d features, %d code columns and no positional encoding's width beside them" % (params["views_linears.0.weight"].shape[1], W, n_code))
-    ev = encode(viewdirs.reshape(-1, 3).to(flat.dtype), (chv - 3) // 6).to(dtype)
-    parts = [feature, ev[:, None].expand(rays, samples, chv).reshape(-1, chv)]
+    ev = encode(viewdirs.reshape(-1, 3).to(flat.dtype), freqs_views).to(dtype)
+    parts = [feature, ev[:, None].expand(rays, samples, ev.shape[1]).reshape(-1, ev.shape[1])]
     if codes is not None:
         if views.numel() != rays:
             raise ValueError("views has %d entries for %d rays" % (views.numel(), rays))
