@@ -376,8 +376,8 @@ def network_query(inputs, viewdirs, network_fn, codes=None, views=None, code_sca
     [..., 18] float32 (or [..., 1]).  What is held for the backward pass is one 8-bit checkpoint of each activation.
     codes [v, c] and views [n] (int): a code for each training view (photographs differ in exposure and white balance), code_scale * codes[view], beside the direction's
     encoding of every sample of the ray: views_linears.0 then takes c more columns (checkpoint.bake_view_code makes the network of one view for rendering); the codes
-    receive their gradient by sorted views.  (Such a network queried without its codes is refused by its width, unless c is a multiple of 6: then its shapes are those of a
-    network with more frequencies.)
+    receive their gradient by sorted views.  c may be no multiple of 6 (ValueError): such a network's shapes would be those of one with more frequencies, and queried, loaded or
+    rendered without its codes it would be taken for that one; any other width is refused there.
     dtype: the type of the layers between the encodings and the heads (float32, bfloat16, float16: the last for a scaled loss); parameters stay what they are, heads are float32.
     None: what the module's attribute `layer_dtype` says, or float32."""
     dtype = dtype or getattr(network_fn, "layer_dtype", None) or torch.float32
@@ -388,6 +388,9 @@ def network_query(inputs, viewdirs, network_fn, codes=None, views=None, code_sca
         raise ValueError("codes and views come together")
     lead, flat = inputs.shape[:-1], inputs.reshape(-1, 3)
     n_code = 0 if codes is None else codes.shape[1]
+    if codes is not None and n_code % 6 == 0:
+        raise ValueError("codes of %d columns: a multiple of 6 looks like the encoding of %d more frequencies to whatever meets the network without its codes; take another width "
+                         "(one more column)" % (n_code, n_code // 6))
     depth, _, freqs, freqs_views = _network(params, n_code, viewdirs is not None)
     e = encode(flat, freqs).to(dtype)
     h, kept = dense(e, *_linear(params, "positions_linears.0"), relu=True)

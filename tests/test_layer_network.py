@@ -179,3 +179,22 @@ def test_refuses_layers_that_it_would_not_run(plain):
     assert layers.network_query(p, None, net(fourth)).shape == (2, 3, 1)                       # (the density has nothing to do with them)
     n = net(lambda n: n.register_parameter("my_codes", torch.nn.Parameter(torch.zeros(4, 5))))  # parameters that are no layer of the network stay out of its way
     assert layers.network_query(p, d, n).shape == (2, 3, 18)
+
+
+@pytest.mark.parametrize("c", [6, 12, 48])
+def test_a_codes_width_is_never_that_of_frequencies(plain, c):
+    """a network trained with codes of 6 m columns would be read as one of m more direction frequencies wherever it is met without them: not trained; any other width is refused there"""
+    arch = (6, 32, 4, 2)
+    p, d, views = torch.zeros(4, 3, 3), torch.ones(4, 3), torch.zeros(4, dtype=torch.int32)
+    net = RefShaped(arch=arch)
+    codes = with_codes(net, c, 2)
+    assert ck.arch_of(net.state_dict()) == (6, 32, 4, 2 + c // 6)
+    with pytest.raises(ValueError, match="multiple of 6"):
+        layers.network_query(p, d, net, codes=codes, views=views)
+    net = RefShaped(arch=arch)
+    codes = with_codes(net, c + 1, 2)
+    assert layers.network_query(p, d, net, codes=codes, views=views).shape == (4, 3, 18)
+    with pytest.raises(ValueError, match="columns"):
+        layers.network_query(p, d, net)
+    with pytest.raises(ValueError, match="encoding"):
+        ck.arch_of(net.state_dict())
