@@ -180,16 +180,36 @@ def layered(network_fn):
     return (ch - 3) % 6 == 0 and (chv - 3) % 6 == 0 and not ck.is_member_of_built((len(trunk), W, (ch - 3) // 6, (chv - 3) // 6)) and not _ci(network_fn)
 
 
+def _exact_query(inputs, viewdirs, network_fn):
+    """A query of a network outside the built shape that needs no gradient: the render path's, layer by layer in exact fp32 -> raw rows, or None where the query has to run in
+    layers.network_query (something requires a gradient, the module names a layer_dtype, or a graph is being captured: the render path may upload the weights first)."""
+    import torch
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (inputs, viewdirs, *network_fn.parameters())):
+        return None
+    if getattr(network_fn, "layer_dtype", None) is not None or (torch.cuda.is_available() and torch.cuda.is_current_stream_capturing()):
+        return None
+    r = _query_renderer(network_fn)
+    lead, points = inputs.shape[:-1], inputs.numel() // 3
+    rays = points if viewdirs is None else viewdirs.shape[0]
+    if rays == 0 or points % rays:
+        if points:
+            raise ValueError("%d points do not divide among %d directions" % (points, rays))
+        return torch.zeros(lead + (1 if viewdirs is None else 18,), dtype=torch.float32, device=r.device)
+    x = inputs if inputs.dim() == 3 and (viewdirs is None or inputs.shape[0] == rays) else inputs.reshape(rays, -1, 3)
+    return r.network_query(x, viewdirs, 0).reshape(lead + (1 if viewdirs is None else 18,))
+
+
 def fused_trunk_query(inputs, network_fn):
     """`network_query_fn(inputs, None, network_fn)` (the trunk-only query, ibl_nerf.py:175-176) WITH autograd, both directions on the
     fused kernels: forward = the trunk query, backward = iblnerf_trunk_backward (the forward is recomputed there with the pass bits
     kept, as under activation checkpointing), which hands dL/dinputs and the gradients of positions_linears.0-7 / sigma_linear back
     to torch.  `network_fn` is the torch module whose parameters carry those names (the reference's IBLNeRF).  First derivatives only.
-    A network outside the built shape runs layer by layer (layers.network_query)."""
+    A network outside the built shape runs layer by layer (layers.network_query; without a gradient as it renders)."""
     import torch
     if layered(network_fn):
         from . import layers
-        return layers.network_query(inputs, None, network_fn)
+        exact = _exact_query(inputs, None, network_fn)
+        return layers.network_query(inputs, None, network_fn) if exact is None else exact
     named = dict(network_fn.named_parameters())
     params = [named[k] for k in TRUNK_PARAMS]
 
@@ -267,10 +287,14 @@ def fused_network_query(inputs, viewdirs, network_fn, codes=None, views=None, co
     """`network_query_fn(inputs, viewdirs, network_fn)` WITH autograd, the whole network on the fused kernels in both directions: forward =
     the precise network query, backward = iblnerf_network_backward (dL/d raw rows in; dL/dinputs and all 46 parameter gradients out).
     A network outside the built shape, and any network with a code for each view (codes, views, code_scale: layers.network_query), runs layer by layer from 8-bit
-    checkpoints, its layers in layer_dtype (None: the module's attribute of that name, or float32; a training render takes the attribute)."""
+    checkpoints, its layers in layer_dtype (None: the module's attribute of that name, or float32; a training render takes the attribute).  Where nothing requires a gradient and no
+    type or code is asked for, it is evaluated as it renders, in exact fp32."""
     import torch
     if codes is not None or layer_dtype is not None or layered(network_fn):
         from . import layers
+        exact = _exact_query(inputs, viewdirs, network_fn) if codes is None and views is None and layer_dtype is None else None
+        if exact is not None:
+            return exact
         return layers.network_query(inputs, viewdirs, network_fn, codes=codes, views=views, code_scale=code_scale, dtype=layer_dtype)
     named = dict(network_fn.named_parameters())
     params = [named[k] for k in ALL_PARAMS]

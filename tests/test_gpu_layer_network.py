@@ -393,3 +393,29 @@ def test_memory_of_a_wide_networks_gradients(monkeypatch):
     parameters = sum(4 * p.numel() for p in net.parameters())
     workspaces = 64 << 20          # (the weight gradient's pieces: up to 512 / tiles of a layer's float32 weights, a few MB each)
     assert torch.cuda.max_memory_allocated() - before <= (1 << 30) + 4 * parameters + workspaces
+
+
+@pytest.mark.parametrize("arch", [(8, 264, 10, 4), (10, 258, 4, 2)])
+def test_queries_without_a_gradient_are_the_render_paths(arch):
+    """exact fp32, bit for bit what a render evaluates (and what these queries gave before they could be trained); a gradient, a type or a capture takes the trained layers"""
+    net = RefShaped(ck.synthetic_arch_state_dict(9, arch, 1.5), arch).cuda()
+    g = torch.Generator().manual_seed(2)
+    pts, dirs = (torch.rand(20, 8, 3, generator=g) - 0.5).cuda(), torch.randn(20, 3, generator=g).cuda()
+    want, sigma = M.network_query_fn(pts, dirs, net), M.network_query_fn(pts, None, net)
+    with torch.no_grad():
+        assert torch.equal(M.fused_network_query(pts, dirs, net), want) and torch.equal(M.fused_query(pts, dirs, net), want)
+        assert torch.equal(M.fused_trunk_query(pts, net), sigma) and torch.equal(M.fused_query(pts, None, net), sigma)
+        assert torch.equal(M.fused_trunk_query(pts.reshape(160, 3), net), sigma.reshape(160, 1))
+        assert torch.equal(M.fused_network_query(pts.reshape(160, 3), dirs, net), want.reshape(160, 18))
+        assert M.fused_network_query(pts[:0], dirs[:0], net).shape == (0, 8, 18) and M.fused_trunk_query(pts[:0], net).shape == (0, 8, 1)
+        with pytest.raises(ValueError, match="divide"):
+            M.fused_network_query(pts, dirs[:7], net)
+        low = M.fused_network_query(pts, dirs, net, layer_dtype=torch.bfloat16)
+    trained = M.fused_network_query(pts, dirs, net)
+    assert trained.requires_grad and not torch.equal(trained, want) and not torch.equal(low, want)
+    for p in net.parameters():
+        p.requires_grad_(False)
+    assert torch.equal(M.fused_network_query(pts, dirs, net), want)
+    assert M.fused_trunk_query(pts.clone().requires_grad_(True), net).requires_grad
+    net.layer_dtype = torch.bfloat16
+    assert torch.equal(M.fused_network_query(pts, dirs, net), low)
