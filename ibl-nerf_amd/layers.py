@@ -226,7 +226,8 @@ class _Dense(torch.autograd.Function):
         if x_codes is None:
             own = checkpoint(x)
             x_codes, x_scales, x_signed = own.codes, own.scales, True
-        ctx.relu, ctx.x_signed, ctx.has_bias, ctx.type, ctx.bias_dtype = relu, x_signed, bias is not None, x.dtype, None if bias is None else bias.dtype
+        ctx.relu, ctx.x_signed, ctx.has_bias, ctx.type = relu, x_signed, bias is not None, x.dtype
+        ctx.wide = any(t is not None and t.dtype not in (torch.bfloat16, torch.float16) for t in (weight, bias))      # (a gradient is cast to its parameter's type by autograd)
         ctx.save_for_backward(weight, x_codes, x_scales, *((kept.codes, kept.scales) if relu else ()))
         ctx.mark_non_differentiable(kept.codes, kept.scales)
         ctx.set_materialize_grads(False)                       # (or zeros of the codes' size would be written for them)
@@ -241,14 +242,14 @@ class _Dense(torch.autograd.Function):
         k, o = weight.shape[1], weight.shape[0]
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
         dx, dw, db = dense_backward(dy.to(ctx.type), Checkpoint(xc, xs, k, ctx.x_signed), weight.to(ctx.type), Checkpoint(*out, o) if ctx.relu else None, need_x, need_w, need_b and ctx.has_bias,
-                                    torch.float32 if weight.dtype == torch.float32 else None)
+                                    torch.float32 if ctx.wide else None)
         return dx, dw, db, None, None, None, None
 
 
 def dense(x, weight, bias=None, relu=False, kept=None):
     """dense_forward with autograd -> (y, Checkpoint of y).  kept: the Checkpoint of x that an earlier layer has written (None: one is made here, signed) — the backward pass
-    reads the checkpoints of x and, under a ReLU, of y, so neither tensor is held for it.  Parameters may be float32 beside 16-bit activations: they are cast for the
-    products, and their gradients are float32 sums.  First derivatives only.
+    reads the checkpoints of x and, under a ReLU, of y, so neither tensor is held for it.  Parameters may be float32 beside 16-bit activations (either of them): they are cast for
+    the products, and their gradients are float32 sums.  First derivatives only.
     A backward pass may be captured into a graph while no eager result of the same leaves is alive (RuntimeError otherwise)."""
     if kept is not None and (kept.columns != x.shape[-1] or kept.rows * kept.columns != x.numel()):
         raise ValueError("kept is a checkpoint of [%d, %d], x is %s" % (kept.rows, kept.columns, tuple(x.shape)))

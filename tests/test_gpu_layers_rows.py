@@ -109,3 +109,18 @@ def test_wide_layers(n, k, o, dtype):
     again = L.checkpoint(got, signed=False)
     assert torch.equal(kept.codes, again.codes) and torch.equal(kept.scales, again.scales)
     gradients(n, k, o, dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES[1:])
+@pytest.mark.parametrize("wide", ["weight", "bias", "both", "neither"])
+def test_gradients_of_wider_parameters_are_wide_sums(wide, dtype):
+    """a float32 weight or bias beside 16-bit activations gets a sum that 16 bits do not hold; a 16-bit one that sum rounded once"""
+    x, w, b, dy, _ = inputs(3001, 40, 33)
+    x, dy = x.abs() + 1, dy.abs() + 1          # (sums of 6 000 and 20 000)
+    w = w.to(torch.float32 if wide in ("weight", "both") else dtype).requires_grad_(True)
+    b = b.to(torch.float32 if wide in ("bias", "both") else dtype).requires_grad_(True)
+    y, _ = L.dense(x.to(dtype), w, b)
+    y.backward(dy.to(dtype))
+    for p, want in ((w, dy.t() @ x), (b, dy.sum(0))):
+        assert p.grad.dtype == p.dtype and torch.equal(p.grad, want.to(p.dtype))
+        assert not torch.equal(want, want.to(dtype).double())
