@@ -199,15 +199,22 @@ def dense_backward(dy, x, weight, relu=None, need_dx=True, need_dw=True, need_db
     return (dx if dx is None or len(lead) == 1 else dx.reshape(lead + (k,))), (dw if need_dw else None), db
 
 
+def _phase(like, capturing):
+    """(is a graph being captured, does an eager result made now stand in a capture's way: is the current stream the default one)"""
+    if capturing is None and like.is_cuda:
+        with _on(like)[2] or contextlib.nullcontext():
+            return torch.cuda.is_current_stream_capturing(), _raw_stream(like.get_device()) == 0
+    return capturing, True
+
+
 def _leaves(*tensors, capturing=None):
     """A leaf's gradient is accumulated on the stream of the first live graph that reads the leaf.  Under stream capture an EAGER graph of the default stream that still lives would
     pull that stream into the captured backward pass, where nothing can be reported and the process ends; so such graphs sign the accumulation node (it lives as long as
-    they do: called behind the operator that holds it), and a capture that meets the sign is refused."""
+    they do, or as what else holds it: called behind the operator that holds it), and a capture that meets the sign is refused."""
     leaves = [t for t in tensors if t is not None and t.requires_grad and t.is_leaf]
-    default = True
-    if capturing is None and leaves and leaves[0].is_cuda:
-        with _on(leaves[0])[2] or contextlib.nullcontext():
-            capturing, default = torch.cuda.is_current_stream_capturing(), _raw_stream(leaves[0].get_device()) == 0
+    if not leaves:
+        return
+    capturing, default = _phase(leaves[0], capturing)
     if not (capturing or default):
         return
     for t in leaves:
@@ -215,7 +222,20 @@ def _leaves(*tensors, capturing=None):
         if not capturing:
             sign["eager"] = True
         elif "eager" in sign:
-            raise RuntimeError("a graph is being captured while an eager result of the same leaf (%s) is alive: delete that result (or its loss) first" % (tuple(t.shape),))
+            raise RuntimeError("a graph is being captured while an eager result of the same leaf (%s) is alive, or something else that holds the leaf's gradient accumulator of the default "
+                               "stream (a hook on it, a distributed wrapper): delete that result (or its loss) first; make such a wrapper, and warm up, on a side stream" % (tuple(t.shape),))
+
+
+def sign(result, capturing=None):
+    """The same sign on the leaves that `result`, what an autograd Function has just given, was computed from (the framework's fused passes: their eager results stand in a captured
+    backward pass's way as a layer's do)."""
+    if result.grad_fn is None:
+        return
+    capturing, default = _phase(result, capturing)
+    if default and not capturing:
+        for node, _ in result.grad_fn.next_functions:
+            if hasattr(node, "variable"):
+                node.metadata["eager"] = True
 
 
 class _Dense(torch.autograd.Function):
@@ -250,7 +270,8 @@ def dense(x, weight, bias=None, relu=False, kept=None):
     """dense_forward with autograd -> (y, Checkpoint of y).  kept: the Checkpoint of x that an earlier layer has written (None: one is made here, signed) — the backward pass
     reads the checkpoints of x and, under a ReLU, of y, so neither tensor is held for it.  Parameters may be float32 beside 16-bit activations (either of them): they are cast for
     the products, and their gradients are float32 sums.  First derivatives only.
-    A backward pass may be captured into a graph while no eager result of the same leaves is alive (RuntimeError otherwise)."""
+    A backward pass may be captured into a graph while no eager result of the same leaves is alive (RuntimeError otherwise; results of torch's own operations on them are not seen
+    here, and end the process there)."""
     if kept is not None and (kept.columns != x.shape[-1] or kept.rows * kept.columns != x.numel()):
         raise ValueError("kept is a checkpoint of [%d, %d], x is %s" % (kept.rows, kept.columns, tuple(x.shape)))
     y, codes, scales = _Dense.apply(x, weight, bias, bool(relu), *((None, None, True) if kept is None else (kept.codes, kept.scales, kept.signed)))
@@ -409,7 +430,10 @@ def network_query(inputs, viewdirs, network_fn, codes=None, views=None, code_sca
         return y
 
     if viewdirs is None:
-        return head(h, ("sigma_linear",), kept).reshape(lead + (1,))
+        sigma = head(h, ("sigma_linear",), kept).reshape(lead + (1,))
+        if sigma.requires_grad:
+            _leaves(inputs)
+        return sigma
     sigma_rough = head(h, ("sigma_linear", "roughness_linear"), kept)
 
     def branch(x, kept_x, feature, out):
@@ -431,7 +455,10 @@ def network_query(inputs, viewdirs, network_fn, codes=None, views=None, code_sca
     h2, kept2 = dense(torch.cat(parts, -1), *_linear(params, "views_linears.0"), relu=True)
     out = [sigma_rough[:, :1], albedo, sigma_rough[:, 1:], irradiance, head(h2, ("radiance_linear",), kept2)]
     out += [branch(h2, kept2, "additional_radiance_feature_linear.%d" % k, "additional_radiance_linear.%d" % k) for k in range(3)]
-    return torch.cat(out, -1).reshape(lead + (18,))
+    raw = torch.cat(out, -1).reshape(lead + (18,))
+    if raw.requires_grad:
+        _leaves(inputs, viewdirs)
+    return raw
 
 
 GRADIENT_BYTES = 24 << 30      # what a piece of network_gradients may take beside the batch (of the card's 288 GB)

@@ -180,6 +180,13 @@ def layered(network_fn):
     return (ch - 3) % 6 == 0 and (chv - 3) % 6 == 0 and not ck.is_member_of_built((len(trunk), W, (ch - 3) // 6, (chv - 3) // 6)) and not _ci(network_fn)
 
 
+def _signed(result):
+    """What a fused pass has given, its leaves signed (layers.sign)."""
+    from . import layers
+    layers.sign(result[0] if isinstance(result, tuple) else result)
+    return result
+
+
 def _exact_query(inputs, viewdirs, network_fn):
     """A query of a network outside the built shape that needs no gradient: the render path's, layer by layer in exact fp32 -> raw rows, or None where the query has to run in
     layers.network_query (something requires a gradient, the module names a layer_dtype, or a graph is being captured: the render path may upload the weights first)."""
@@ -227,7 +234,7 @@ def fused_trunk_query(inputs, network_fn):
             return (dpts if ctx.needs_input_grad[0] else None,) + tuple(
                 grads[k].reshape(p.shape) if ctx.needs_input_grad[1 + i] else None for i, (k, p) in enumerate(zip(TRUNK_PARAMS, params)))
 
-    return _Fn.apply(inputs, *params)
+    return _signed(_Fn.apply(inputs, *params))
 
 
 def fused_trunk_features(inputs, network_fn):
@@ -251,7 +258,7 @@ def fused_trunk_features(inputs, network_fn):
             return (dpts if ctx.needs_input_grad[0] else None,) + tuple(
                 grads[k].reshape(p.shape) if ctx.needs_input_grad[1 + i] else None for i, (k, p) in enumerate(zip(names, params)))
 
-    return _Fn.apply(inputs, *params)
+    return _signed(_Fn.apply(inputs, *params))
 
 
 FEAT2_PARAMS = TRUNK_PARAMS[:16] + ("feature_linear.weight", "feature_linear.bias", "views_linears.0.weight", "views_linears.0.bias")
@@ -277,7 +284,7 @@ def fused_trunk_features2(inputs, viewdirs, network_fn):
             return (dpts if ctx.needs_input_grad[0] else None, None) + tuple(
                 grads[k].reshape(p.shape) if ctx.needs_input_grad[2 + i] else None for i, (k, p) in enumerate(zip(FEAT2_PARAMS, params)))
 
-    return _Fn.apply(inputs, viewdirs, *params)
+    return _signed(_Fn.apply(inputs, viewdirs, *params))
 
 
 ALL_PARAMS = tuple(n + s for n, _, _ in ck.SCHEMA for s in (".weight", ".bias"))
@@ -312,7 +319,7 @@ def fused_network_query(inputs, viewdirs, network_fn, codes=None, views=None, co
             return (dpts if ctx.needs_input_grad[0] else None, None) + tuple(
                 grads[k].reshape(p.shape) if ctx.needs_input_grad[2 + i] else None for i, (k, p) in enumerate(zip(ALL_PARAMS, params)))
 
-    return _Fn.apply(inputs, viewdirs, *params)
+    return _signed(_Fn.apply(inputs, viewdirs, *params))
 
 
 def fused_query(inputs, viewdirs, network_fn):

@@ -683,4 +683,6 @@ def render_rays_train(r, rays_o, rays_d, near, far, net_c, net_f, lut, *, approx
             return (None, None) + tuple(out)
 
     outs = _Fn.apply(ro, rd, *params, *aux_params)
+    from . import layers
+    layers.sign(next((o for o in outs if o.requires_grad), outs[0]))
     return dict(zip(keys, outs))

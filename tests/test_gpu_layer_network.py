@@ -419,3 +419,51 @@ def test_queries_without_a_gradient_are_the_render_paths(arch):
     assert M.fused_trunk_query(pts.clone().requires_grad_(True), net).requires_grad
     net.layer_dtype = torch.bfloat16
     assert torch.equal(M.fused_network_query(pts, dirs, net), low)
+
+
+def test_a_capture_meets_the_frameworks_own_eager_results(lut):
+    """A fused query's result and a training render's, eager and alive, stand in a captured training pass's way like a layer's: refused at the forward pass.  (No backward pass is
+    captured here; without the refusal one would end the process.)"""
+    from ibl_nerf_amd import renderer as R
+    built, larger = (8, 256, 10, 4), (2, 264, 4, 1)
+    net = RefShaped(ck.synthetic_arch_state_dict(9, built), built).cuda()
+    g = torch.Generator().manual_seed(2)
+    pts, dirs = torch.rand(16, 8, 3, generator=g).cuda(), torch.randn(16, 3, generator=g).cuda()
+
+    def refused(query):
+        with pytest.raises(RuntimeError, match="alive"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                query()
+
+    query = lambda: M.fused_network_query(pts, dirs, net, layer_dtype=torch.bfloat16)      # noqa: E731
+    query()
+    for eager in (lambda: M.fused_network_query(pts, dirs, net), lambda: M.fused_trunk_query(pts, net), lambda: M.fused_trunk_features(pts, net),
+                  lambda: M.fused_trunk_features2(pts, dirs, net)[1], lambda: M.fused_query(pts, dirs, net)):
+        alive = eager()
+        refused(query)
+        del alive
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            query()
+    nets = [RefShaped(ck.synthetic_arch_state_dict(s, larger, 1.5, sigma_bias=1.0), larger).cuda() for s in (1, 2)]
+    for n in nets:
+        n.coarse_radiance_number = 3
+    rays = torch.stack([torch.zeros(40, 3), torch.nn.functional.normalize(torch.randn(40, 3, generator=g), dim=-1)]).cuda()
+    kw = dict(network_fn=nets[0], network_fine=nets[1], N_samples=32, N_importance=32, perturb=0.0, brdf_lut=torch.from_numpy(lut).cuda(), lut_coefficient="F", gamma_correct=True,
+              use_radiance_linear=False, near=0.5, far=4.0)
+    query = lambda: M.fused_network_query(pts, dirs, nets[1])      # noqa: E731
+    query()
+    res = R.render_decomp(8, 12, np.eye(3, dtype=np.float32), rays=rays, gt_values={}, approximate_radiance=False, **kw)
+    loss = res["radiance_map"].sum()
+    del res
+    refused(query)
+    del loss
+    with torch.cuda.graph(torch.cuda.CUDAGraph()):
+        query()
+    moving = pts.clone().requires_grad_(True)
+    alive = M.fused_network_query(moving, dirs, nets[1])
+    for p in nets[1].parameters():
+        p.requires_grad_(False)
+    del alive
+    alive = M.fused_network_query(moving, dirs, nets[1])
+    refused(lambda: M.fused_network_query(moving, dirs, nets[1]))
+    del alive

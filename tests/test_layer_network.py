@@ -198,3 +198,49 @@ def test_a_codes_width_is_never_that_of_frequencies(plain, c):
         layers.network_query(p, d, net)
     with pytest.raises(ValueError, match="encoding"):
         ck.arch_of(net.state_dict())
+
+
+def test_a_functions_result_signs_its_leaves():
+    class Twice(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, x, w):
+            return 2 * w, 3 * w
+
+        @staticmethod
+        def backward(ctx, a, b):
+            return None, 2 * a + 3 * b
+
+    w, b, x = torch.nn.Parameter(torch.zeros(3)), torch.nn.Parameter(torch.zeros(3)), torch.zeros(3)
+    y = Twice.apply(x, w)
+    layers.sign(y[0], capturing=True)                           # made within a capture: nothing stands in its way
+    layers._leaves(w, capturing=True)
+    layers.sign(y[0], capturing=False)
+    with pytest.raises(RuntimeError, match="alive"):
+        layers._leaves(b, w, capturing=True)
+    layers._leaves(b, capturing=True)
+    del y
+    layers._leaves(w, capturing=True)
+    layers.sign(Twice.apply(x, x)[0], capturing=False)          # (nothing to differentiate)
+
+
+def test_what_holds_an_accumulator_is_named():
+    """a distributed wrapper or a hook keeps the node, and the sign, with no result alive: the refusal says so"""
+    w = torch.nn.Parameter(torch.zeros(3))
+    held = w.view_as(w).grad_fn.next_functions[0][0]
+    (w * 2).sum()
+    layers._leaves(w, capturing=False)
+    with pytest.raises(RuntimeError, match="wrapper.*side stream"):
+        layers._leaves(w, capturing=True)
+    del held
+    layers._leaves(w, capturing=True)
+
+
+def test_points_that_carry_a_gradient_are_signed(plain, monkeypatch):
+    seen = []
+    monkeypatch.setattr(layers, "_leaves", lambda *t, **k: seen.extend(t))
+    net, p, d = RefShaped(arch=(6, 32, 4, 2)), torch.zeros(4, 3, 3, requires_grad=True), torch.ones(4, 3, requires_grad=True)
+    layers.network_query(p, d, net)
+    assert any(t is p for t in seen) and any(t is d for t in seen)
+    seen.clear()
+    layers.network_query(p, None, net)
+    assert any(t is p for t in seen)
