@@ -467,3 +467,29 @@ def test_a_capture_meets_the_frameworks_own_eager_results(lut):
     alive = M.fused_network_query(moving, dirs, nets[1])
     refused(lambda: M.fused_network_query(moving, dirs, nets[1]))
     del alive
+
+
+def test_weights_changed_before_the_backward_pass_are_refused(lut):
+    """The layers' gradients come from a second forward pass on the module's parameters: an optimizer step between a render and its backward pass is an error, as it is in torch"""
+    from ibl_nerf_amd import renderer as R
+    arch = (2, 264, 4, 1)
+    nets = [RefShaped(ck.synthetic_arch_state_dict(s, arch, 1.5, sigma_bias=1.0), arch).cuda() for s in (1, 2)]
+    for n in nets:
+        n.coarse_radiance_number = 3
+    g = torch.Generator().manual_seed(2)
+    rays = torch.stack([torch.zeros(40, 3), torch.nn.functional.normalize(torch.randn(40, 3, generator=g), dim=-1)]).cuda()
+    kw = dict(network_fn=nets[0], network_fine=nets[1], N_samples=32, N_importance=32, perturb=0.0, brdf_lut=torch.from_numpy(lut).cuda(), lut_coefficient="F", gamma_correct=True,
+              use_radiance_linear=False, near=0.5, far=4.0)
+    params = [p for n in nets for p in n.parameters()]
+
+    def loss():
+        return (R.render_decomp(8, 12, np.eye(3, dtype=np.float32), rays=rays, gt_values={}, approximate_radiance=False, **kw)["radiance_map"] - 0.3).square().sum()
+    want = torch.autograd.grad(loss(), params, allow_unused=True)
+    first, second = loss(), loss()
+    got = torch.autograd.grad(first, params, allow_unused=True)
+    assert all((a is None) == (b is None) and (a is None or torch.equal(a, b)) for a, b in zip(got, want))
+    with torch.no_grad():
+        nets[1].positions_linears[0].weight.mul_(1.5)
+    with pytest.raises(RuntimeError, match="modified"):
+        torch.autograd.grad(second, params, allow_unused=True)
+    torch.autograd.grad(loss(), params, allow_unused=True)
