@@ -305,6 +305,10 @@ def _lookup(table, index, scale, rows_per_index, out):
         _same(out, table, "out", table.dtype)
         if out.dim() != 2 or tuple(out.shape) != (n * per, d) or (d > 1 and out.stride(1) != 1) or (out.shape[0] > 1 and not d <= out.stride(0) <= MAX_STRIDE):
             raise ValueError("out must be [%d, %d] with unit stride along a row, got %s strides %s" % (n * per, d, tuple(out.shape), tuple(out.stride())))
+        if out.requires_grad and torch.is_grad_enabled():
+            raise ValueError("out is written without autograd: it may not require a gradient")
+        if not out.is_inference():
+            torch.autograd.graph.increment_version(out)          # (what an earlier operation has kept of it for its backward pass is no longer what it read)
     ld_out = out.stride(0) if out.dim() == 2 and out.shape[0] > 1 else d
     _call(guard, lib.iblnerf_lookup, stream, t, tab.data_ptr(), ld, v, d, idx.data_ptr(), bits, n, per, float(scale), out.data_ptr(), ld_out)
     return out
@@ -343,7 +347,8 @@ class _Lookup(torch.autograd.Function):
 def lookup(table, index, scale=1.0, rows_per_index=1, out=None):
     """scale * table[index]: table [v, d], index [...] int32 or int64 -> [..., d]; rows_per_index > 1 repeats each row (a ray's code for each of its samples): the last axis of
     index grows by that factor.  A negative index is a row without a code (zeros, no gradient); one beyond the table reads NaN.  Differentiable in the table; `out`
-    ([n, d], rows may be strided: a slice of a wider input) is written instead of a new tensor, without autograd."""
+    ([n, d], rows may be strided: a slice of a wider input) is written instead of a new tensor, without autograd (an in-place write like torch's own: a backward pass that kept the
+    tensor before says so)."""
     if out is None and torch.is_grad_enabled() and table.requires_grad:
         rows = _Lookup.apply(table, index, float(scale), int(rows_per_index))
         _leaves(table)

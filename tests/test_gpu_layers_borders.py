@@ -78,3 +78,21 @@ def test_a_bad_block_is_nan_beside_large_ones():
     for signed in (True, False):
         v = L.checkpoint(x, signed=signed).values()
         assert torch.isfinite(v[0]).all() and torch.isfinite(v[1, :32]).all() and torch.isnan(v[1, 32:]).all()
+
+
+def test_a_written_slice_is_an_in_place_write():
+    """what an operation kept of a tensor for its backward pass is gone once codes are written into it: torch's own error, not the gradient of other numbers"""
+    table, index = torch.randn(5, 6, device=DEV), torch.tensor([1, 4, 0], device=DEV)
+    wide, w = torch.randn(3, 10, device=DEV), torch.randn(10, 4, device=DEV, requires_grad=True)
+    y = (wide @ w).sum()
+    L.lookup(table, index, out=wide[:, 4:])
+    assert torch.equal(wide[:, 4:], table[index])
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+    (wide @ w).sum().backward()
+    with pytest.raises(ValueError, match="require a gradient"):
+        L.lookup(table, index, out=torch.ones(3, 6, device=DEV) * w[0, 0])
+    with torch.no_grad():
+        L.lookup(table, index, out=torch.ones(3, 6, device=DEV) * w[0, 0])
+    with torch.inference_mode():
+        assert torch.equal(L.lookup(table, index, out=torch.empty(3, 6, device=DEV)), table[index])
