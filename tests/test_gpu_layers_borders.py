@@ -96,3 +96,40 @@ def test_a_written_slice_is_an_in_place_write():
         L.lookup(table, index, out=torch.ones(3, 6, device=DEV) * w[0, 0])
     with torch.inference_mode():
         assert torch.equal(L.lookup(table, index, out=torch.empty(3, 6, device=DEV)), table[index])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,k,o", [(70, 5, 3), (70, 40, 40), (130, 3, 200)])
+def test_the_longest_strides(dtype, n, k, o):
+    """rows 2^24 elements apart, the most that a call takes without a copy: a step's rows lie up to 4 GB apart"""
+    ld = L.MAX_STRIDE
+    room = torch.empty((n - 1) * ld + max(k, o), dtype=dtype, device=DEV)
+    g = torch.Generator(device=DEV)
+    g.manual_seed(n + k)
+
+    def far(rows, cols):
+        t = torch.as_strided(room, (rows, cols), (ld, 1))
+        t.copy_(torch.randint(-3, 4, (rows, cols), generator=g, device=DEV))
+        return t, t.clone().contiguous()
+    x, xc = far(n, k)
+    w = torch.randint(-3, 4, (o, k), generator=g, device=DEV).to(dtype)
+    kx = L.checkpoint(x)
+    assert torch.equal(kx.values(dtype), xc)
+    y, ky = L.dense_forward(x, w, relu=True)
+    assert torch.equal(y, (xc.double() @ w.double().t()).clamp_min(0).to(dtype))
+    index = torch.randint(0, n, (50,), generator=g, device=DEV)
+    assert torch.equal(L.lookup(x, index), xc[index])
+    far(n, k)                                    # (the room has been read)
+    L.lookup(xc, torch.arange(n, device=DEV), out=x)
+    assert torch.equal(x, xc)
+    dy, dyc = far(n, o)
+    dx, dw, db = L.dense_backward(dy, kx, w, relu=ky, grad_dtype=torch.float32)
+    dz = torch.where(y > 0, dyc, torch.zeros_like(dyc)).double()
+    assert torch.equal(dx, (dz @ w.double()).to(dtype)) and torch.equal(dw.double(), dz.t() @ xc.double()) and torch.equal(db.double(), dz.sum(0))
+    want = torch.zeros(9, o, dtype=torch.float64, device=DEV).index_add_(0, torch.arange(n, device=DEV) % 9, dyc.double())
+    assert torch.equal(L.lookup_backward(dy, torch.arange(n, device=DEV) % 9, 9), want.to(dtype))
+    if o <= n:                                   # (the room holds a weight too)
+        wf, wc = far(o, k)
+        y2, _ = L.dense_forward(xc, wf)
+        dx2, _, _ = L.dense_backward(dyc, kx, wf, need_dw=False, need_db=False)
+        assert torch.equal(y2, (xc.double() @ wc.double().t()).to(dtype)) and torch.equal(dx2, (dyc.double() @ wc.double()).to(dtype))
