@@ -273,8 +273,9 @@ template <bool DX, int TO, int TP> __device__ __forceinline__ void begin(f32x16 
 // ------------------------------------------------------------------------------------------------------------------------------ Y = act(A B + bias)
 // One workgroup = BP rows x BO outputs, 4 waves of (BP / 2) x (BO / 2); D[output][row] so that a lane's accumulators are runs of 4 outputs of ONE row.  The reduction runs
 // in steps of BK staged through LDS: the next step's elements travel into registers while this step's products run.
-// Neighbouring workgroups of one XCD take the output tiles of the same rows (the rows are read from HBM once and then from that XCD's L2).  float32 is bound by the six products:
-// 64 064 x 384 -> 384 121 us (156 TFLOP/s of float32, 936 of products; a library's float32 product of 786 432 rows reaches 132), its input gradient 125 for 65 536 rows.
+// Neighbouring workgroups of one XCD take the output tiles of the same rows (the rows are read from HBM once and then from that XCD's L2).  float32 is bound by the six products
+// and their operands' splitting and staging: 64 064 x 384 -> 384 121 us (156 TFLOP/s of float32, 936 of products: matrix cores busy 42 %, vector units 37 %; a library's largest
+// bfloat16 product reaches 1 155 to 1 320, its float32 product of 786 432 rows 132), its input gradient 126 for 65 536 rows.
 template <int T, bool DX, int BP, int BO>
 __global__ __launch_bounds__(256, 2) void k_dense_rows(DenseRows a) {
     constexpr int PARTS = T == LT_F32 ? 3 : 1, BK = T == LT_F32 ? 32 : 64;
@@ -677,12 +678,13 @@ template <int T, int MODE> __device__ __forceinline__ void write_rows64(const De
     }
 }
 
-// The 16-bit types' form for many rows.  What bounds it is HBM (a 512-wide layer: 2.5 KB a row against 0.5 MFLOP), then L2 (the weights are read once for each 128 rows) and the
-// address units (see write_rows64).  Two workgroups stay on each compute unit and flow through their work, 128 rows x 256 outputs at a time: while a piece of the rows
+// The 16-bit types' form for many rows.  No unit is full: for 786 432 x 512 -> 512 with the checkpoint the address units (see write_rows64) are busy 58 % of the time, the matrix cores
+// 29 %, HBM carries 3.0 TB/s, and the waves wait a third of their time (as the input gradient: 63 %, 32 %, 3.9 TB/s).  Two workgroups stay on each compute unit (one beyond 6 passes) and
+// flow through their work, 128 rows x 256 outputs at a time: while a piece of the rows
 // (128 x COLS columns) is multiplied out of one LDS buffer, the next one — the next work item's first, too — is on its way in registers, goes to the other buffer, and the
 // piece after that is asked for before results are written; the other workgroup multiplies meanwhile.  A wave takes 128 rows x 64 outputs, so a fragment of the rows is
 // read once from LDS for each wave, and a fragment of the weights once from L2 for the workgroup.  Items of the same rows are neighbours on one XCD.  COLS: 128, or 64 for
-// layers that read no more.  786 432 x 512 x 512 bfloat16: 690 us with the checkpoint (2.0 GB: 2.9 TB/s), 570 us without, 620 us as the input gradient.  Tried and slower:
+// layers that read no more.  786 432 x 512 x 512 bfloat16: 700 us with the checkpoint (2.1 GB: 3.0 TB/s), 570 us without, 630 us as the input gradient.  Tried and slower:
 // steps of 64 columns with one step under way (940 us); all columns of 64 rows at once, the weights read twice as often (750); weights kept in LDS and rows straight to
 // registers as operands (915: 16 bytes of 32 rows a load, address units full).
 template <int T, int MODE, int COLS>
@@ -821,8 +823,9 @@ __global__ __launch_bounds__(256, 2) void k_dense_tall(DenseRows a, const u32x4*
 // bits every time.
 //
 // 128 x 128: 4 waves of 64 x 64, two workgroups on a compute unit; 256 x 256: 16 waves, half as many reads of either operand; 32 on the side of a narrow layer: a wave has one
-// 32 x 32 tile, or a share of the rows of the only one.  786 432 x 512 -> 512 float16: 550 us (1.6 GB: 2.9 TB/s; 750 TFLOP/s), bound by the way through registers and LDS that
-// turns and decodes the operands; 65 536 x 384 float32 85 us; 196 608 x 512 -> 4 float32 52.
+// 32 x 32 tile, or a share of the rows of the only one.  786 432 x 512 -> 512 float16: 545 us (1.7 GB: 3.2 TB/s; 760 TFLOP/s), on the way through registers and LDS that
+// turns and decodes the operands (vector units busy 45 % of the time, address units 44 %, matrix cores 38 %, LDS 29 %; the waves wait 42 % of theirs); 65 536 x 384 float32 86 us (41, 29,
+// 27, 18); 196 608 x 512 -> 4 float32 52.
 template <int T, int WO, int WK> struct WeightsTile {
     static constexpr int NT = WO == 256 ? 1024 : 256, PARTS = T == LT_F32 ? 3 : 1, BR = T == LT_F32 && WO != 32 ? 32 : 64;
     static constexpr int ZPLANE = BR * WO, XPLANE = BR * WK, BUFFER = PARTS * ZPLANE + XPLANE;
@@ -1145,8 +1148,10 @@ long few_blocks(long n, int o) { return ((n + 31) / 32) * ((o + 31) / 32); }
 constexpr long FEW_BLOCKS = 1024;
 
 // Which form Y = act(A B + bias) runs in, and the fragments' memory.  For the 16-bit types, beyond few rows: the narrow form for at most 32 outputs (100 000 rows of 26 -> 18: 8 us, 30
-// in the tall form; of 500 -> 32: 34, 55; longer rows would take more LDS than leaves room for four workgroups), else the tall form once its tiles of 128 rows give every
-// compute unit one (rows of 8 elements at least: it reads whole chunks; and as long as the biases of all passes fit LDS beside the two buffers).  A pass makes 256 outputs.
+// in the tall form; of 500 -> 32: 34, 55; its weights leave room for four workgroups on a compute unit up to 352 columns and for three up to 512: 262 144 rows of 512 -> 32 66 us,
+// of 528 in the tall form 112), else the tall form once its tiles of 128 rows give every compute unit one (32 767 rows of 512 -> 512 in k_dense_rows 36 us, 32 768 here 30; rows of 8
+// elements at least: it reads whole chunks; up to 8 passes, whose biases lie in LDS beside the two buffers).  A pass makes 256 outputs.  (Beyond 6 passes the biases, for which the input
+// gradient keeps room too, leave a compute unit one workgroup: 65 536 x 512 bfloat16 -> 1 536 157 us, 1 537 229, 2 048 254, 2 049 in k_dense_rows 261.)
 struct RowsPlan { bool few, narrow, tall; int passes, steps; };
 RowsPlan rows_plan(int type, long n, int r, int o) {
     RowsPlan p{};

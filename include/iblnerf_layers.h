@@ -42,6 +42,7 @@ int iblnerf_dense_forward(void* stream, int dtype, const void* d_x, int64_t ld_x
 
 /* The backward of that layer from the checkpoint of its input (d_x_codes / d_x_scales, x_is_signed) and, under a ReLU, of its output (d_y_codes; NULL: no ReLU):
  *   dZ = dY where the output's code is not 0 (elsewhere 0, whatever dY holds there);  dX [n, k] = dZ w;  dW [o, k] = dZ^T X;  db [o] = sum over the rows of dZ
+ * (float32 by the forward's products: an entry of dZ or w that is infinite or beyond 3.39e38 gives NaN in dX and dW, and in db, which adds up the same parts.)
  * d_dx may be NULL, d_dw and d_db may be NULL together, d_db alone may be.  d_dw and d_db are contiguous and written, not accumulated, in grad_dtype: dtype itself, or
  * IBLNERF_FLOAT32 for parameters that are kept in float32 beside 16-bit activations.  For float16 a checkpoint of float16
  * activations is read exactly (65536 as 65504); values of another origin are rounded to float16. */
