@@ -9,7 +9,7 @@
 // A block with a non-finite entry has scale byte 255 and codes 1: all its values are NaN, and its ReLUs count as open.  Rows are padded to 32 columns with zeros.
 //
 // PRODUCTS.  16-bit types: one v_mfma_f32_32x32x16 per 32 x 32 x 16 block, fp32 accumulation, one rounding to the type at the end.  float32: every operand is cut
-// into three bfloat16 parts, each the rest rounded to nearest, x = h + l + r EXACTLY (8 + 8 + 8 bits), and the six products hh + hl + lh + ll + hr + rh are added up in the
+// into three bfloat16 parts, each the rest rounded to nearest, x = h + l + r EXACTLY (8 + 8 + 8 bits; below 2^-110 the last part is a multiple of 2^-133: off by up to 2^-134), and the six products hh + hl + lh + ll + hr + rh are added up in the
 // same fp32 accumulator: what is left out (lr + rl + rr) is at most 2^-24 of |x||w|, the size of fp32's own rounding of a product; six 16-bit products take 24 matrix-core
 // slots where the fp32 instruction takes 64.  (An infinity in a float32 operand, or a magnitude above bfloat16's largest, 3.39e38, comes out as NaN: its lower parts are
 // inf - inf.)  A checkpoint's value is one part by itself: three products.

@@ -34,8 +34,8 @@ int iblnerf_checkpoint(void* stream, int dtype, const void* d_x, int64_t ld_x, i
 int iblnerf_checkpoint_values(void* stream, const uint8_t* d_codes, const uint8_t* d_scales, int64_t n, int k, int is_signed, int dtype, void* d_out, int64_t ld_out);
 
 /* y [n, o] = x [n, k] w^T + bias (w [o, k] as nn.Linear holds it; bias [o] or NULL), negative values to 0 if relu; with d_codes / d_scales (both or neither) also y's
- * checkpoint, unsigned if relu, else signed.  float32 products are taken in six bfloat16 products of the operands' exact three-part splits (about fp32's own accuracy; an
- * operand that is infinite or beyond 3.39e38 gives NaN). */
+ * checkpoint, unsigned if relu, else signed.  float32 products are taken in six bfloat16 products of the operands' three-part splits, exact for magnitudes
+ * from 2^-110 on (about fp32's own accuracy; smaller operands are off by up to 2^-134, half of bfloat16's smallest step; one that is infinite or beyond 3.39e38 gives NaN). */
 size_t iblnerf_dense_forward_workspace(int dtype, int64_t n, int k, int o);
 int iblnerf_dense_forward(void* stream, int dtype, const void* d_x, int64_t ld_x, int64_t n, int k, const void* d_w, int64_t ld_w, int o, const void* d_bias, int relu,
                           void* d_y, int64_t ld_y, uint8_t* d_codes, uint8_t* d_scales, void* d_workspace, size_t workspace_bytes);

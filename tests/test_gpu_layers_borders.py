@@ -133,3 +133,23 @@ def test_the_longest_strides(dtype, n, k, o):
         y2, _ = L.dense_forward(xc, wf)
         dx2, _, _ = L.dense_backward(dyc, kx, wf, need_dw=False, need_db=False)
         assert torch.equal(y2, (xc.double() @ wc.double().t()).to(dtype)) and torch.equal(dx2, (dyc.double() @ wc.double()).to(dtype))
+
+
+@pytest.mark.parametrize("e", [-100, -110, -114, -120, -127, -135])
+def test_small_float32_operands(e):
+    """Of three bfloat16 parts the last is a multiple of 2^-133: an operand below 2^-110 is off by up to 2^-134, which its partners' magnitudes multiply; beside that the bound of any
+    other size (half a step of the result, 2^-23 of the magnitudes summed for each addition and product).  Subnormal parts are operands like any others."""
+    g = torch.Generator(device=DEV)
+    g.manual_seed(-e)
+    n, k, o = 70, 48, 40
+    x, w = torch.randn(n, k, generator=g, device=DEV) * 2.0 ** e, torch.randn(o, k, generator=g, device=DEV)
+    dy = torch.randn(n, o, generator=g, device=DEV) * 2.0 ** e
+    kept = L.checkpoint(torch.randn(n, k, generator=g, device=DEV))
+    y, _ = L.dense_forward(x, w, keep=False)
+    dx, dw, db = L.dense_backward(dy, kept, w)
+    xv = kept.values().double()
+    for got, a, b in ((y, x.double(), w.double().t()), (dx, dy.double(), w.double()), (dw, dy.double().t(), xv), (db[:, None], dy.double().t(), torch.ones(n, 1, dtype=torch.float64, device=DEV))):
+        want, size, lost = a @ b, a.abs() @ b.abs(), torch.ones_like(a) @ b.abs()
+        bound = 2.0 ** -24 * want.abs() + 2.0 ** -149 + (n + 8) * 2.0 ** -23 * size + 2.0 ** -134 * lost
+        assert ((got.double() - want).abs() <= bound * (1 + 2.0 ** -8)).all()
+    assert y.any() and dx.any() and dw.any()
