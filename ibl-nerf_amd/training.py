@@ -525,6 +525,9 @@ def render_rays_train(r, rays_o, rays_d, near, far, net_c, net_f, lut, *, approx
         order = order[:i_n] + ["inferred_normal_map"] + order[i_n:]
     keys = [k + s for s in ("", "0") for k in order] + ["z_std"]
 
+    again = [nm[k] for nm, ks, arch in zip(named, pnames, archs) if not ck.is_member_of_built(arch) for k in ks]      # parameters that the backward pass reads once more
+    versions = lambda: [0 if p_.is_inference() else p_._version for p_ in again]      # noqa: E731
+
     class _Fn(torch.autograd.Function):
         @staticmethod
         def forward(ctx, ro_, rd_, *ps):
@@ -544,7 +547,7 @@ def render_rays_train(r, rays_o, rays_d, near, far, net_c, net_f, lut, *, approx
             else:
                 res, sv = _forward_direct(r, st, ro_, rd_, near, far, t_rand, u, flags, noise, gt_const, rows)
             ctx.saved = dict(sv, ro=ro_, rd=rd_)
-            ctx.versions = [p_._version for p_ in ps]
+            ctx.versions = versions()
             if normal_on or (incident_gradient and approximate_radiance):
                 ctx.saved.update(tdepth=res["target_depth_map"].detach().clone(), tdepth0=res["target_depth_map0"].detach().clone())
             if incident_gradient and approximate_radiance:
@@ -573,8 +576,8 @@ def render_rays_train(r, rays_o, rays_d, near, far, net_c, net_f, lut, *, approx
         def backward(ctx, *gouts):
             sv = ctx.saved
             gout = dict(zip(keys, gouts))
-            if any(not ck.is_member_of_built(a) for a in archs) and ctx.versions != [p_._version for p_ in params + aux_params]:
-                # (layer by layer the backward pass evaluates the module's parameters again, as they are now: gradients at other weights than the render's)
+            if ctx.versions != versions():
+                # (layer by layer the backward pass evaluates the network on the module's parameters as they are now: gradients at other weights than the render's)
                 raise RuntimeError("a parameter of a network outside the built shape was modified in place between this render and its backward pass")
             grads_all, oks = [], []
             aux_grads = {name: None for name in aux_named}
